@@ -378,6 +378,128 @@ int ckv_copy_rows(void* dst, size_t dst_pitch, const void* src, size_t src_pitch
 int ckv_gather(const ckv_layer* layer, int32_t window, const int32_t* idx, int32_t kept, int32_t per_head,
                void* out_k, void* out_v, ckv_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Paged 8-bit decode cache (no reference counterpart: the reference appends to a 16-bit
+ * torch cache).  A layer's keys and values live in blocks of block_size tokens of a pool,
+ * as 8-bit codes with one fp32 scale per (block, KV head); value = code * scale.  Scales are
+ * powers of two: the smallest (2^-126 at least) with max |x| / scale <= 448 (e4m3) or 127
+ * (int8), or NaN when the block holds a NaN or an infinity.
+ * Slot of a token: block * block_size + its place in the block.
+ */
+enum ckv_cache_format { CKV_CACHE_E4M3 = 0, CKV_CACHE_INT8 = 1 };
+
+typedef struct ckv_cache {
+  void* k;                 /* codes: [num_blocks][num_kv_heads][block_size][head_dim], any strides */
+  void* v;
+  float* k_scale;          /* [num_blocks][num_kv_heads], contiguous */
+  float* v_scale;
+  int64_t k_block_stride, k_head_stride, k_tok_stride;   /* bytes, multiples of 16; head_dim contiguous */
+  int64_t v_block_stride, v_head_stride, v_tok_stride;
+  int32_t num_blocks, num_kv_heads;
+  int32_t block_size;      /* 16, 32, 64 or 128 */
+  int32_t head_dim;        /* 64 or 128 */
+  int32_t format;          /* enum ckv_cache_format */
+} ckv_cache;
+
+/* One step of the block tables, on the device.  Request r holds lens[r] tokens in the
+ * ceil(lens[r] / block_size) first blocks of tables[r] and gets new_tokens[r] more (0: none;
+ * negative: it ends and its blocks return).  free_list[0 .. free_count) is a stack: returned
+ * blocks go on top, requests in order; fresh blocks come off the top, requests in order.  A
+ * request that its table row cannot hold, or for which the stack (and those before it) leaves too
+ * few blocks, is refused: it gets nothing and keeps its length.
+ * Outputs: out_lens; out_free_count; out_cu [requests + 1], the tokens asked for before each
+ * request; per token t < total: out_slots (-1 for a refused request's tokens and for t past
+ * out_cu[requests]) and out_positions = place in the request + shift[r] (0 past the end);
+ * out_granted [requests].  out_lens may be lens and out_free_count may be free_count; called
+ * again on the same lens and free_count, the step gives the same outputs. */
+typedef struct ckv_table_step {
+  const int32_t* lens;
+  const int32_t* new_tokens;
+  const int32_t* shift;        /* per request, may be NULL: tokens evicted from it */
+  int32_t* tables;             /* [requests][table_width], rows table_stride apart */
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t* free_list;          /* [free_capacity] */
+  int32_t free_capacity;
+  const int32_t* free_count;
+  int32_t block_size;
+  int32_t requests;            /* at most 8192 */
+  int32_t total;               /* length of out_slots and out_positions */
+  int32_t* out_lens;
+  int32_t* out_free_count;
+  int32_t* out_cu;
+  int64_t* out_slots;
+  int64_t* out_positions;
+  int32_t* out_granted;
+} ckv_table_step;
+int ckv_block_tables(const ckv_table_step* step, ckv_stream_t stream);
+
+/* Rotary positions of queries and keys: pair i of a head turns by positions[t] * inv_freq[i]
+ * (pairs (x[i], x[i + rotary_dim / 2]), or (x[2i], x[2i + 1]) when interleaved), cosine and
+ * sine times factor; dimensions past rotary_dim pass through.  inverse: by the negative angle
+ * (the gradient).  Angles are reduced in 64 bits.  k may be NULL with k_heads 0; out_q / out_k
+ * may be q / k themselves, and may not overlap them otherwise.  Strides in elements. */
+typedef struct ckv_rotary_args {
+  const void* q;
+  int64_t q_tok_stride, q_head_stride;
+  const void* k;
+  int64_t k_tok_stride, k_head_stride;
+  void* out_q;
+  int64_t out_q_tok_stride, out_q_head_stride;
+  void* out_k;
+  int64_t out_k_tok_stride, out_k_head_stride;
+  const int64_t* positions;    /* [tokens] */
+  const double* inv_freq;      /* [rotary_dim / 2], radians per position */
+  float factor;
+  int32_t tokens, q_heads, k_heads, head_dim, rotary_dim;
+  int32_t dtype, interleaved, inverse;
+  int32_t heads_per_cta;       /* set by the library */
+} ckv_rotary_args;
+int ckv_rotary(const ckv_rotary_args* args, ckv_stream_t stream);
+
+/* Write token rows k, v [tokens][num_kv_heads][head_dim] (strides in elements) into their
+ * slots.  Tokens of one block stand next to one another in the list (as ckv_block_tables
+ * gives them); a slot outside the pool is no token; of a slot named twice in a row of such
+ * neighbours the last token stays.  Neighbours that include a block's first place begin the
+ * block anew; otherwise the block's other tokens stay, in the larger of its old and new scale. */
+int ckv_cache_write(const ckv_cache* cache, const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+                    int64_t v_tok_stride, int64_t v_head_stride, int32_t dtype, const int64_t* slots, int32_t tokens,
+                    ckv_stream_t stream);
+
+/* The values at `slots`, as contiguous [tokens][num_kv_heads][head_dim] rows; zeros for a slot
+ * outside the pool. */
+int ckv_cache_read(const ckv_cache* cache, void* k, void* v, int32_t dtype, const int64_t* slots, int32_t tokens,
+                   ckv_stream_t stream);
+
+/* Attention of each sequence's last query tokens over its cached tokens (their own keys
+ * among them).  Sequence r: query rows cu[r] .. cu[r + 1) of q (cu NULL: one row each,
+ * requests == tokens), lens[r] tokens in tables[r].  causal: query i of m sees the first
+ * lens[r] - m + i + 1 tokens; a row that sees none gives 0 and lse -inf.  Query head h reads KV
+ * head h / (q_heads / num_kv_heads).  lse (may be NULL): natural log of the sum of exponentials,
+ * [tokens][q_heads] fp32.  Rows of q past cu[requests] are left alone.  A table entry outside the
+ * pool reads as NaN.  Workspace: ckv_cache_attention_workspace bytes, 256-byte aligned. */
+typedef struct ckv_attention_args {
+  const void* q;
+  int64_t q_tok_stride, q_head_stride;       /* elements; rows 16-byte aligned */
+  void* out;
+  int64_t out_tok_stride, out_head_stride;
+  float* lse;
+  const int32_t* tables;
+  int64_t table_stride;
+  int32_t table_width;
+  const int32_t* lens;
+  const int32_t* cu;
+  int32_t requests, tokens;
+  int32_t max_q;               /* at least the most query tokens of a sequence */
+  int32_t q_heads;
+  int32_t causal;
+  float scale;
+  int32_t dtype;               /* of q and out */
+} ckv_attention_args;
+int ckv_cache_attention_workspace(int32_t head_dim, int32_t max_q, int32_t q_heads, int32_t num_kv_heads, size_t* bytes);
+int ckv_cache_attention(const ckv_cache* cache, const ckv_attention_args* args, void* workspace, size_t workspace_bytes,
+                        ckv_stream_t stream);
+
 /* Per-stage timing (no counterpart in the reference; for benchmarks): while
  * set, each ckv_score_evict call on this thread records events[0] before its
  * first kernel and events[i] after its i-th stage (window moments, pooling,

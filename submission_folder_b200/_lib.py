@@ -24,10 +24,12 @@ EXPORTED = (
     "ckv_window_pool", "ckv_choose_heads", "ckv_pool_rows_given", "ckv_graph_update", "ckv_circuit_walk",
     "ckv_pcg_seed", "ckv_spectral_scores", "ckv_combine_scores", "ckv_landmark_workspace_size",
     "ckv_landmark_walk", "ckv_influence_walk", "ckv_influence_walk_dense", "ckv_walk_workspace_size",
-    "ckv_rng_fill", "ckv_gather", "ckv_device_accessible", "ckv_copy_rows", "ckv_set_stage_events", "ckv_last_error_string",
-    "ckv_version",
+    "ckv_rng_fill", "ckv_gather", "ckv_device_accessible", "ckv_copy_rows", "ckv_block_tables", "ckv_rotary",
+    "ckv_cache_write", "ckv_cache_read", "ckv_cache_attention_workspace", "ckv_cache_attention", "ckv_set_stage_events",
+    "ckv_last_error_string", "ckv_version",
 )
 RNG_PHILOX, RNG_PCG = 0, 1
+CACHE_E4M3, CACHE_INT8 = 0, 1
 LANDMARK_POSITIONAL, LANDMARK_REACHABILITY, LANDMARK_ABSORBING = 0, 1, 2
 
 
@@ -91,6 +93,60 @@ class Outputs(ctypes.Structure):
     ]
 
 
+class Cache(ctypes.Structure):
+    """Mirror of ``struct ckv_cache``."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("k_block_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64), ("k_tok_stride", ctypes.c_int64),
+        ("v_block_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64), ("v_tok_stride", ctypes.c_int64),
+        ("num_blocks", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32), ("block_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("format", ctypes.c_int32),
+    ]
+
+
+class TableStep(ctypes.Structure):
+    """Mirror of ``struct ckv_table_step``."""
+
+    _fields_ = [
+        ("lens", ctypes.c_void_p), ("new_tokens", ctypes.c_void_p), ("shift", ctypes.c_void_p),
+        ("tables", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int32),
+        ("free_list", ctypes.c_void_p), ("free_capacity", ctypes.c_int32), ("free_count", ctypes.c_void_p),
+        ("block_size", ctypes.c_int32), ("requests", ctypes.c_int32), ("total", ctypes.c_int32),
+        ("out_lens", ctypes.c_void_p), ("out_free_count", ctypes.c_void_p), ("out_cu", ctypes.c_void_p),
+        ("out_slots", ctypes.c_void_p), ("out_positions", ctypes.c_void_p), ("out_granted", ctypes.c_void_p),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    """Mirror of ``struct ckv_rotary_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("q_tok_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("k", ctypes.c_void_p), ("k_tok_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+        ("out_q", ctypes.c_void_p), ("out_q_tok_stride", ctypes.c_int64), ("out_q_head_stride", ctypes.c_int64),
+        ("out_k", ctypes.c_void_p), ("out_k_tok_stride", ctypes.c_int64), ("out_k_head_stride", ctypes.c_int64),
+        ("positions", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p), ("factor", ctypes.c_float),
+        ("tokens", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32),
+        ("heads_per_cta", ctypes.c_int32),
+    ]
+
+
+class AttentionArgs(ctypes.Structure):
+    """Mirror of ``struct ckv_attention_args``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("q_tok_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("out_tok_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64),
+        ("lse", ctypes.c_void_p), ("tables", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+        ("table_width", ctypes.c_int32), ("lens", ctypes.c_void_p), ("cu", ctypes.c_void_p),
+        ("requests", ctypes.c_int32), ("tokens", ctypes.c_int32), ("max_q", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32), ("causal", ctypes.c_int32), ("scale", ctypes.c_float), ("dtype", ctypes.c_int32),
+    ]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -109,6 +165,7 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
             "`python -m submission_folder_b200.build` (nvcc, sm_100a)")
     lib = ctypes.CDLL(path)
     vp, sz, i32, f32, u64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32, ctypes.c_float, ctypes.c_uint64
+    i64 = ctypes.c_int64
     P, L, O = ctypes.POINTER(Params), ctypes.POINTER(Layer), ctypes.POINTER(Outputs)
     sig = {
         "ckv_default_params": (None, [P]),
@@ -140,6 +197,12 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         "ckv_gather": (i32, [L, i32, vp, i32, i32, vp, vp, vp]),
         "ckv_device_accessible": (i32, [vp, ctypes.POINTER(i32)]),
         "ckv_copy_rows": (i32, [vp, sz, vp, sz, sz, i32, vp]),
+        "ckv_block_tables": (i32, [ctypes.POINTER(TableStep), vp]),
+        "ckv_rotary": (i32, [ctypes.POINTER(RotaryArgs), vp]),
+        "ckv_cache_write": (i32, [ctypes.POINTER(Cache), vp, i64, i64, vp, i64, i64, i32, vp, i32, vp]),
+        "ckv_cache_read": (i32, [ctypes.POINTER(Cache), vp, vp, i32, vp, i32, vp]),
+        "ckv_cache_attention_workspace": (i32, [i32, i32, i32, i32, ctypes.POINTER(sz)]),
+        "ckv_cache_attention": (i32, [ctypes.POINTER(Cache), ctypes.POINTER(AttentionArgs), vp, sz, vp]),
         "ckv_set_stage_events": (i32, [ctypes.POINTER(vp), i32]),
         "ckv_last_error_string": (ctypes.c_char_p, []),
         "ckv_version": (ctypes.c_char_p, []),

@@ -11,6 +11,7 @@
 #include <string>
 #include <vector>
 
+#include "ckv_cache.h"
 #include "ckv_common.cuh"
 #include "ckv_gather.h"
 #include "ckv_monitor.h"
@@ -857,6 +858,121 @@ int ckv_device_accessible(const void* ptr, int32_t* accessible) {
   else if (at.type == cudaMemoryTypeHost)   // page-locked: mapped at the same address under UVA
     *accessible = at.devicePointer == ptr ? 1 : 0;
   return CKV_OK;
+}
+
+static bool aligned16(const void* p, int64_t s0, int64_t s1, int es) {
+  return (uintptr_t)p % 16 == 0 && (s0 * es) % 16 == 0 && (s1 * es) % 16 == 0;
+}
+static bool known_dtype(int dtype) { return dtype == CKV_BF16 || dtype == CKV_FP16 || dtype == CKV_FP32; }
+
+static int check_cache(const ckv_cache* c) {
+  if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return fail(CKV_ERR_ARG, "null cache pointer");
+  if (c->format != CKV_CACHE_E4M3 && c->format != CKV_CACHE_INT8)
+    return fail(CKV_ERR_DTYPE, "cache format must be e4m3 or int8");
+  if (c->head_dim != 64 && c->head_dim != 128) return fail(CKV_ERR_UNSUPPORTED, "cache head_dim must be 64 or 128");
+  if (c->block_size != 16 && c->block_size != 32 && c->block_size != 64 && c->block_size != 128)
+    return fail(CKV_ERR_UNSUPPORTED, "cache block_size must be 16, 32, 64 or 128");
+  if (c->num_blocks < 1 || c->num_kv_heads < 1 || c->num_kv_heads > 65535)
+    return fail(CKV_ERR_ARG, "cache needs at least one block and 1 to 65535 heads");
+  if (!aligned16(c->k, c->k_block_stride, c->k_head_stride, 1) || c->k_tok_stride % 16 ||
+      !aligned16(c->v, c->v_block_stride, c->v_head_stride, 1) || c->v_tok_stride % 16)
+    return fail(CKV_ERR_ARG, "cache pointers and strides must be multiples of 16 bytes");
+  return CKV_OK;
+}
+
+int ckv_block_tables(const ckv_table_step* s, ckv_stream_t stream) {
+  if (!s || !s->lens || !s->new_tokens || !s->tables || !s->free_list || !s->free_count || !s->out_lens ||
+      !s->out_free_count || !s->out_cu || !s->out_granted || (s->total > 0 && (!s->out_slots || !s->out_positions)))
+    return fail(CKV_ERR_ARG, "null argument");
+  if (s->requests < 1 || s->requests > kMaxRequests) return fail(CKV_ERR_ARG, "1 to 8192 requests");
+  if (s->total < 0 || s->table_width < 1 || s->table_stride < s->table_width || s->free_capacity < 0)
+    return fail(CKV_ERR_ARG, "bad table geometry");
+  if (s->block_size < 1) return fail(CKV_ERR_ARG, "block_size must be at least 1");
+  const cudaError_t e = launch_block_tables(*s, (cudaStream_t)stream);
+  return e == cudaSuccess ? CKV_OK : cuda_fail(e, "block tables");
+}
+
+int ckv_rotary(const ckv_rotary_args* a, ckv_stream_t stream) {
+  if (!a) return fail(CKV_ERR_ARG, "null argument");
+  if (!known_dtype(a->dtype)) return fail(CKV_ERR_DTYPE, "dtype must be bf16, fp16 or fp32");
+  if (a->tokens < 0 || a->q_heads < 1 || a->k_heads < 0 || a->q_heads + a->k_heads > 65535)
+    return fail(CKV_ERR_ARG, "bad token or head count");
+  if (a->rotary_dim < 2 || a->rotary_dim % 2 || a->rotary_dim > a->head_dim || a->head_dim > 1024)
+    return fail(CKV_ERR_ARG, "rotary_dim must be even, in [2, head_dim], with head_dim at most 1024");
+  if (a->tokens == 0) return CKV_OK;
+  if (!a->q || !a->out_q || !a->positions || !a->inv_freq || (a->k_heads > 0 && (!a->k || !a->out_k)))
+    return fail(CKV_ERR_ARG, "null argument");
+  const cudaError_t e = launch_rotary(*a, (cudaStream_t)stream);
+  return e == cudaSuccess ? CKV_OK : cuda_fail(e, "rotary");
+}
+
+static int cache_rows(const ckv_cache* c, void* k, int64_t kts, int64_t khs, void* v, int64_t vts, int64_t vhs, int dtype,
+                      const int64_t* slots, int32_t tokens, CacheRows* r) {
+  const int rc = check_cache(c);
+  if (rc) return rc;
+  if (!known_dtype(dtype)) return fail(CKV_ERR_DTYPE, "dtype must be bf16, fp16 or fp32");
+  if (tokens < 0 || (tokens > 0 && (!k || !v || !slots))) return fail(CKV_ERR_ARG, "null rows or slots");
+  const int es = dtype == CKV_FP32 ? 4 : 2;
+  if (!aligned16(k, kts, khs, es) || !aligned16(v, vts, vhs, es))
+    return fail(CKV_ERR_ARG, "row pointers and strides must be 16-byte aligned (contiguous head_dim rows)");
+  r->k = k; r->kts = kts; r->khs = khs; r->v = v; r->vts = vts; r->vhs = vhs;
+  r->dtype = dtype; r->slots = slots; r->tokens = tokens;
+  return CKV_OK;
+}
+
+int ckv_cache_write(const ckv_cache* cache, const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v,
+                    int64_t v_tok_stride, int64_t v_head_stride, int32_t dtype, const int64_t* slots, int32_t tokens,
+                    ckv_stream_t stream) {
+  CacheRows r;
+  const int rc = cache_rows(cache, const_cast<void*>(k), k_tok_stride, k_head_stride, const_cast<void*>(v), v_tok_stride,
+                            v_head_stride, dtype, slots, tokens, &r);
+  if (rc || tokens == 0) return rc;
+  const cudaError_t e = launch_cache_write(*cache, r, (cudaStream_t)stream);
+  return e == cudaSuccess ? CKV_OK : cuda_fail(e, "cache write");
+}
+
+int ckv_cache_read(const ckv_cache* cache, void* k, void* v, int32_t dtype, const int64_t* slots, int32_t tokens,
+                   ckv_stream_t stream) {
+  CacheRows r;
+  const int64_t hs = cache ? cache->head_dim : 0, ts = cache ? hs * cache->num_kv_heads : 0;
+  const int rc = cache_rows(cache, k, ts, hs, v, ts, hs, dtype, slots, tokens, &r);
+  if (rc || tokens == 0) return rc;
+  const cudaError_t e = launch_cache_read(*cache, r, (cudaStream_t)stream);
+  return e == cudaSuccess ? CKV_OK : cuda_fail(e, "cache read");
+}
+
+int ckv_cache_attention_workspace(int32_t head_dim, int32_t max_q, int32_t q_heads, int32_t num_kv_heads, size_t* bytes) {
+  if (!bytes) return fail(CKV_ERR_ARG, "null argument");
+  if (head_dim != 64 && head_dim != 128) return fail(CKV_ERR_UNSUPPORTED, "cache head_dim must be 64 or 128");
+  if (max_q < 1 || num_kv_heads < 1 || q_heads < 1 || q_heads % num_kv_heads)
+    return fail(CKV_ERR_ARG, "q_heads must be a multiple of num_kv_heads, and max_q at least 1");
+  const int64_t rows = (int64_t)max_q * (q_heads / num_kv_heads);
+  *bytes = attention_workspace_bytes(head_dim, rows > 1 << 20 ? 1 << 20 : (int)rows);
+  return CKV_OK;
+}
+
+int ckv_cache_attention(const ckv_cache* cache, const ckv_attention_args* a, void* workspace, size_t workspace_bytes,
+                        ckv_stream_t stream) {
+  int rc = check_cache(cache);
+  if (rc) return rc;
+  if (!a) return fail(CKV_ERR_ARG, "null argument");
+  if (!known_dtype(a->dtype)) return fail(CKV_ERR_DTYPE, "dtype must be bf16, fp16 or fp32");
+  if (a->requests < 0 || a->tokens < 0 || a->table_width < 1 || a->table_stride < a->table_width)
+    return fail(CKV_ERR_ARG, "bad request count or table geometry");
+  if (!a->cu && a->requests != a->tokens) return fail(CKV_ERR_ARG, "without cu there is one query token per request");
+  const int es = a->dtype == CKV_FP32 ? 4 : 2;
+  if (!aligned16(a->q, a->q_tok_stride, a->q_head_stride, es) || !aligned16(a->out, a->out_tok_stride, a->out_head_stride, es))
+    return fail(CKV_ERR_ARG, "q and out pointers and strides must be 16-byte aligned (contiguous head_dim rows)");
+  size_t need = 0;
+  rc = ckv_cache_attention_workspace(cache->head_dim, a->max_q, a->q_heads, cache->num_kv_heads, &need);
+  if (rc) return rc;
+  if ((int64_t)a->max_q * a->q_heads > 1 << 20) return fail(CKV_ERR_UNSUPPORTED, "too many query rows per sequence");
+  if (!workspace || (uintptr_t)workspace % 256 != 0) return fail(CKV_ERR_WORKSPACE, "workspace must be 256-byte aligned and non-null");
+  if (workspace_bytes < need) return fail(CKV_ERR_WORKSPACE, "workspace too small (see ckv_cache_attention_workspace)");
+  if (a->requests == 0 || a->tokens == 0) return CKV_OK;
+  if (!a->q || !a->out || !a->tables || !a->lens) return fail(CKV_ERR_ARG, "null argument");
+  const cudaError_t e = launch_cache_attention(*cache, *a, workspace, (cudaStream_t)stream);
+  return e == cudaSuccess ? CKV_OK : cuda_fail(e, "cache attention");
 }
 
 int ckv_set_stage_events(void* const* events, int32_t count) {

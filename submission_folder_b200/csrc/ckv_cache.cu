@@ -1,0 +1,326 @@
+// Write and read of the paged 8-bit decode cache.
+//
+// Keys and values are held in 8 bits (e4m3 or int8) with one scale for each (block, KV
+// head): the smallest power of two, 2^-126 at least, with max |x| / scale at most the
+// format's largest value (448, 127).  Powers of two make x / scale exact, so a code is
+// the one rounding of its value, and when a later token raises a block's scale the e4m3
+// codes move by an exponent without a second rounding (above the subnormals); int8 codes are
+// shifted and rounded once.  A NaN or an infinity makes the scale NaN: everything read from
+// that (block, head) is NaN rather than quietly wrong.
+//
+// Write.  The call's tokens come with their slots; neighbours in one block form a run.  A CTA
+// owns the runs that begin in its piece of the token list, for one head and one of K / V: all
+// warps read the run's rows once into registers (16 rows per warp), the CTA agrees on the
+// largest magnitude, the block's scale follows, and the rows leave as codes.  A run that has
+// the block's first token begins the block anew; any other run keeps what the block holds,
+// rescaled when the scale grew.  One CTA per (run, head, K / V), so no atomics and the same
+// result every time.
+//
+// Bound: HBM; (element size + 1) bytes per element.
+#include "ckv_cache.h"
+#include "ckv_common.cuh"
+
+namespace ckv {
+
+constexpr int kRowsPerWarp = 16;
+
+// Smallest power-of-two scale (as a float) for a largest magnitude given by its bits; NaN for
+// a NaN or an infinity.  448 = 1.75 2^8, 127 = 1.984375 2^6.
+template <int kFmt> CKV_DEV float scale_for(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return __uint_as_float(0x7fffffffu);
+  constexpr uint32_t kMant = kFmt == CKV_CACHE_E4M3 ? 0x600000u : 0x7e0000u;
+  constexpr int kExp = kFmt == CKV_CACHE_E4M3 ? 8 : 6;
+  int e = (int)(amax_bits >> 23) - kExp + ((amax_bits & 0x7fffffu) > kMant ? 1 : 0);   // biased by 127
+  e = max(e, 1);   // 2^-126, also for zero and subnormal magnitudes
+  return __uint_as_float((uint32_t)e << 23);
+}
+// 1 / scale of a power of two in [2^-126, 2^121].
+CKV_DEV float inv_pow2(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
+
+// Four codes from four values already divided by the scale.
+template <int kFmt> CKV_DEV uint32_t encode4(float a, float b, float c, float d) {
+  uint32_t r;
+  if constexpr (kFmt == CKV_CACHE_E4M3) {
+    asm("{\n.reg .b16 lo, hi;\ncvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\ncvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n"
+        "mov.b32 %0, {lo, hi};\n}\n" : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
+  } else {
+    const int x = __float2int_rn(a), y = __float2int_rn(b), z = __float2int_rn(c), w = __float2int_rn(d);
+    r = (uint32_t)(x & 255) | (uint32_t)(y & 255) << 8 | (uint32_t)(z & 255) << 16 | (uint32_t)(w & 255) << 24;
+  }
+  return r;
+}
+template <int kFmt> CKV_DEV void decode4(uint32_t w, float (&o)[4]) {
+  if constexpr (kFmt == CKV_CACHE_E4M3) {
+    uint32_t lo, hi;
+    asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}\n"
+        : "=r"(lo), "=r"(hi) : "r"(w));
+    const float2 p = __half22float2(*reinterpret_cast<__half2*>(&lo)), q = __half22float2(*reinterpret_cast<__half2*>(&hi));
+    o[0] = p.x; o[1] = p.y; o[2] = q.x; o[3] = q.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = (float)(int8_t)(w >> (8 * i));
+  }
+}
+
+// 16 elements of a row as fp32, and back.
+CKV_DEV void load16(const float* p, float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(p) + i);
+    x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+  }
+}
+template <typename H> CKV_DEV void load16(const H* p, float (&x)[16]) {
+  H h[16];
+  *reinterpret_cast<uint4*>(h) = __ldg(reinterpret_cast<const uint4*>(p));
+  *reinterpret_cast<uint4*>(h + 8) = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = to_f32(h[i]);
+}
+CKV_DEV void store16(float* p, const float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+}
+CKV_DEV uint32_t pack2(float a, float b, __nv_bfloat16*) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+CKV_DEV uint32_t pack2(float a, float b, __half*) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename H> CKV_DEV void store16(H* p, const float (&x)[16]) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack2(x[2 * i], x[2 * i + 1], (H*)nullptr);
+  reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+struct WriteArgs {
+  ckv_cache c;
+  CacheRows r;
+  int piece;       // tokens of the list whose runs a CTA owns
+  int block_log2;
+};
+
+// grid (pieces, heads, 2); block_size / 16 warps.
+template <typename T, int kFmt, int D>
+__global__ void __launch_bounds__(kCacheMaxBlock / kRowsPerWarp * 32) k_cache_write(const WriteArgs a) {
+  constexpr int kLanesPerRow = D / 16, kRowsPerStep = 32 / kLanesPerRow, kSteps = kRowsPerWarp / kRowsPerStep;
+  __shared__ uint32_t s_max[kCacheMaxBlock / kRowsPerWarp];
+  __shared__ uint32_t s_new[kCacheMaxBlock / 32];   // offsets of the block that this run writes
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  const int h = blockIdx.y;
+  const bool isv = blockIdx.z != 0;
+  const int bs = a.c.block_size, T0 = blockIdx.x * a.piece, T1 = min(a.r.tokens, T0 + a.piece);
+  const int64_t pool = (int64_t)a.c.num_blocks << a.block_log2;
+  const T* src = static_cast<const T*>(isv ? a.r.v : a.r.k) + h * (isv ? a.r.vhs : a.r.khs);
+  const int64_t ts = isv ? a.r.vts : a.r.kts;
+  char* dst = static_cast<char*>(isv ? a.c.v : a.c.k) + h * (isv ? a.c.v_head_stride : a.c.k_head_stride);
+  const int64_t bstr = isv ? a.c.v_block_stride : a.c.k_block_stride, tstr = isv ? a.c.v_tok_stride : a.c.k_tok_stride;
+  float* scales = isv ? a.c.v_scale : a.c.k_scale;
+  const int64_t* slots = a.r.slots;
+  auto block_of = [&](int t) -> int64_t {
+    const int64_t s = __ldg(slots + t);
+    return s >= 0 && s < pool ? s >> a.block_log2 : -1;
+  };
+  int t = T0;
+  while (t < T1) {   // every warp takes the same path
+    // the next token that begins a run: its block is not the token's before it
+    const int cand = t + lane;
+    const int64_t mine = cand < T1 ? block_of(cand) : -1;
+    const uint32_t begins = __ballot_sync(0xffffffffu, mine >= 0 && (cand == 0 || block_of(cand - 1) != mine));
+    if (begins == 0) { t += 32; continue; }
+    t += __ffs(begins) - 1;
+    const int64_t blk = __shfl_sync(0xffffffffu, mine, __ffs(begins) - 1);
+    // the run's end, and whether it has the block's first token and rising slots
+    int end = t;
+    bool rising = true, anew = false;
+    for (bool more = true; more;) {
+      const int i = end + lane;
+      const bool in = i < a.r.tokens && block_of(i) == blk;
+      const uint32_t m = __ballot_sync(0xffffffffu, in);
+      const int n = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
+      const bool own = lane < n;
+      const int64_t s = own ? __ldg(slots + i) : 0;
+      rising = rising && __all_sync(0xffffffffu, !own || i == t || __ldg(slots + i - 1) < s);
+      anew = anew || __any_sync(0xffffffffu, own && (s & (bs - 1)) == 0);
+      end += n;
+      more = n == 32;
+    }
+    const int64_t sidx = blk * a.c.num_kv_heads + h;
+    const float old = anew ? 0.f : scales[sidx];
+    if (threadIdx.x < kCacheMaxBlock / 32) s_new[threadIdx.x] = 0;
+    const int rows_per_round = nw * kRowsPerWarp;
+    const bool once = end - t <= rows_per_round;
+    float x[kSteps][16];
+    uint32_t top = 0;
+    for (int r0 = t; r0 < end; r0 += rows_per_round) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int i = r0 + wid * kRowsPerWarp + s * kRowsPerStep + lane / kLanesPerRow;
+        if (i < end) load16(src + i * ts + (lane % kLanesPerRow) * 16, x[s]);
+        else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[s][e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[s][e]) & 0x7fffffffu);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    __syncthreads();   // s_new cleared, the last run's s_max read
+    if (lane == 0) s_max[wid] = top;
+    for (int i = t + threadIdx.x; i < end; i += blockDim.x) {
+      const int o = (int)(__ldg(slots + i) & (bs - 1));
+      atomicOr(&s_new[o >> 5], 1u << (o & 31));
+    }
+    __syncthreads();
+    for (int w = 0; w < nw; ++w) top = max(top, s_max[w]);
+    float scale = scale_for<kFmt>(top);
+    if (isnan(old) || isnan(scale)) scale = __uint_as_float(0x7fffffffu);
+    else scale = fmaxf(scale, old);
+    const bool bad = isnan(scale);
+    const float inv = bad ? 0.f : inv_pow2(scale);
+    char* blk_dst = dst + blk * bstr;
+    for (int r0 = t; r0 < end; r0 += rows_per_round) {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int i = r0 + wid * kRowsPerWarp + s * kRowsPerStep + lane / kLanesPerRow;
+        if (i >= end) continue;
+        const int64_t slot = __ldg(slots + i);
+        if (!rising) {   // a slot named again later in the run: its last token stays
+          bool again = false;
+          for (int j = i + 1; j < end; ++j) again = again || __ldg(slots + j) == slot;
+          if (again) continue;
+        }
+        if (!once) load16(src + i * ts + (lane % kLanesPerRow) * 16, x[s]);
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = bad ? 0u : encode4<kFmt>(x[s][4 * e] * inv, x[s][4 * e + 1] * inv, x[s][4 * e + 2] * inv, x[s][4 * e + 3] * inv);
+        *reinterpret_cast<uint4*>(blk_dst + (slot & (bs - 1)) * tstr + (lane % kLanesPerRow) * 16) =
+            make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    if (!anew && !bad && scale > old) {   // the tokens that stay, in the new scale
+      const float ratio = old * inv;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int o = wid * kRowsPerWarp + s * kRowsPerStep + lane / kLanesPerRow;
+        if (o >= bs || (s_new[o >> 5] >> (o & 31) & 1u)) continue;
+        uint4* p = reinterpret_cast<uint4*>(blk_dst + o * tstr + (lane % kLanesPerRow) * 16);
+        const uint4 v = *p;
+        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float f[4];
+          decode4<kFmt>(w[e], f);
+          w[e] = encode4<kFmt>(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+        }
+        *p = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+    if (threadIdx.x == 0) scales[sidx] = scale;
+    t = end;
+    __syncthreads();   // s_new and s_max are free for the next run
+  }
+}
+
+// One thread per 16 codes: grid over tokens * heads * D / 16, z = K / V.
+template <typename T, int kFmt>
+__global__ void __launch_bounds__(256) k_cache_read(const ckv_cache c, const CacheRows r, int block_log2) {
+  const int per_row = c.head_dim / 16;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int v16 = (int)(i % per_row);
+  const int64_t th = i / per_row;
+  const int h = (int)(th % c.num_kv_heads);
+  const int64_t t = th / c.num_kv_heads;
+  if (t >= r.tokens) return;
+  const bool isv = blockIdx.y != 0;
+  const int64_t s = __ldg(r.slots + t);
+  float x[16];
+  if (s >= 0 && s < ((int64_t)c.num_blocks << block_log2)) {
+    const int64_t blk = s >> block_log2, o = s & (c.block_size - 1);
+    const char* p = isv ? static_cast<const char*>(c.v) + blk * c.v_block_stride + h * c.v_head_stride + o * c.v_tok_stride
+                        : static_cast<const char*>(c.k) + blk * c.k_block_stride + h * c.k_head_stride + o * c.k_tok_stride;
+    const uint4 q = *(reinterpret_cast<const uint4*>(p) + v16);
+    const float sc = (isv ? c.v_scale : c.k_scale)[blk * c.num_kv_heads + h];
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float f[4];
+      decode4<kFmt>(w[e], f);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[4 * e + k] = f[k] * sc;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = 0.f;
+  }
+  T* out = isv ? static_cast<T*>(r.v) + t * r.vts + h * r.vhs : static_cast<T*>(r.k) + t * r.kts + h * r.khs;
+  store16(out + v16 * 16, x);
+}
+
+static int log2_of(int x) {
+  int l = 0;
+  while ((1 << l) < x) ++l;
+  return l;
+}
+
+template <typename T, int kFmt>
+static void write_launch(const WriteArgs& a, dim3 grid, int threads, cudaStream_t st) {
+  if (a.c.head_dim == 64) k_cache_write<T, kFmt, 64><<<grid, threads, 0, st>>>(a);
+  else k_cache_write<T, kFmt, 128><<<grid, threads, 0, st>>>(a);
+}
+
+cudaError_t launch_cache_write(const ckv_cache& c, const CacheRows& r, cudaStream_t st) {
+  WriteArgs a;
+  a.c = c; a.r = r; a.block_log2 = log2_of(c.block_size);
+  // a decode step has a run per token: one CTA each; a prompt's runs are whole blocks
+  a.piece = r.tokens <= 1024 ? 1 : c.block_size;
+  const dim3 grid((r.tokens + a.piece - 1) / a.piece, c.num_kv_heads, 2);
+  const int threads = c.block_size / kRowsPerWarp * 32;
+  const bool e4 = c.format == CKV_CACHE_E4M3;
+  switch (r.dtype) {
+    case CKV_BF16:
+      e4 ? write_launch<__nv_bfloat16, CKV_CACHE_E4M3>(a, grid, threads, st)
+         : write_launch<__nv_bfloat16, CKV_CACHE_INT8>(a, grid, threads, st);
+      break;
+    case CKV_FP16:
+      e4 ? write_launch<__half, CKV_CACHE_E4M3>(a, grid, threads, st) : write_launch<__half, CKV_CACHE_INT8>(a, grid, threads, st);
+      break;
+    default:
+      e4 ? write_launch<float, CKV_CACHE_E4M3>(a, grid, threads, st) : write_launch<float, CKV_CACHE_INT8>(a, grid, threads, st);
+      break;
+  }
+  return cudaGetLastError();
+}
+
+cudaError_t launch_cache_read(const ckv_cache& c, const CacheRows& r, cudaStream_t st) {
+  const int64_t n = (int64_t)r.tokens * c.num_kv_heads * (c.head_dim / 16);
+  const dim3 grid((unsigned)((n + 255) / 256), 2);
+  const int bl = log2_of(c.block_size);
+  const bool e4 = c.format == CKV_CACHE_E4M3;
+  switch (r.dtype) {
+    case CKV_BF16:
+      e4 ? k_cache_read<__nv_bfloat16, CKV_CACHE_E4M3><<<grid, 256, 0, st>>>(c, r, bl)
+         : k_cache_read<__nv_bfloat16, CKV_CACHE_INT8><<<grid, 256, 0, st>>>(c, r, bl);
+      break;
+    case CKV_FP16:
+      e4 ? k_cache_read<__half, CKV_CACHE_E4M3><<<grid, 256, 0, st>>>(c, r, bl)
+         : k_cache_read<__half, CKV_CACHE_INT8><<<grid, 256, 0, st>>>(c, r, bl);
+      break;
+    default:
+      e4 ? k_cache_read<float, CKV_CACHE_E4M3><<<grid, 256, 0, st>>>(c, r, bl)
+         : k_cache_read<float, CKV_CACHE_INT8><<<grid, 256, 0, st>>>(c, r, bl);
+      break;
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace ckv

@@ -1,0 +1,131 @@
+// Rotary positions of queries and keys, both in one launch.
+//
+// Pair i of a head turns by the angle position * f_i: (a, b) -> (a c - b s, b c + a s) with
+// c, s = factor * cos, sin.  `inverse` turns by the negative angle, which is the transpose
+// and so the gradient with respect to the unrotated vector.  The pairs are (x[i], x[i + d/2])
+// or, interleaved, (x[2i], x[2i + 1]), for the first d dimensions; the rest pass through.
+//
+// Angles: position * f / 2 pi in 64 bits, reduced to a fraction of a turn in (-1/2, 1/2],
+// then single precision with the residual of that rounding put back to first order, so a
+// position of 10^6 loses nothing (in 32 bits its angle would be off by 0.06).  They are
+// computed once per token and shared by all heads through shared memory.
+//
+// Bound: HBM (each element read once and written once).
+#include "ckv_cache.h"
+#include "ckv_common.cuh"
+
+namespace ckv {
+
+constexpr int kRotThreads = 256;
+constexpr int kRotMaxDim = 512;
+
+template <typename T> CKV_DEV T from_f32(float x);
+template <> CKV_DEV float from_f32<float>(float x) { return x; }
+template <> CKV_DEV __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> CKV_DEV __half from_f32<__half>(float x) { return __float2half_rn(x); }
+
+template <typename T, int N> struct alignas(sizeof(T) * N) Vec { T x[N]; };
+
+// One unit = N elements of the first halves and their N partners (half layout), 2N adjacent
+// elements (interleaved), or N elements past the rotated part.
+template <typename T, int N, bool kInter>
+__global__ void __launch_bounds__(kRotThreads) k_rotary(const ckv_rotary_args a, int tokens_per_cta) {
+  extern __shared__ float2 rot_cs[];   // [tokens_per_cta][pairs]
+  const int pairs = a.rotary_dim / 2;
+  const int t0 = blockIdx.x * tokens_per_cta;
+  const int nt = min(tokens_per_cta, a.tokens - t0);
+  for (int i = threadIdx.x; i < nt * pairs; i += kRotThreads) {
+    const int t = i / pairs, p = i - t * pairs;
+    const double turns = (double)a.positions[t0 + t] * (a.inv_freq[p] * 0.15915494309189533577);
+    const double r = turns - rint(turns);
+    const float hi = (float)r, lo = (float)(r - (double)hi) * 6.2831853f;
+    float s, c;
+    sincospif(2.f * hi, &s, &c);
+    const float c1 = fmaf(-lo, s, c), s1 = fmaf(lo, c, s);
+    rot_cs[i] = make_float2(c1 * a.factor, (a.inverse ? -s1 : s1) * a.factor);
+  }
+  __syncthreads();
+  const int turn_units = pairs / N;                                   // per head
+  const int rest_units = (a.head_dim - a.rotary_dim) / N;
+  const int units = turn_units + rest_units;
+  const int heads = a.q_heads + a.k_heads;
+  const int h0 = blockIdx.y * a.heads_per_cta, h1 = min(heads, h0 + a.heads_per_cta);
+  const int per_token = (h1 - h0) * units;
+  for (int i = threadIdx.x; i < nt * per_token; i += kRotThreads) {
+    const int t = i / per_token, j = i - t * per_token;
+    const int hh = j / units, u = j - hh * units;
+    const int h = h0 + hh;
+    const bool isk = h >= a.q_heads;
+    const int64_t tok = t0 + t;
+    const T* src = isk ? static_cast<const T*>(a.k) + tok * a.k_tok_stride + (h - a.q_heads) * a.k_head_stride
+                       : static_cast<const T*>(a.q) + tok * a.q_tok_stride + h * a.q_head_stride;
+    T* dst = isk ? static_cast<T*>(a.out_k) + tok * a.out_k_tok_stride + (h - a.q_heads) * a.out_k_head_stride
+                 : static_cast<T*>(a.out_q) + tok * a.out_q_tok_stride + h * a.out_q_head_stride;
+    using V = Vec<T, N>;
+    if (u < turn_units) {
+      const float2* cs = rot_cs + t * pairs + u * N;
+      const int i0 = kInter ? 2 * u * N : u * N, i1 = kInter ? i0 + N : i0 + pairs;
+      const V x = *reinterpret_cast<const V*>(src + i0), y = *reinterpret_cast<const V*>(src + i1);
+      V ox, oy;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        if constexpr (!kInter) {
+          const float c = cs[e].x, s = cs[e].y, p = to_f32(x.x[e]), q = to_f32(y.x[e]);
+          ox.x[e] = from_f32<T>(p * c - q * s);
+          oy.x[e] = from_f32<T>(q * c + p * s);
+        } else if constexpr (N == 1) {
+          const float c = cs[0].x, s = cs[0].y, p = to_f32(x.x[0]), q = to_f32(y.x[0]);
+          ox.x[0] = from_f32<T>(p * c - q * s);
+          oy.x[0] = from_f32<T>(q * c + p * s);
+        } else if (e % 2 == 0) {
+          const float c = cs[e / 2].x, s = cs[e / 2].y, p = to_f32(x.x[e]), q = to_f32(x.x[e + 1]);
+          ox.x[e] = from_f32<T>(p * c - q * s);
+          ox.x[e + 1] = from_f32<T>(q * c + p * s);
+          const float c2 = cs[N / 2 + e / 2].x, s2 = cs[N / 2 + e / 2].y;
+          const float p2 = to_f32(y.x[e]), q2 = to_f32(y.x[e + 1]);
+          oy.x[e] = from_f32<T>(p2 * c2 - q2 * s2);
+          oy.x[e + 1] = from_f32<T>(q2 * c2 + p2 * s2);
+        }
+      }
+      *reinterpret_cast<V*>(dst + i0) = ox;
+      *reinterpret_cast<V*>(dst + i1) = oy;
+    } else if (src != dst) {
+      const int i0 = a.rotary_dim + (u - turn_units) * N;
+      *reinterpret_cast<V*>(dst + i0) = *reinterpret_cast<const V*>(src + i0);
+    }
+  }
+}
+
+template <typename T, int N>
+static void rot_launch(const ckv_rotary_args& a, int tpc, dim3 grid, cudaStream_t st) {
+  const size_t smem = (size_t)tpc * (a.rotary_dim / 2) * sizeof(float2);
+  if (a.interleaved) k_rotary<T, N, true><<<grid, kRotThreads, smem, st>>>(a, tpc);
+  else k_rotary<T, N, false><<<grid, kRotThreads, smem, st>>>(a, tpc);
+}
+
+cudaError_t launch_rotary(const ckv_rotary_args& args, cudaStream_t st) {
+  ckv_rotary_args a = args;
+  const int es = a.dtype == CKV_FP32 ? 4 : 2, n = 16 / es;
+  const int heads = a.q_heads + a.k_heads;
+  // 16-byte vectors need every row and every half to start on 16 bytes
+  auto al = [&](const void* p, int64_t ts, int64_t hs) {
+    return (uintptr_t)p % 16 == 0 && (ts * es) % 16 == 0 && (hs * es) % 16 == 0;
+  };
+  const bool vec = al(a.q, a.q_tok_stride, a.q_head_stride) && al(a.out_q, a.out_q_tok_stride, a.out_q_head_stride) &&
+                   (a.k_heads == 0 || (al(a.k, a.k_tok_stride, a.k_head_stride) &&
+                                       al(a.out_k, a.out_k_tok_stride, a.out_k_head_stride))) &&
+                   (a.rotary_dim / 2) % n == 0 && a.head_dim % n == 0;
+  // few tokens: one per CTA and the heads spread over CTAs (latency); many: four per CTA
+  const int tpc = a.tokens >= 1024 ? 4 : 1;
+  const int splits = a.tokens >= 1024 ? 1 : (a.tokens >= 148 ? 2 : 8);
+  a.heads_per_cta = (heads + splits - 1) / splits;
+  const dim3 grid((a.tokens + tpc - 1) / tpc, (heads + a.heads_per_cta - 1) / a.heads_per_cta);
+  switch (a.dtype) {
+    case CKV_BF16: vec ? rot_launch<__nv_bfloat16, 8>(a, tpc, grid, st) : rot_launch<__nv_bfloat16, 1>(a, tpc, grid, st); break;
+    case CKV_FP16: vec ? rot_launch<__half, 8>(a, tpc, grid, st) : rot_launch<__half, 1>(a, tpc, grid, st); break;
+    default: vec ? rot_launch<float, 4>(a, tpc, grid, st) : rot_launch<float, 1>(a, tpc, grid, st); break;
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace ckv

@@ -8,7 +8,7 @@ the GPU first and results copied back; nothing runs on the CPU.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -396,3 +396,277 @@ def gather(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, idx: 
     check(_lib.load().ckv_gather(ctypes.byref(L), window, idx.data_ptr(), kept, int(idx.dim() == 2),
                                  k_out.data_ptr(), v_out.data_ptr(), _stream(k.device)), "ckv_gather")
     return k_out, v_out
+
+
+# ---------------------------------------------------------------------------
+# paged 8-bit decode cache: block tables, rotary positions, write / read, attention
+# ---------------------------------------------------------------------------
+_CACHE_FORMATS = {torch.float8_e4m3fn: _lib.CACHE_E4M3, torch.int8: _lib.CACHE_INT8}
+_CODES = {dt: _lib.DTYPE_CODES[name] for dt, name in _DT.items()}
+
+
+class _on_device:
+    """Makes ``device`` the current one for a launch (nothing to do when it is already)."""
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def _same_device(*ts: Optional[torch.Tensor]) -> torch.device:
+    """The one CUDA device that all the tensors are on."""
+    dev = ts[0].device
+    if dev.type != "cuda":
+        _require_cuda(*ts)
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"tensors are on different devices: {dev} and {t.device}")
+    return dev
+
+
+def _int_tensor(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str) -> None:
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _no_grad_needed(what: str, *ts: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError(f"{what} records no autograd graph; call it on detached tensors")
+
+
+def _rows(t: torch.Tensor, what: str) -> None:
+    if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] != 1):
+        raise ValueError(f"{what} must be [tokens, heads, head_dim] with contiguous head_dim")
+    if t.dtype not in _CODES:
+        raise TypeError(f"{what} must be bf16, fp16 or fp32, got {t.dtype}")
+
+
+class TableStep(NamedTuple):
+    """What ``block_tables`` says of a step: per request ``lens`` (after it) and ``granted``, the
+    free count, ``cu`` (first token of each request), and each token's slot and position."""
+
+    lens: torch.Tensor         # int32 [R]
+    free_count: torch.Tensor   # int32 [1]
+    cu: torch.Tensor           # int32 [R + 1]
+    slots: torch.Tensor        # int64 [total], -1: no token
+    positions: torch.Tensor    # int64 [total]
+    granted: torch.Tensor      # int32 [R]
+
+
+def block_tables(lens: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, free_list: torch.Tensor,
+                 free_count: torch.Tensor, block_size: int, total: int, shift: Optional[torch.Tensor] = None,
+                 lens_out: Optional[torch.Tensor] = None, free_count_out: Optional[torch.Tensor] = None) -> TableStep:
+    """One step of the block tables of a paged cache, on the device (``ckv_block_tables``).
+
+    Request ``r`` holds ``lens[r]`` tokens and gets ``new[r]`` more (0: none; negative: it ends
+    and its blocks return to the free list).  ``tables`` int32 ``[R, width]`` and the stack
+    ``free_list`` / ``free_count`` are updated in place, and so are ``lens`` and ``free_count``
+    unless ``lens_out`` / ``free_count_out`` take them.  ``total``: the number of token rows in
+    this step's tensors, at least the sum of ``new`` where a token's slot matters; rows past the
+    sum get slot -1.  ``shift`` int32 ``[R]`` is added to the positions (the number of tokens
+    evicted from the request).  A request that does not fit gets slots of -1 and ``granted`` 0.
+    """
+    dev = _same_device(lens, new, tables, free_list, free_count, shift, lens_out, free_count_out)
+    R = lens.shape[0] if lens.dim() == 1 else -1
+    i32 = torch.int32
+    _int_tensor(lens, i32, (R,), "lens")
+    _int_tensor(new, i32, (R,), "new")
+    _int_tensor(free_count, i32, (1,), "free_count")
+    if tables.dtype != i32 or tables.dim() != 2 or tables.shape[0] != R or tables.stride(1) != 1:
+        raise ValueError("tables must be an int32 tensor [requests, width] with contiguous rows")
+    if free_list.dtype != i32 or free_list.dim() != 1 or not free_list.is_contiguous():
+        raise ValueError("free_list must be a contiguous int32 vector")
+    if shift is not None:
+        _int_tensor(shift, i32, (R,), "shift")
+    if total < 0:
+        raise ValueError("total must not be negative")
+    if lens_out is None:
+        lens_out = lens
+    else:
+        _int_tensor(lens_out, i32, (R,), "lens_out")
+    if free_count_out is None:
+        free_count_out = free_count
+    else:
+        _int_tensor(free_count_out, i32, (1,), "free_count_out")
+    small = torch.empty(2 * R + 1, dtype=i32, device=dev)
+    wide = torch.empty(2, total, dtype=torch.int64, device=dev)
+    cu, granted = small[:R + 1], small[R + 1:]
+    s = _lib.TableStep(lens.data_ptr(), new.data_ptr(), _ptr(shift), tables.data_ptr(), max(tables.stride(0), tables.shape[1]),
+                       tables.shape[1], free_list.data_ptr(), free_list.numel(), free_count.data_ptr(), block_size, R, total,
+                       lens_out.data_ptr(), free_count_out.data_ptr(), cu.data_ptr(), wide.data_ptr(),
+                       wide.data_ptr() + 8 * total, granted.data_ptr())
+    with _on_device(dev):
+        check(_lib.load().ckv_block_tables(ctypes.byref(s), _stream(dev)), "ckv_block_tables")
+    return TableStep(lens_out, free_count_out, cu, wide[0], wide[1], granted)
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
+           interleaved: bool = False, factor: float = 1.0, inverse: bool = False,
+           out: Optional[Tuple[torch.Tensor, Optional[torch.Tensor]]] = None):
+    """Rotary positions of ``q`` ``[T, H, D]`` and ``k`` ``[T, Hk, D]`` (or None) in one launch.
+
+    ``positions`` int64 ``[T]``; ``inv_freq`` float64 ``[rotary_dim / 2]`` radians per position
+    (``rotary.rotary_frequencies``): the first ``2 * len(inv_freq)`` dimensions turn, in pairs
+    ``(i, i + rotary_dim / 2)`` or, ``interleaved``, ``(2i, 2i + 1)``.  ``factor`` scales cosine and
+    sine.  ``inverse`` turns back: with the same ``factor`` it is the transpose, so
+    ``rotary(grad_q, grad_k, ..., inverse=True)`` is the backward pass.  ``out=(q, k)`` works in
+    place.  Returns ``(q_out, k_out)``.
+    """
+    dev = _same_device(q, k, positions, inv_freq)
+    _no_grad_needed("rotary", q, k)
+    _rows(q, "q")
+    T, H, D = q.shape
+    Hk = 0
+    if k is not None:
+        _rows(k, "k")
+        if k.dtype != q.dtype or k.shape[0] != T or k.shape[2] != D:
+            raise ValueError("q and k must agree in dtype, tokens and head_dim")
+        Hk = k.shape[1]
+    _int_tensor(positions, torch.int64, (T,), "positions")
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous float64 vector")
+    if out is None:
+        qo = torch.empty(T, H, D, dtype=q.dtype, device=dev)
+        ko = None if k is None else torch.empty(T, Hk, D, dtype=q.dtype, device=dev)
+    else:
+        qo, ko = out
+        _same_device(q, qo, ko)
+        for x, o, what in ((q, qo, "out[0]"), (k, ko, "out[1]")):
+            if (x is None) != (o is None) or (x is not None and (o.shape != x.shape or o.dtype != x.dtype)):
+                raise ValueError(f"{what} must be like its input")
+            if o is not None:
+                _rows(o, what)
+    a = _lib.RotaryArgs(q.data_ptr(), q.stride(0), q.stride(1), _ptr(k), *((0, 0) if k is None else k.stride()[:2]),
+                        qo.data_ptr(), qo.stride(0), qo.stride(1), _ptr(ko), *((0, 0) if k is None else ko.stride()[:2]),
+                        positions.data_ptr(), inv_freq.data_ptr(), factor, T, H, Hk, D, 2 * inv_freq.shape[0],
+                        _CODES[q.dtype], interleaved, inverse, 0)
+    with _on_device(dev):
+        check(_lib.load().ckv_rotary(ctypes.byref(a), _stream(dev)), "ckv_rotary")
+    return qo, ko
+
+
+def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> _lib.Cache:
+    if k_cache.dtype not in _CACHE_FORMATS or v_cache.dtype != k_cache.dtype:
+        raise TypeError("k_cache and v_cache must both be float8_e4m3fn or int8")
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+        raise ValueError("k_cache and v_cache must be [blocks, kv_heads, block_size, head_dim] with contiguous head_dim")
+    N, H, B, D = k_cache.shape
+    for s in (k_scale, v_scale):
+        if s.dtype != torch.float32 or s.dim() != 2 or s.shape[0] != N or s.shape[1] != H or not s.is_contiguous():
+            raise ValueError(f"scales must be contiguous float32 tensors of shape {(N, H)}")
+    ks, vs = k_cache.stride(), v_cache.stride()
+    return _lib.Cache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), ks[0], ks[1], ks[2],
+                      vs[0], vs[1], vs[2], N, H, B, D, _CACHE_FORMATS[k_cache.dtype])
+
+
+def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                v_scale: torch.Tensor, slots: torch.Tensor) -> None:
+    """Quantise rows ``k``, ``v`` ``[T, Hkv, D]`` into their ``slots`` (int64 ``[T]``) of a paged 8-bit
+    cache (``ckv_cache_write``): ``k_cache`` / ``v_cache`` float8_e4m3fn or int8 ``[blocks, Hkv,
+    block_size, D]``, ``k_scale`` / ``v_scale`` float32 ``[blocks, Hkv]``.
+
+    A block's scale is the smallest power of two that holds its largest magnitude.  Tokens of one
+    block stand next to one another in the list; if the block's first place is among them the block
+    begins anew, otherwise its other tokens stay (rescaled where the scale grew).  Slots outside the
+    pool (-1) are no tokens.  A NaN or an infinity makes its block and head read as NaN.
+    """
+    dev = _same_device(k, v, k_cache, v_cache, k_scale, v_scale, slots)
+    _no_grad_needed("cache_write", k, v)
+    _rows(k, "k")
+    _rows(v, "v")
+    c = _cache(k_cache, v_cache, k_scale, v_scale)
+    if v.dtype != k.dtype or v.shape != k.shape or k.shape[1] != c.num_kv_heads or k.shape[2] != c.head_dim:
+        raise ValueError(f"k and v must be [tokens, {c.num_kv_heads}, {c.head_dim}] of one dtype")
+    _int_tensor(slots, torch.int64, (k.shape[0],), "slots")
+    with _on_device(dev):
+        check(_lib.load().ckv_cache_write(ctypes.byref(c), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                                          v.stride(1), _CODES[k.dtype], slots.data_ptr(), k.shape[0], _stream(dev)),
+              "ckv_cache_write")
+
+
+def cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+               slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The values at ``slots`` (int64 ``[T]``) of a paged 8-bit cache as ``(k, v)`` ``[T, Hkv, D]`` of
+    ``dtype``; a slot outside the pool gives zeros.  A cache that is to be scored and compressed
+    again goes through here back to ``score_evict``."""
+    dev = _same_device(k_cache, v_cache, k_scale, v_scale, slots)
+    if dtype not in _CODES:
+        raise TypeError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
+    c = _cache(k_cache, v_cache, k_scale, v_scale)
+    _int_tensor(slots, torch.int64, (slots.numel(),), "slots")
+    T = slots.shape[0]
+    k = torch.empty(T, c.num_kv_heads, c.head_dim, dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    with _on_device(dev):
+        check(_lib.load().ckv_cache_read(ctypes.byref(c), k.data_ptr(), v.data_ptr(), _CODES[dtype], slots.data_ptr(), T,
+                                         _stream(dev)), "ckv_cache_read")
+    return k, v
+
+
+_att_ws_bytes = {}
+
+
+def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                    v_scale: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, cu: Optional[torch.Tensor] = None,
+                    max_q: int = 1, scale: Optional[float] = None, causal: bool = True, want_lse: bool = False,
+                    out: Optional[torch.Tensor] = None):
+    """Attention of the new query tokens ``q`` ``[T, H, D]`` over a paged 8-bit cache
+    (``ckv_cache_attention``), reading each code once; meant for a few query tokens per sequence.
+
+    Sequence ``r`` has query rows ``cu[r] .. cu[r + 1]`` (int32 ``[R + 1]``, at most ``max_q`` each;
+    None: one row each) and ``lens[r]`` cached tokens (int32 ``[R]``, the new ones included) in the
+    blocks ``tables[r]`` (int32 ``[R, width]``).  ``causal``: the new tokens see one another in order.
+    Query head ``h`` reads KV head ``h // (H // Hkv)``.  ``scale`` defaults to ``D ** -0.5``.  A row that
+    sees nothing gives zeros (log-sum-exp -inf); rows past ``cu[R]`` are left as they were (in
+    ``out``, if given).  Returns ``out``, or ``(out, lse)`` with ``want_lse``: natural-log
+    log-sum-exp, float32 ``[T, H]``.
+    """
+    dev = _same_device(q, k_cache, v_cache, k_scale, v_scale, tables, lens, cu, out)
+    _no_grad_needed("cache_attention", q)
+    _rows(q, "q")
+    c = _cache(k_cache, v_cache, k_scale, v_scale)
+    T, H, D = q.shape
+    R = tables.shape[0]
+    if D != c.head_dim or H % c.num_kv_heads:
+        raise ValueError(f"q must be [tokens, heads, {c.head_dim}] with a multiple of {c.num_kv_heads} heads")
+    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.stride(1) != 1:
+        raise ValueError("tables must be an int32 tensor [requests, width] with contiguous rows")
+    _int_tensor(lens, torch.int32, (R,), "lens")
+    if cu is None:
+        if R != T:
+            raise ValueError("without cu, q has one row per request")
+        max_q = 1
+    else:
+        _int_tensor(cu, torch.int32, (R + 1,), "cu")
+    if out is None:
+        out = torch.empty(T, H, D, dtype=q.dtype, device=dev)
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out must be like q")
+        _rows(out, "out")
+    lse = torch.empty(T, H, dtype=torch.float32, device=dev) if want_lse else None
+    lib = _lib.load()
+    key = (D, max_q, H, c.num_kv_heads)
+    nbytes = _att_ws_bytes.get(key)
+    if nbytes is None:
+        b = ctypes.c_size_t()
+        check(lib.ckv_cache_attention_workspace(D, max_q, H, c.num_kv_heads, ctypes.byref(b)),
+              "ckv_cache_attention_workspace")
+        nbytes = _att_ws_bytes[key] = b.value
+    # from the allocator for each call: two streams, or two captured graphs, never share it
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    a = _lib.AttentionArgs(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse),
+                           tables.data_ptr(), max(tables.stride(0), tables.shape[1]), tables.shape[1], lens.data_ptr(), _ptr(cu), R, T,
+                           max_q, H, causal, D ** -0.5 if scale is None else scale, _CODES[q.dtype])
+    with _on_device(dev):
+        check(lib.ckv_cache_attention(ctypes.byref(c), ctypes.byref(a), ws.data_ptr(), nbytes, _stream(dev)),
+              "ckv_cache_attention")
+    return (out, lse) if want_lse else out

@@ -1,0 +1,149 @@
+"""The paged 8-bit decode cache without a GPU: the C ABI's argument checks, the rotary
+frequencies, and the refusal to run on host tensors."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from submission_folder_b200 import _lib, ops
+from submission_folder_b200.cache import PagedKVCache
+from submission_folder_b200.rotary import rotary_frequencies
+
+P = 4096   # a pointer that is never followed: every call here is refused first
+
+
+def _cache(**over):
+    a = dict(k=P, v=P, k_scale=P, v_scale=P, k_block_stride=4096, k_head_stride=2048, k_tok_stride=128, v_block_stride=4096,
+             v_head_stride=2048, v_tok_stride=128, num_blocks=4, num_kv_heads=2, block_size=16, head_dim=128, format=0)
+    a.update(over)
+    return _lib.Cache(**a)
+
+
+@pytest.mark.parametrize("over,code", [
+    (dict(k=None), -1), (dict(v_scale=None), -1), (dict(format=2), -2), (dict(head_dim=96), -3), (dict(block_size=24), -3),
+    (dict(num_blocks=0), -1), (dict(num_kv_heads=0), -1), (dict(num_kv_heads=70000), -1), (dict(k=P + 8), -1),
+    (dict(v_tok_stride=120), -1), (dict(k_head_stride=2056), -1)])
+def test_bad_caches_are_refused(over, code):
+    lib, c = _lib.load(), _cache(**over)
+    assert lib.ckv_cache_read(ctypes.byref(c), P, P, 0, P, 3, None) == code
+    assert lib.ckv_cache_write(ctypes.byref(c), P, 256, 128, P, 256, 128, 0, P, 3, None) == code
+    a = _lib.AttentionArgs(q=P, q_tok_stride=1024, q_head_stride=128, out=P, out_tok_stride=1024, out_head_stride=128, tables=P,
+                           table_stride=4, table_width=4, lens=P, requests=1, tokens=1, max_q=1, q_heads=8, scale=1.0)
+    assert lib.ckv_cache_attention(ctypes.byref(c), ctypes.byref(a), P, 1 << 30, None) == code
+    assert lib.ckv_last_error_string()
+
+
+def test_bad_rows_are_refused():
+    lib, c = _lib.load(), _cache()
+    ref = ctypes.byref(c)
+    assert lib.ckv_cache_write(ref, P, 256, 128, P, 256, 128, 7, P, 3, None) == -2       # dtype
+    assert lib.ckv_cache_write(ref, P, 256, 128, P, 256, 128, 0, None, 3, None) == -1    # no slots
+    assert lib.ckv_cache_write(ref, P, 256, 128, P, 256, 128, 0, P, -1, None) == -1
+    assert lib.ckv_cache_write(ref, P + 2, 256, 128, P, 256, 128, 0, P, 3, None) == -1   # alignment
+    assert lib.ckv_cache_write(ref, P, 250, 128, P, 256, 128, 0, P, 3, None) == -1
+    assert lib.ckv_cache_read(ref, P, None, 0, P, 3, None) == -1
+    assert lib.ckv_cache_write(ref, None, 0, 0, None, 0, 0, 0, None, 0, None) == 0       # nothing to write
+    assert lib.ckv_cache_read(None, P, P, 0, P, 3, None) == -1
+
+
+@pytest.mark.parametrize("over,code", [
+    (dict(q=None), -1), (dict(tables=None), -1), (dict(lens=None), -1), (dict(dtype=5), -2), (dict(q=P + 4), -1),
+    (dict(out_tok_stride=1020), -1), (dict(q_heads=7), -1), (dict(max_q=0), -1), (dict(table_width=0), -1),
+    (dict(table_stride=3), -1), (dict(tokens=2), -1), (dict(requests=-1), -1), (dict(cu=P, max_q=1 << 20), -3)])
+def test_bad_attention_is_refused(over, code):
+    lib, c = _lib.load(), _cache()
+    a = dict(q=P, q_tok_stride=1024, q_head_stride=128, out=P, out_tok_stride=1024, out_head_stride=128, tables=P, table_stride=4,
+             table_width=4, lens=P, requests=1, tokens=1, max_q=1, q_heads=8, scale=1.0)
+    a.update(over)
+    s = _lib.AttentionArgs(**a)
+    assert lib.ckv_cache_attention(ctypes.byref(c), ctypes.byref(s), P, 1 << 40, None) == code
+
+
+def test_attention_workspace_is_checked():
+    lib, c = _lib.load(), _cache()
+    a = _lib.AttentionArgs(q=P, q_tok_stride=1024, q_head_stride=128, out=P, out_tok_stride=1024, out_head_stride=128, tables=P,
+                           table_stride=4, table_width=4, lens=P, requests=1, tokens=1, max_q=1, q_heads=8, scale=1.0)
+    need = ctypes.c_size_t()
+    assert lib.ckv_cache_attention_workspace(128, 1, 8, 2, ctypes.byref(need)) == 0 and need.value > 0
+    for ws, size in ((None, need.value), (P + 64, need.value), (P, need.value - 1)):
+        assert lib.ckv_cache_attention(ctypes.byref(c), ctypes.byref(a), ws, size, None) == -4
+    assert lib.ckv_cache_attention_workspace(80, 1, 8, 2, ctypes.byref(need)) == -3
+    assert lib.ckv_cache_attention_workspace(128, 1, 7, 2, ctypes.byref(need)) == -1
+    assert lib.ckv_cache_attention_workspace(128, 1, 8, 2, None) == -1
+
+
+@pytest.mark.parametrize("over", [dict(lens=None), dict(out_slots=None), dict(out_granted=None), dict(requests=0), dict(requests=8193),
+                                  dict(total=-1), dict(table_width=0), dict(table_stride=1), dict(block_size=0),
+                                  dict(free_capacity=-1)])
+def test_bad_table_steps_are_refused(over):
+    a = dict(lens=P, new_tokens=P, tables=P, table_stride=4, table_width=4, free_list=P, free_capacity=8, free_count=P,
+             block_size=16, requests=2, total=2, out_lens=P, out_free_count=P, out_cu=P, out_slots=P, out_positions=P,
+             out_granted=P)
+    a.update(over)
+    s = _lib.TableStep(**a)
+    assert _lib.load().ckv_block_tables(ctypes.byref(s), None) == -1
+
+
+@pytest.mark.parametrize("over,code", [(dict(q=None), -1), (dict(k_heads=1), -1), (dict(dtype=3), -2), (dict(rotary_dim=0), -1),
+                                       (dict(rotary_dim=7), -1), (dict(rotary_dim=66), -1), (dict(tokens=-1), -1),
+                                       (dict(q_heads=0), -1), (dict(head_dim=2048, rotary_dim=64), -1), (dict(tokens=0), 0)])
+def test_bad_rotary_is_refused(over, code):
+    a = dict(q=P, q_tok_stride=64, q_head_stride=64, out_q=P, out_q_tok_stride=64, out_q_head_stride=64, positions=P, inv_freq=P,
+             factor=1.0, tokens=2, q_heads=1, k_heads=0, head_dim=64, rotary_dim=64, dtype=0)
+    a.update(over)
+    s = _lib.RotaryArgs(**a)
+    assert _lib.load().ckv_rotary(ctypes.byref(s), None) == code
+
+
+def test_host_tensors_are_refused():
+    """The kernels never run on the CPU."""
+    x, i = torch.zeros(2, 2, 64), torch.zeros(2, dtype=torch.int32)
+    c = PagedKVCache(1, 4, 2, 32, 2, 64, 16, device="cpu")
+    for call in (lambda: ops.rotary(x, None, i.long(), rotary_frequencies(64)[0]),
+                 lambda: ops.cache_write(x, x, *c.layer(0), i.long()), lambda: ops.cache_read(*c.layer(0), i.long()),
+                 lambda: ops.cache_attention(x, *c.layer(0), c.tables, c.lens), lambda: c.step(i)):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+@pytest.mark.parametrize("over", [dict(num_layers=0), dict(block_size=48), dict(head_dim=80), dict(dtype=torch.uint8),
+                                  dict(max_tokens=0)])
+def test_bad_paged_caches_are_refused(over):
+    a = dict(num_layers=1, num_blocks=4, max_requests=2, max_tokens=32, num_key_value_heads=2, head_dim=64, block_size=16, device="cpu")
+    with pytest.raises(ValueError):
+        PagedKVCache(**{**a, **over})
+
+
+def test_rotary_frequencies():
+    f, factor = rotary_frequencies(128)
+    assert f.dtype == torch.float64 and factor == 1.0 and f[0] == 1.0
+    assert torch.allclose(f, torch.tensor([10000.0 ** (-2 * i / 128) for i in range(64)], dtype=torch.float64), rtol=1e-14)
+    assert torch.equal(rotary_frequencies(64, scaling=dict(type="linear", factor=4.0))[0], rotary_frequencies(64)[0] / 4)
+    # dynamic: unchanged up to the original length; at twice it the slowest pair turns as far as before
+    s = dict(rope_type="dynamic", factor=1.0, original_max_position_embeddings=2048)
+    assert torch.equal(rotary_frequencies(64, scaling=s, seq_len=100)[0], rotary_frequencies(64)[0])
+    slow = rotary_frequencies(64, scaling=s, seq_len=4096)[0][-1] * 4096
+    assert math.isclose(float(slow), float(rotary_frequencies(64)[0][-1]) * 2048, rel_tol=1e-12)
+    # llama3: fast pairs stay, slow pairs are divided, the blend lies between
+    s = dict(rope_type="llama3", factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0, original_max_position_embeddings=8192)
+    plain, got = rotary_frequencies(128, 500000.0)[0], rotary_frequencies(128, 500000.0, s)[0]
+    wave = 2 * math.pi / plain
+    assert torch.equal(got[wave < 2048], plain[wave < 2048]) and torch.allclose(got[wave > 8192], plain[wave > 8192] / 8, rtol=1e-15)
+    mid = (wave > 2048) & (wave < 8192)
+    smooth = (8192 / wave - 1.0) / 3.0
+    assert mid.any() and torch.allclose(got[mid], ((1 - smooth) * plain / 8 + smooth * plain)[mid], rtol=1e-12)
+    # yarn: ends as above, and the attention factor
+    s = dict(rope_type="yarn", factor=16.0, original_max_position_embeddings=4096)
+    got, factor = rotary_frequencies(128, 10000.0, s)
+    plain = rotary_frequencies(128)[0]
+    assert got[0] == plain[0] and math.isclose(float(got[-1]), float(plain[-1]) / 16, rel_tol=1e-12)
+    assert math.isclose(factor, 0.1 * math.log(16.0) + 1.0) and torch.all(got <= plain) and torch.all(got >= plain / 16)
+    assert rotary_frequencies(128, 10000.0, dict(s, attention_factor=1.0))[1] == 1.0
+    for bad in (dict(rope_type="other", factor=2.0), dict(rope_type="linear", factor=0.5)):
+        with pytest.raises(ValueError):
+            rotary_frequencies(64, scaling=bad)
+    for dim in (0, 3):
+        with pytest.raises(ValueError):
+            rotary_frequencies(dim)
