@@ -3,23 +3,30 @@
 // out = sum_j softmax_j(scale q.k_j) v_j with k_j = ks[b] * ck_j, v_j = vs[b] * cv_j: codes
 // c in 8 bits, scales by (block b, KV head).  One pass, with a running maximum.  The scales
 // never touch the codes: ks multiplies the logit after its dot product, and vs joins the
-// weight as an exponent, w_j = 2^(s_j + log2 vs - m'), which has its own running maximum m'
-// beside the softmax's m; the two meet once, at the end.  So the matrix products run on the
-// codes, which fp16 holds exactly.
+// weight as an exponent, w_j = 2^(s_j + log2 vs - m'), which has its own reference m' beside
+// the softmax's m; the two meet once, at the end.  So the matrix products run on the codes,
+// which fp16 holds exactly.
 //
-// Precision: fp16 products with fp32 sums.  The other operands are split in two fp16 terms,
-// x = hi + lo / 4096 (22 bits): the query rows after a power of two brings each row to
-// [1, 2), and the weights, which lie in [0, 1].  The two terms fill rows 0-7 and 8-15 of one
-// m16n8k16 product, whose 16 rows the few rows of a KV head (its query heads times the new
-// tokens) leave half empty anyway, so the second term costs nothing.  The products of one
-// step are summed by the tensor core and added to the output in fp32 with rounding (the
-// tensor core truncates, which over thousands of steps would lean one way).
+// Products: m16n8k16 in fp16 with fp32 sums, tokens (or value dimensions) as the 16 rows of the
+// left operand and 8 query rows (a KV head's query heads times the new tokens) as the
+// columns, so few rows waste nothing: logits^T = K Q^T, out^T = V^T P^T.  The weights come out
+// of the first product with tokens by rows and go into the second with tokens by pairs: one
+// 8 x 8 transposition (movmatrix) per 8 tokens.
+//
+// Precision: a query row is brought to [2^14, 2^15) by a power of two, the weights to at most
+// 2^15, and both are rounded to fp16 once for bf16 queries (2^-12, against 2^-9 of the
+// output's own rounding; a bf16 query is exact in fp16).  fp16 and fp32 queries take two fp16
+// terms each, hi + lo (22 bits), at twice the products; there the products of one step are also
+// summed apart and added in fp32 with rounding, because the tensor core's own sums truncate.
+//
+// The references m, m' only move when a logit passes them by more than 2^kSlack, so a step
+// usually costs one vote instead of the reductions and the rescaling.
 //
 // Split: the unit of work is 32 tokens of one (sequence, KV head, tile of query rows).  All
 // units stand in one line, which is cut evenly into one piece per CTA and then per warp, so a
 // ragged batch, a single long sequence and a large batch fill the GPU alike, from lengths
 // that only the device knows.  Each warp runs on its own: it copies its tokens' codes with
-// cp.async into its own ring of shared memory (kStages - 1 steps ahead) and multiplies from
+// cp.async into its own ring of shared memory, a step or two ahead, and multiplies from
 // there.  Pieces of one unit are merged in the CTA, then across CTAs by k_attend_merge in
 // ascending order: no atomics, and the same bits every time.
 //
@@ -29,15 +36,22 @@
 
 namespace ckv {
 
-constexpr int kAttWarps = 8;
-constexpr int kAttStep = 32;     // tokens per step
-constexpr int kAttStages = 3;
+constexpr int kAttStep = 32;      // tokens per step
 constexpr int kAttMaxCtas = 148;
+constexpr int kAttMaxWarps = 12;
+constexpr float kNone = -3e38f;   // a running maximum that has seen nothing
+constexpr float kSlack = 6.f;     // weights may pass their reference by 2^kSlack
+constexpr float kTop = 9.f;       // and stand at 2^kTop there: at most 2^15 in fp16
+
+// Warps and ring stages of a CTA: 12 x 2 steps of 8 KB where the registers allow 12 warps
+// (8 query rows in one term), else 8 x 3.
+__host__ __device__ constexpr int att_warps(int nt, int terms) { return nt * terms == 1 ? 12 : 8; }
+__host__ __device__ constexpr int att_stages(int nt, int terms) { return nt * terms == 1 ? 2 : 3; }
 
 struct AttArgs {
   ckv_cache c;
   ckv_attention_args a;
-  float* ws;                     // [ctas][kAttWarps + 2] partial results
+  float* ws;                     // [ctas][kAttMaxWarps + 2] partial results
   int4* desc;                    // [ctas][2]: what k_attend_merge has to merge from this CTA on
   int block_log2, group, ctas;
 };
@@ -47,7 +61,10 @@ __host__ __device__ constexpr int part_floats(int D, int rows) { return rows * (
 
 // ---- small pieces -------------------------------------------------------------------
 CKV_DEV uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-CKV_DEV void cp16(uint32_t dst, const void* src, uint32_t bytes) {   // bytes 0: zero fill, src not read
+CKV_DEV void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+CKV_DEV void cp16_or_zero(uint32_t dst, const void* src, uint32_t bytes) {   // bytes 0: zero fill, src not read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 CKV_DEV void cp4(uint32_t dst, const void* src) {
@@ -71,9 +88,25 @@ CKV_DEV float lds1(uint32_t a) {
   return v;
 }
 CKV_DEV void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+CKV_DEV void mma16816_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {   // d = a b
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// 8 x 8 fp16 transposition: lane (g, t) gives (row g, columns 2t, 2t + 1) and gets (rows 2t,
+// 2t + 1, column g).
+CKV_DEV uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+CKV_DEV uint32_t half2_bits(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 // Four codes to two fp16 pairs, exactly.
 template <int kFmt> CKV_DEV void codes4(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -90,15 +123,13 @@ template <int kFmt> CKV_DEV void codes4(uint32_t w, uint32_t& lo, uint32_t& hi) 
     hi = *reinterpret_cast<const uint32_t*>(&y);
   }
 }
-// (x, y) as two fp16 pairs: x ~ hi + lo / 4096.
+// (x, y) ~ hi + lo as two fp16 pairs.
 CKV_DEV void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __floats2half2_rn(x, y);
   const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn((x - f.x) * 4096.f, (y - f.y) * 4096.f);
   hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = *reinterpret_cast<const uint32_t*>(&l);
+  lo = half2_bits(x - f.x, y - f.y);
 }
-constexpr float kLo = 1.f / 4096.f;
 
 // A position in the line of units.
 struct Place {
@@ -164,7 +195,7 @@ CKV_DEV void row_home(const AttArgs& p, int q0, int head, int rho, int64_t& out,
   lse = (int64_t)(q0 + i) * (p.c.num_kv_heads * p.group) + hq;
 }
 // The factor on a row's sums and its log-sum-exp, from its maxima (base 2) and its sum.
-CKV_DEV float row_factor(float m, float mw, float l) { return l > 0.f || isnan(l) ? exp2f(mw - m) / l : 0.f; }
+CKV_DEV float row_factor(float m, float mw, float l) { return l > 0.f || isnan(l) ? exp2f(mw - m - kTop) / l : 0.f; }
 CKV_DEV float row_lse(float m, float l) { return l > 0.f || isnan(l) ? (m + log2f(l)) * kLn2 : -INFINITY; }
 
 // Merge of `count` partial results of one unit, part(i) their places, by the warps of a CTA
@@ -177,7 +208,7 @@ CKV_DEV void merge_parts(const AttArgs& p, F part, int count, int w0, int nw, fl
   for (int row = w0; row < 8 * NT; row += nw) {
     const int rho = tile * 8 * NT + row;
     if (!dst && rho >= nq * p.group) break;
-    float m = -INFINITY, mw = -INFINITY;
+    float m = kNone, mw = kNone;
     for (int i = lane; i < count; i += 32) {
       const float* s = part(i) + row * 4;
       m = fmaxf(m, get(s));
@@ -185,16 +216,24 @@ CKV_DEV void merge_parts(const AttArgs& p, F part, int count, int w0, int nw, fl
     }
     m = warp_max(m);
     mw = warp_max(mw);
-    const float m0 = m == -INFINITY ? 0.f : m, mw0 = mw == -INFINITY ? 0.f : mw;
     float l = 0.f, o[PER] = {};
-    for (int i = 0; i < count; ++i) {
-      const float* s = part(i) + row * 4;
-      l += get(s + 2) * exp2f(get(s) - m0);
-      const float f = exp2f(get(s + 1) - mw0);
-      const float* x = part(i) + 8 * NT * 4 + row * D + lane * PER;
+    for (int i0 = 0; i0 < count; i0 += 32) {   // lane i weighs part i0 + i, then all lanes add up the parts
+      float f = 0.f;
+      if (i0 + lane < count) {
+        const float* s = part(i0 + lane) + row * 4;
+        l += get(s + 2) * exp2f(get(s) - m);
+        f = exp2f(get(s + 1) - mw);
+      }
+      const int nn = min(32, count - i0);
+#pragma unroll 4
+      for (int i = 0; i < nn; ++i) {
+        const float fi = __shfl_sync(0xffffffffu, f, i);
+        const float* x = part(i0 + i) + 8 * NT * 4 + row * D + lane * PER;
 #pragma unroll
-      for (int e = 0; e < PER; ++e) o[e] += get(x + e) * f;
+        for (int e = 0; e < PER; ++e) o[e] += get(x + e) * fi;
+      }
     }
+    l = warp_sum(l);
     if (dst) {
       if (lane == 0) { dst[row * 4] = m; dst[row * 4 + 1] = mw; dst[row * 4 + 2] = l; }
 #pragma unroll
@@ -202,7 +241,7 @@ CKV_DEV void merge_parts(const AttArgs& p, F part, int count, int w0, int nw, fl
     } else {
       int64_t at, lat;
       row_home(p, q0, head, rho, at, lat);
-      const float f = row_factor(m, mw0, l);
+      const float f = row_factor(m, mw, l);
       if constexpr (PER == 4) {
         store_out4(p.a.out, p.a.dtype, at + lane * 4, make_float4(o[0] * f, o[1] * f, o[2] * f, o[3] * f));
       } else {
@@ -221,41 +260,46 @@ struct Entry {     // a piece of a unit that ended in this CTA without being the
   const float* part;
 };
 
-template <int D, int kFmt, int NT>
-__global__ void __launch_bounds__(kAttWarps * 32, 1) k_attend(const AttArgs p) {
+// NT tiles of 8 query rows share the codes that a warp has converted; kTerms fp16 terms.
+template <int D, int kFmt, int NT, int kTerms>
+__global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const AttArgs p) {
+  constexpr int kWarps = att_warps(NT, kTerms), kStages = att_stages(NT, kTerms);
   constexpr int kSteps16 = D / 16;               // k16 steps of the logit product
-  constexpr int kDims = D / 8;                   // dims of one lane group, n8 tiles of the output
+  constexpr int kTiles = D / 16;                 // m16 tiles of the output
   constexpr int kStageBytes = 2 * kAttStep * D;  // K then V
-  constexpr int kRing = kAttStages * kStageBytes;
+  constexpr int kRing = kStages * kStageBytes;
+  constexpr int kAhead = 2;                      // steps in flight: the ring's third stage is refilled before a step's
+                                                 // products, the second of two after them
+  static_assert(kStages == 2 || kStages == 3, "ring");
   constexpr int kPart = part_floats(D, 8 * NT);
   extern __shared__ __align__(128) char att_smem[];
-  __shared__ float s_scale[kAttWarps][kAttStages][4];   // K, V of the step's first and second 16 tokens
-  __shared__ Entry s_entry[2 * kAttWarps];
-  __shared__ Place s_place[kAttWarps];
-  __shared__ int s_scan[32];
-  __shared__ long long s_tot[kAttWarps];
+  __shared__ float s_scale[kWarps][kStages][4];  // K, V of the step's first and second 16 tokens
+  __shared__ Entry s_entry[2 * kWarps];
+  __shared__ Place s_place[kWarps];
+  __shared__ long long s_tot[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x, R = p.a.requests;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (tid < 2 * kAttWarps) s_entry[tid].used = 0;
+  if (tid < 2 * kWarps) s_entry[tid].used = 0;
   if (tid < 2) p.desc[cta * 2 + tid] = make_int4(0, 0, 0, 0);
 
   // ---- the line of units: its length, and where this CTA's warps stand in it
-  long long total = 0;
-  for (int r = tid; r < R; r += kAttWarps * 32) total += seq_work<NT>(p, r);
+  const long long first = tid < R ? seq_work<NT>(p, tid) : 0;
+  long long total = first;
+  for (int r = tid + kWarps * 32; r < R; r += kWarps * 32) total += seq_work<NT>(p, r);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane == 0) s_tot[wid] = total;
   __syncthreads();
   total = 0;
-  for (int w = 0; w < kAttWarps; ++w) total += s_tot[w];
-  const int nctas = (int)min((long long)p.ctas, (total + kAttWarps - 1) / kAttWarps);
+  for (int w = 0; w < kWarps; ++w) total += s_tot[w];
+  const int nctas = (int)min((long long)p.ctas, (total + kWarps - 1) / kWarps);
   const long long c0 = cta < nctas ? total * cta / nctas : total, c1 = cta < nctas ? total * (cta + 1) / nctas : total;
-  auto warp_at = [&](int w) { return c0 + (c1 - c0) * w / kAttWarps; };
+  auto warp_at = [&](int w) { return c0 + (c1 - c0) * w / kWarps; };
   long long before = 0;   // work of the sequences before this chunk of threads
-  for (int base = 0; base < R; base += kAttWarps * 32) {
+  for (int base = 0; base < R && before < c1; base += kWarps * 32) {
     const int r = base + tid;
-    const long long mine = r < R ? seq_work<NT>(p, r) : 0;
+    const long long mine = base == 0 ? first : r < R ? seq_work<NT>(p, r) : 0;
     long long x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -267,43 +311,49 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) k_attend(const AttArgs p) {
     __syncthreads();
     long long at = before;
     for (int w = 0; w < wid; ++w) at += s_tot[w];
-    for (int w = 0; w < kAttWarps; ++w) before += s_tot[w];
+    for (int w = 0; w < kWarps; ++w) before += s_tot[w];
     at += x - mine;
-    if (r < R) {
+    if (mine > 0 && at < c1 && at + mine > c0) {
       Place pl;
       pl.r = r;
       pl.n = seq_len(p, r);
       seq_queries(p, r, pl.q0, pl.nq);
       pl.units = seq_units<NT>(p, pl.nq);
       pl.steps = (pl.n + kAttStep - 1) / kAttStep;
-      for (int w = 0; w < kAttWarps; ++w) {
+      for (int w = 0; w < kWarps; ++w) {
         const long long a = warp_at(w);
-        if (mine > 0 && a >= at && a < at + mine && a < c1) {
+        if (a >= at && a < at + mine && a < c1) {
           pl.unit = (int)((a - at) / pl.steps);
           pl.step = (int)((a - at) % pl.steps);
           s_place[w] = pl;
         }
       }
-      // sequences with nothing to see: zeros
-      if (pl.n == 0 && r % (int)gridDim.x == cta) {
-        for (int i = 0; i < pl.nq; ++i)
-          for (int hq = 0; hq < p.c.num_kv_heads * p.group; ++hq) {
-            const int64_t o = (pl.q0 + i) * p.a.out_tok_stride + hq * p.a.out_head_stride;
-            for (int d = 0; d < D; d += 4) store_out4(p.a.out, p.a.dtype, o + d, make_float4(0.f, 0.f, 0.f, 0.f));
-            if (p.a.lse) p.a.lse[(int64_t)(pl.q0 + i) * (p.c.num_kv_heads * p.group) + hq] = -INFINITY;
-          }
-      }
     }
   }
   __syncthreads();
+  // sequences with nothing to see: zeros
+  for (int r = cta; r < R; r += gridDim.x)
+    if (seq_len(p, r) == 0) {
+      int q0, nq;
+      seq_queries(p, r, q0, nq);
+      const int hq = p.c.num_kv_heads * p.group;
+      for (int i = tid; i < nq * hq * (D / 4); i += kWarps * 32) {
+        const int row = i / (D / 4), d = i % (D / 4) * 4, tok = q0 + row / hq, h = row % hq;
+        store_out4(p.a.out, p.a.dtype, tok * p.a.out_tok_stride + h * p.a.out_head_stride + d, make_float4(0.f, 0.f, 0.f, 0.f));
+        if (p.a.lse && d == 0) p.a.lse[(int64_t)tok * hq + h] = -INFINITY;
+      }
+    }
 
   // ---- this warp's piece
   long long left = warp_at(wid + 1) - warp_at(wid);
   char* ring = att_smem + wid * kRing;
   const uint32_t ring_a = smem_u32(ring), scale_a = smem_u32(&s_scale[wid][0][0]);
-  auto swz = [&](int row, int chunk) -> uint32_t {   // 16-byte chunk of a row: no bank conflicts by rows or by columns
+  // 16-byte chunk of a row, so that neither reads by rows nor reads by columns meet in a bank
+  auto swz = [&](int row, int chunk) -> uint32_t {
     return D == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
   };
+  constexpr int kChunks = D / 16, kRows = 32 / kChunks;   // of one copy instruction
+  const int crow = lane / kChunks, cchunk = lane % kChunks;
   if (left > 0) {
     Place pl = s_place[wid];
     bool first_piece = true;
@@ -316,8 +366,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) k_attend(const AttArgs p) {
       const int n = pl.n;
       const int32_t* table = p.a.tables + pl.r * p.a.table_stride;
       const int pages = (n + (1 << p.block_log2) - 1) >> p.block_log2;
-      const char* kh = static_cast<const char*>(p.c.k) + head * p.c.k_head_stride;
-      const char* vh = static_cast<const char*>(p.c.v) + head * p.c.v_head_stride;
+      const char* kh = static_cast<const char*>(p.c.k) + head * p.c.k_head_stride + crow * p.c.k_tok_stride + cchunk * 16;
+      const char* vh = static_cast<const char*>(p.c.v) + head * p.c.v_head_stride + crow * p.c.v_tok_stride + cchunk * 16;
 
       // block ids: lane l holds page pbase + l, and the next 32 pages stand by
       int pbase = (s_begin * kAttStep) >> p.block_log2;
@@ -335,231 +385,258 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) k_attend(const AttArgs p) {
               pnext = page(pbase + 32 + lane);
             }
             const int blk = __shfl_sync(0xffffffffu, pcur, pi - pbase);
-            const bool good = blk >= 0 && blk < p.c.num_blocks;
+            const bool good = (uint32_t)blk < (uint32_t)p.c.num_blocks;
             const int64_t b = good ? blk : 0;
             const int off = tok0 & ((1 << p.block_log2) - 1);
-            constexpr int kChunks = D / 16, kRows = 32 / kChunks;
-            const int row = lane / kChunks, chunk = lane % kChunks;
-            const char* ks = kh + b * p.c.k_block_stride + (off + row) * p.c.k_tok_stride + chunk * 16;
-            const char* vs = vh + b * p.c.v_block_stride + (off + row) * p.c.v_tok_stride + chunk * 16;
+            const int have = good ? n - tok0 : 0;   // rows of these 16 that hold tokens
+            const char* ks = kh + b * p.c.k_block_stride + off * p.c.k_tok_stride;
+            const char* vs = vh + b * p.c.v_block_stride + off * p.c.v_tok_stride;
+            if (have >= 16) {
 #pragma unroll
-            for (int i = 0; i < 16 / kRows; ++i) {
-              const bool in = good && tok0 + i * kRows + row < n;
-              const uint32_t d = st + swz(half * 16 + i * kRows + row, chunk);
-              cp16(d, in ? ks + i * kRows * p.c.k_tok_stride : kh, in ? 16u : 0u);
-              cp16(d + kAttStep * D, in ? vs + i * kRows * p.c.v_tok_stride : vh, in ? 16u : 0u);
+              for (int i = 0; i < 16 / kRows; ++i) {
+                const uint32_t d = st + swz(half * 16 + i * kRows + crow, cchunk);
+                cp16(d, ks + i * kRows * p.c.k_tok_stride);
+                cp16(d + kAttStep * D, vs + i * kRows * p.c.v_tok_stride);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16 / kRows; ++i) {
+                const uint32_t in = i * kRows + crow < have ? 16u : 0u;
+                const uint32_t d = st + swz(half * 16 + i * kRows + crow, cchunk);
+                cp16_or_zero(d, in ? ks + i * kRows * p.c.k_tok_stride : kh, in);
+                cp16_or_zero(d + kAttStep * D, in ? vs + i * kRows * p.c.v_tok_stride : vh, in);
+              }
             }
             if (lane < 2) {
-              const float* sc = (lane ? p.c.v_scale : p.c.k_scale) + b * p.c.num_kv_heads + head;
-              const uint32_t d = scale_a + (stage * 4 + half * 2 + lane) * 4;
-              if (good && tok0 < n) cp4(d, sc);
+              if (have > 0) cp4(scale_a + (stage * 4 + half * 2 + lane) * 4, (lane ? p.c.v_scale : p.c.k_scale) + b * p.c.num_kv_heads + head);
               else s_scale[wid][stage][half * 2 + lane] = tok0 < n ? __uint_as_float(0x7fffffffu) : 0.f;   // a bad page reads as NaN
             }
           }
         }
         cp_commit();
       };
-#pragma unroll
-      for (int i = 0; i < kAttStages - 1; ++i) issue(s_begin + i, i);
 
-      // query rows: row g of each tile, split in two fp16 terms
-      uint32_t qf[NT][kSteps16][4];
-      float qs[NT];           // scale * log2 e * the row's power of two
-      int see[NT];            // tokens that the row sees
+      // query rows: lane (g, t) loads row g's dimensions of its chunks
+      uint32_t qf[NT][kTerms][kSteps16][2];
+      float qs[NT][2];        // rows 2t, 2t + 1: scale * log2 e * the row's power of two
+      int see[NT][2];         // tokens that they see
       int see_min = n;
+      float4 x[NT][kSteps16];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int rho = (tile * NT + nt) * 8 + g;
-        const bool real = rho < rows;
         const int i = rho / p.group, hq = head * p.group + rho % p.group;
-        float4 x[kSteps16];
-        float top = 0.f;
 #pragma unroll
         for (int k = 0; k < kSteps16; ++k) {
           const int dim = D == 128 ? (2 * t + k / 4) * 16 + (k & 3) * 4 : t * 16 + k * 4;
-          x[k] = real ? load_q4(p.a.q, p.a.dtype, (pl.q0 + i) * p.a.q_tok_stride + hq * p.a.q_head_stride + dim)
-                      : make_float4(0.f, 0.f, 0.f, 0.f);
-          top = fmaxf(fmaxf(fmaxf(top, fabsf(x[k].x)), fmaxf(fabsf(x[k].y), fabsf(x[k].z))), fabsf(x[k].w));
+          x[nt][k] = rho < rows ? load_q4(p.a.q, p.a.dtype, (pl.q0 + i) * p.a.q_tok_stride + hq * p.a.q_head_stride + dim)
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
         }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) issue(s_begin + i, i);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int rho = (tile * NT + nt) * 8 + g;
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < kSteps16; ++k)
+          top = fmaxf(fmaxf(fmaxf(top, fabsf(x[nt][k].x)), fmaxf(fabsf(x[nt][k].y), fabsf(x[nt][k].z))), fabsf(x[nt][k].w));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);   // biased exponent
-        const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-        qs[nt] = p.a.scale * kLog2e * __uint_as_float((uint32_t)e << 23);
-        see[nt] = real && p.a.causal ? n - pl.nq + i + 1 : n;
-        see_min = min(see_min, see[nt]);
+        // the row times 2^(14 - exponent); exponents at the ends of the range are clamped
+        const int e = min(max((int)(__float_as_uint(top) >> 23), 16), 254);   // biased
+        const float up = __uint_as_float((uint32_t)(268 - e) << 23);
+        const float mine = p.a.scale * kLog2e / up;
+        const int sees = rho < rows && p.a.causal ? n - pl.nq + rho / p.group + 1 : n;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          qs[nt][r] = __shfl_sync(0xffffffffu, mine, (2 * t + r) * 4);
+          see[nt][r] = __shfl_sync(0xffffffffu, sees, (2 * t + r) * 4);
+          see_min = min(see_min, see[nt][r]);
+        }
 #pragma unroll
         for (int k = 0; k < kSteps16; ++k) {
-          split2(x[k].x * down, x[k].y * down, qf[nt][k][0], qf[nt][k][1]);
-          split2(x[k].z * down, x[k].w * down, qf[nt][k][2], qf[nt][k][3]);
+          const float4 v = x[nt][k];
+          if constexpr (kTerms == 1) {
+            qf[nt][0][k][0] = half2_bits(v.x * up, v.y * up);
+            qf[nt][0][k][1] = half2_bits(v.z * up, v.w * up);
+          } else {
+            split2(v.x * up, v.y * up, qf[nt][0][k][0], qf[nt][1][k][0]);
+            split2(v.z * up, v.w * up, qf[nt][0][k][1], qf[nt][1][k][1]);
+          }
         }
       }
       see_min = __reduce_min_sync(0xffffffffu, see_min);
 
-      float o[NT][kDims][2];
-      float m[NT], mw[NT], l[NT];
+      // out^T: tile i has dims (g * kTiles * 2 + 2 i, + 1) x rows (2t, 2t + 1)
+      float o[NT][kTiles][4];
+      float m[NT][2], mw[NT][2], l[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        m[nt] = mw[nt] = -INFINITY;
-        l[nt] = 0.f;
 #pragma unroll
-        for (int j = 0; j < kDims; ++j) o[nt][j][0] = o[nt][j][1] = 0.f;
+        for (int r = 0; r < 2; ++r) { m[nt][r] = mw[nt][r] = kNone; l[nt][r] = 0.f; }
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
       }
 
       int stage = 0;
       for (int s = s_begin; s < s_end; ++s) {
-        cp_wait<kAttStages - 2>();
+        cp_wait<kAhead - 1>();
         __syncwarp();
-        {
-          const int ahead = stage == 0 ? kAttStages - 1 : stage - 1;
-          issue(s + kAttStages - 1, ahead);
-        }
+        if constexpr (kStages > 2) issue(s + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
         const uint32_t kst = ring_a + stage * kStageBytes, vst = kst + kAttStep * D;
-        // logits
-        float sc[NT][4][4];
+        // logits^T: lane holds tokens g, g + 8 of each 16 x rows 2t, 2t + 1
+        float sc[NT][2][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) sc[nt][j][0] = sc[nt][j][1] = sc[nt][j][2] = sc[nt][j][3] = 0.f;
-          const int row = j * 8 + g;
+        for (int u = 0; u < 2; ++u) {
+          const int row = u * 16 + g;
 #pragma unroll
           for (int c = 0; c < D / 64; ++c) {
-            const uint4 w = lds4(kst + swz(row, D == 128 ? 2 * t + c : t));
-            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+            const uint4 wa = lds4(kst + swz(row, D == 128 ? 2 * t + c : t)), wb = lds4(kst + swz(row + 8, D == 128 ? 2 * t + c : t));
+            const uint32_t a4[4] = {wa.x, wa.y, wa.z, wa.w}, b4[4] = {wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              uint32_t b0, b1;
-              codes4<kFmt>(ww[e], b0, b1);
+              uint32_t a[4];
+              codes4<kFmt>(a4[e], a[0], a[2]);
+              codes4<kFmt>(b4[e], a[1], a[3]);
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma16816(sc[nt][j], qf[nt][c * 4 + e], b0, b1);
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < kTerms; ++k) {
+                  const uint32_t(&b)[2] = qf[nt][k][c * 4 + e];
+                  if (c == 0 && e == 0 && k == 0) mma16816_zero(sc[nt][u], a, b[0], b[1]);
+                  else mma16816(sc[nt][u], a, b[0], b[1]);
+                }
             }
           }
         }
-        float ks[2], ve[2], vm[2];
+        float ks[2], ve[2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          ks[half] = lds1(scale_a + (stage * 4 + half * 2) * 4);
-          const float v = lds1(scale_a + (stage * 4 + half * 2 + 1) * 4);
-          const uint32_t u = __float_as_uint(v);
-          vm[half] = __uint_as_float((u & 0x7fffffu) | 0x3f800000u);
-          ve[half] = isnan(v) ? v : (float)((int)(u >> 23 & 255u) - 127);
+        for (int u = 0; u < 2; ++u) {
+          ks[u] = lds1(scale_a + (stage * 4 + u * 2) * 4);
+          const float v = lds1(scale_a + (stage * 4 + u * 2 + 1) * 4);
+          const uint32_t bits = __float_as_uint(v), mant = bits & 0x7fffffu;
+          ve[u] = (float)((int)(bits >> 23 & 255u) - 127);
+          if (mant) ve[u] = isnan(v) ? v : ve[u] + __log2f(__uint_as_float(mant | 0x3f800000u));   // not a power of two
         }
         const bool masked = (s + 1) * kAttStep > see_min;
-        uint32_t pf[NT][2][4];
+        bool past = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float x[4][2], y[4][2];   // logit, and logit + log2 of the value scale (base 2)
-          float mn = m[nt], mwn = mw[nt];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float f = qs[nt] * ks[j >> 1];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              x[j][e] = fmaf(sc[nt][j][2 + e], kLo, sc[nt][j][e]) * f;
-              y[j][e] = x[j][e] + ve[j >> 1];
-              if (masked && s * kAttStep + j * 8 + 2 * t + e >= see[nt]) x[j][e] = y[j][e] = -INFINITY;
-              mn = fmaxf(mn, x[j][e]);
-              mwn = fmaxf(mwn, y[j][e]);
-            }
-          }
-          mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 1));
-          mwn = fmaxf(mwn, __shfl_xor_sync(0xffffffffu, mwn, 1));
-          mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, 2));
-          mwn = fmaxf(mwn, __shfl_xor_sync(0xffffffffu, mwn, 2));
-          const float m0 = mn == -INFINITY ? 0.f : mn, mw0 = mwn == -INFINITY ? 0.f : mwn;
-          if (__any_sync(0xffffffffu, mn > m[nt] || mwn > mw[nt])) {
-            l[nt] *= ex2(m[nt] - m0);
-            const float f = ex2(mw[nt] - mw0);
-#pragma unroll
-            for (int j = 0; j < kDims; ++j) { o[nt][j][0] *= f; o[nt][j][1] *= f; }
-            m[nt] = mn;
-            mw[nt] = mwn;
-          }
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int jj = 0; jj < 2; ++jj) {
-              const int j = 2 * u + jj;
-              l[nt] += ex2(x[j][0] - m0) + ex2(x[j][1] - m0);
-              const float w0 = ex2(y[j][0] - mw0) * vm[u], w1 = ex2(y[j][1] - mw0) * vm[u];
-              split2(w0, w1, pf[nt][u][2 * jj], pf[nt][u][2 * jj + 1]);
+            for (int r = 0; r < 2; ++r) {
+              const float f = qs[nt][r] * ks[u];
+              sc[nt][u][r] *= f;
+              sc[nt][u][2 + r] *= f;
+              if (masked) {
+                const int tok = s * kAttStep + u * 16 + g;
+                if (tok >= see[nt][r]) sc[nt][u][r] = -INFINITY;
+                if (tok + 8 >= see[nt][r]) sc[nt][u][2 + r] = -INFINITY;
+              }
+              const float h = fmaxf(sc[nt][u][r], sc[nt][u][2 + r]);
+              past = past || h > m[nt][r] + kSlack || h + ve[u] > mw[nt][r] + kSlack;
+            }
+        if (__any_sync(0xffffffffu, past)) {
+          // the rows that passed theirs get new references (whole numbers: the rescaling is exact),
+          // the same in all lanes of a row and whatever the other rows do
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float h0 = fmaxf(sc[nt][0][r], sc[nt][0][2 + r]), h1 = fmaxf(sc[nt][1][r], sc[nt][1][2 + r]);
+              float nm = fmaxf(m[nt][r], fmaxf(h0, h1)), nw = fmaxf(mw[nt][r], fmaxf(h0 + ve[0], h1 + ve[1]));
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) {
+                nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, d));
+                nw = fmaxf(nw, __shfl_xor_sync(0xffffffffu, nw, d));
+              }
+              nm = nm > m[nt][r] + kSlack ? ceilf(nm) : m[nt][r];
+              nw = nw > mw[nt][r] + kSlack ? ceilf(nw) : mw[nt][r];
+              l[nt][r] *= ex2(m[nt][r] - nm);
+              const float f = ex2(mw[nt][r] - nw);
+              m[nt][r] = nm;
+              mw[nt][r] = nw;
+#pragma unroll
+              for (int j = 0; j < kTiles; ++j) { o[nt][j][r] *= f; o[nt][j][2 + r] *= f; }
             }
         }
-        // values: lane (g, t) takes dims g * kDims .. of tokens 2t, 2t + 1, 2t + 8, 2t + 9 of each 16
-        if constexpr (D == 128) {
-          uint4 v[2][4];
+        uint32_t pf[NT][kTerms][2][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = e & 1;
+              l[nt][r] += ex2(sc[nt][u][e] - m[nt][r]);
+              w[e] = ex2(sc[nt][u][e] + (ve[u] - mw[nt][r] + kTop));
+              if (masked && sc[nt][u][e] == -INFINITY) w[e] = 0.f;   // whatever the scale
+            }
+            if constexpr (kTerms == 1) {
+              pf[nt][0][u][0] = transpose8(half2_bits(w[0], w[1]));
+              pf[nt][0][u][1] = transpose8(half2_bits(w[2], w[3]));
+            } else {
+              uint32_t h0, l0, h1, l1;
+              split2(w[0], w[1], h0, l0);
+              split2(w[2], w[3], h1, l1);
+              pf[nt][0][u][0] = transpose8(h0);
+              pf[nt][0][u][1] = transpose8(h1);
+              pf[nt][1][u][0] = transpose8(l0);
+              pf[nt][1][u][1] = transpose8(l1);
+            }
+          }
+        // values: lane (g, t) takes dims g * 2 kTiles .. of tokens 2t, 2t + 1, 2t + 8, 2t + 9 of each 16
+        uint32_t v[2][4][D / 32];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = u * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
+            if constexpr (D == 128) {
+              const uint4 q = lds4(vst + swz(row, g));
+              v[u][i][0] = q.x; v[u][i][1] = q.y; v[u][i][2] = q.z; v[u][i][3] = q.w;
+            } else {
+              const uint2 q = lds2(vst + swz(row, g >> 1) + (g & 1) * 8);
+              v[u][i][0] = q.x; v[u][i][1] = q.y;
+            }
+          }
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {   // 4 dims, two tiles
+          uint32_t a[2][2][4];               // [u][tile]
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[u][i] = lds4(vst + swz(u * 16 + 2 * t + (i & 1) + (i >> 1) * 8, g));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float acc[NT][4][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) acc[nt][k][0] = acc[nt][k][1] = acc[nt][k][2] = acc[nt][k][3] = 0.f;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              uint32_t w[4], b0[4], b1[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) w[i] = e == 0 ? v[u][i].x : e == 1 ? v[u][i].y : e == 2 ? v[u][i].z : v[u][i].w;
-              codes4<kFmt>(__byte_perm(w[0], w[1], 0x5140), b0[0], b0[1]);
-              codes4<kFmt>(__byte_perm(w[0], w[1], 0x7362), b0[2], b0[3]);
-              codes4<kFmt>(__byte_perm(w[2], w[3], 0x5140), b1[0], b1[1]);
-              codes4<kFmt>(__byte_perm(w[2], w[3], 0x7362), b1[2], b1[3]);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) mma16816(acc[nt][k], pf[nt][u], b0[k], b1[k]);
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t sel = h ? 0x7362 : 0x5140;
+              codes4<kFmt>(__byte_perm(v[u][0][e], v[u][1][e], sel), a[u][h][0], a[u][h][1]);
+              codes4<kFmt>(__byte_perm(v[u][2][e], v[u][3][e], sel), a[u][h][2], a[u][h][3]);
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                o[nt][e * 4 + k][0] += fmaf(acc[nt][k][2], kLo, acc[nt][k][0]);
-                o[nt][e * 4 + k][1] += fmaf(acc[nt][k][3], kLo, acc[nt][k][1]);
+            for (int h = 0; h < 2; ++h) {
+              float(&acc)[4] = o[nt][2 * e + h];
+              if constexpr (kTerms == 1) {
+                mma16816(acc, a[0][h], pf[nt][0][0][0], pf[nt][0][0][1]);
+                mma16816(acc, a[1][h], pf[nt][0][1][0], pf[nt][0][1][1]);
+              } else {
+                float d[4];
+                mma16816_zero(d, a[0][h], pf[nt][1][0][0], pf[nt][1][0][1]);
+                mma16816(d, a[1][h], pf[nt][1][1][0], pf[nt][1][1][1]);
+                mma16816(d, a[0][h], pf[nt][0][0][0], pf[nt][0][0][1]);
+                mma16816(d, a[1][h], pf[nt][0][1][0], pf[nt][0][1][1]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] += d[k];
               }
-          }
-        } else {
-          uint2 v[2][4];
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              v[u][i] = lds2(vst + swz(u * 16 + 2 * t + (i & 1) + (i >> 1) * 8, g >> 1) + (g & 1) * 8);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float acc[NT][4][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) acc[nt][k][0] = acc[nt][k][1] = acc[nt][k][2] = acc[nt][k][3] = 0.f;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              uint32_t w[4], b0[4], b1[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) w[i] = e == 0 ? v[u][i].x : v[u][i].y;
-              codes4<kFmt>(__byte_perm(w[0], w[1], 0x5140), b0[0], b0[1]);
-              codes4<kFmt>(__byte_perm(w[0], w[1], 0x7362), b0[2], b0[3]);
-              codes4<kFmt>(__byte_perm(w[2], w[3], 0x5140), b1[0], b1[1]);
-              codes4<kFmt>(__byte_perm(w[2], w[3], 0x7362), b1[2], b1[3]);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) mma16816(acc[nt][k], pf[nt][u], b0[k], b1[k]);
             }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                o[nt][e * 4 + k][0] += fmaf(acc[nt][k][2], kLo, acc[nt][k][0]);
-                o[nt][e * 4 + k][1] += fmaf(acc[nt][k][3], kLo, acc[nt][k][1]);
-              }
-          }
         }
         __syncwarp();   // the stage may be filled again
-        stage = stage == kAttStages - 1 ? 0 : stage + 1;
+        if constexpr (kStages == 2) issue(s + 2, stage);
+        stage = stage == kStages - 1 ? 0 : stage + 1;
       }
       cp_wait<0>();
       __syncwarp();
@@ -570,42 +647,40 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) k_attend(const AttArgs p) {
       float* part = nullptr;
       if (!(begins && ends)) {
         // the ring is free once the warp has no further piece
-        part = left > 0 ? p.ws + ((size_t)cta * (kAttWarps + 2) + wid) * kPart : reinterpret_cast<float*>(ring);
+        part = left > 0 ? p.ws + ((size_t)cta * (kAttMaxWarps + 2) + wid) * kPart : reinterpret_cast<float*>(ring);
         if (lane == 0) {
           Entry& en = s_entry[2 * wid + (first_piece ? 0 : 1)];
           en.used = 1; en.r = pl.r; en.unit = pl.unit; en.begins = begins; en.ends = ends; en.part = part;
         }
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float lt = l[nt];
-        lt += __shfl_xor_sync(0xffffffffu, lt, 1);
-        lt += __shfl_xor_sync(0xffffffffu, lt, 2);
-        if (part) {
-          const int row = nt * 8 + g;
-          if (t == 0) { part[row * 4] = m[nt]; part[row * 4 + 1] = mw[nt]; part[row * 4 + 2] = lt; }
-          float4* d = reinterpret_cast<float4*>(part + 8 * NT * 4 + row * D + t * 2 * kDims);
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+        for (int r = 0; r < 2; ++r) {
+          float lt = l[nt][r];
 #pragma unroll
-            for (int j = 0; j < kDims; j += 4)
-              d[(e * kDims + j) / 4] = make_float4(o[nt][j][e], o[nt][j + 1][e], o[nt][j + 2][e], o[nt][j + 3][e]);
-        } else {
-          const int rho = (tile * NT + nt) * 8 + g;
-          if (rho < rows) {
-            int64_t at, lat;
-            row_home(p, pl.q0, head, rho, at, lat);
-            const float f = row_factor(m[nt], mw[nt], lt);
+          for (int d = 4; d < 32; d <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, d);
+          const int row = nt * 8 + 2 * t + r;
+          if (part) {
+            if (g == 0) { part[row * 4] = m[nt][r]; part[row * 4 + 1] = mw[nt][r]; part[row * 4 + 2] = lt; }
+            float4* d = reinterpret_cast<float4*>(part + 8 * NT * 4 + row * D + g * 2 * kTiles);
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int j = 0; j < kTiles; j += 2)
+              d[j / 2] = make_float4(o[nt][j][r], o[nt][j][2 + r], o[nt][j + 1][r], o[nt][j + 1][2 + r]);
+          } else {
+            const int rho = tile * NT * 8 + row;
+            if (rho < rows) {
+              int64_t at, lat;
+              row_home(p, pl.q0, head, rho, at, lat);
+              const float f = row_factor(m[nt][r], mw[nt][r], lt);
 #pragma unroll
-              for (int j = 0; j < kDims; j += 4)
-                store_out4(p.a.out, p.a.dtype, at + t * 2 * kDims + e * kDims + j,
-                           make_float4(o[nt][j][e] * f, o[nt][j + 1][e] * f, o[nt][j + 2][e] * f, o[nt][j + 3][e] * f));
-            if (p.a.lse && t == 0) p.a.lse[lat] = row_lse(m[nt], lt);
+              for (int j = 0; j < kTiles; j += 2)
+                store_out4(p.a.out, p.a.dtype, at + g * 2 * kTiles + 2 * j,
+                           make_float4(o[nt][j][r] * f, o[nt][j][2 + r] * f, o[nt][j + 1][r] * f, o[nt][j + 1][2 + r] * f));
+              if (p.a.lse && g == 0) p.a.lse[lat] = row_lse(m[nt][r], lt);
+            }
           }
         }
-      }
       first_piece = false;
       if (left > 0) {   // on to the next unit
         pl.step = 0;
@@ -625,14 +700,14 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) k_attend(const AttArgs p) {
   __syncthreads();
 
   // ---- merge the pieces of each unit within the CTA
-  const float* list[kAttWarps + 1];
-  for (int i = 0; i < 2 * kAttWarps;) {
+  const float* list[kWarps + 1];
+  for (int i = 0; i < 2 * kWarps;) {
     if (!s_entry[i].used) { ++i; continue; }
     const int r = s_entry[i].r, unit = s_entry[i].unit;
     const bool begins = s_entry[i].begins;
     bool ends = false;
     int count = 0;
-    for (; i < 2 * kAttWarps; ++i) {
+    for (; i < 2 * kWarps; ++i) {
       if (!s_entry[i].used) continue;
       if (s_entry[i].r != r || s_entry[i].unit != unit) break;
       list[count++] = s_entry[i].part;
@@ -643,10 +718,9 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) k_attend(const AttArgs p) {
     const int tiles = seq_units<NT>(p, nq) / p.c.num_kv_heads;
     const int head = unit / tiles, tile = unit - head * tiles;
     // a unit that reaches past this CTA leaves its part in slot 0 (begun before) or 1
-    float* dst = begins && ends ? nullptr : p.ws + ((size_t)cta * (kAttWarps + 2) + kAttWarps + (begins ? 1 : 0)) * kPart;
-    merge_parts<D, NT, false>(p, [&](int k) { return list[k]; }, count, wid, kAttWarps, dst, q0, nq, head, tile);
+    float* dst = begins && ends ? nullptr : p.ws + ((size_t)cta * (kAttMaxWarps + 2) + kAttMaxWarps + (begins ? 1 : 0)) * kPart;
+    merge_parts<D, NT, false>(p, [&](int k) { return list[k]; }, count, wid, kWarps, dst, q0, nq, head, tile);
     if (begins && !ends && tid == 0) {
-      // the CTA with the unit's last step: the first whose end is at or past the unit's end
       p.desc[cta * 2] = make_int4(1, r, head, tile);
     }
     if (!begins && tid == 0) p.desc[cta * 2 + 1] = make_int4(1, ends ? 1 : 0, 0, 0);
@@ -655,8 +729,10 @@ __global__ void __launch_bounds__(kAttWarps * 32, 1) k_attend(const AttArgs p) {
 
 // CTA c merges the unit that begins in CTA c of k_attend and reaches past it: its slot 1 and
 // slot 0 of the CTAs that follow, up to the one where it ends.
+constexpr int kMergeWarps = 8;
+
 template <int D, int NT>
-__global__ void __launch_bounds__(kAttWarps * 32) k_attend_merge(const AttArgs p) {
+__global__ void __launch_bounds__(kMergeWarps * 32) k_attend_merge(const AttArgs p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int kPart = part_floats(D, 8 * NT);
   const int cta = blockIdx.x;
@@ -672,29 +748,30 @@ __global__ void __launch_bounds__(kAttWarps * 32) k_attend_merge(const AttArgs p
   int q0, nq;
   seq_queries(p, d.y, q0, nq);
   merge_parts<D, NT, true>(p, [&](int k) {
-    return p.ws + ((size_t)(cta + k) * (kAttWarps + 2) + kAttWarps + (k == 0 ? 1 : 0)) * kPart;
-  }, count, threadIdx.x >> 5, kAttWarps, nullptr, q0, nq, d.z, d.w);
+    return p.ws + ((size_t)(cta + k) * (kAttMaxWarps + 2) + kAttMaxWarps + (k == 0 ? 1 : 0)) * kPart;
+  }, count, threadIdx.x >> 5, kMergeWarps, nullptr, q0, nq, d.z, d.w);
 }
 
 size_t attention_workspace_bytes(int head_dim, int rows) {
   const int nt = rows > 8 ? 2 : 1;
-  return (size_t)kAttMaxCtas * ((kAttWarps + 2) * part_floats(head_dim, 8 * nt) * sizeof(float) + 2 * sizeof(int4));
+  return (size_t)kAttMaxCtas * ((kAttMaxWarps + 2) * part_floats(head_dim, 8 * nt) * sizeof(float) + 2 * sizeof(int4));
 }
 
-template <int D, int kFmt, int NT>
+template <int D, int kFmt, int NT, int kTerms>
 static cudaError_t att_launch(AttArgs& p, void* ws, cudaStream_t st) {
-  constexpr size_t smem = (size_t)kAttWarps * kAttStages * 2 * kAttStep * D;
-  static_assert(kAttStages * 2 * kAttStep * D >= part_floats(D, 8 * NT) * 4, "a warp's ring holds one partial result");
+  constexpr size_t smem = (size_t)att_warps(NT, kTerms) * att_stages(NT, kTerms) * 2 * kAttStep * D;
+  static_assert(att_stages(NT, kTerms) * 2 * kAttStep * D >= part_floats(D, 8 * NT) * 4, "a warp's ring holds one partial result");
+  static_assert(att_warps(NT, kTerms) <= kAttMaxWarps, "workspace slots");
   p.ws = static_cast<float*>(ws);
-  p.desc = reinterpret_cast<int4*>(p.ws + (size_t)kAttMaxCtas * (kAttWarps + 2) * part_floats(D, 8 * NT));
-  auto fn = k_attend<D, kFmt, NT>;
+  p.desc = reinterpret_cast<int4*>(p.ws + (size_t)kAttMaxCtas * (kAttMaxWarps + 2) * part_floats(D, 8 * NT));
+  auto fn = k_attend<D, kFmt, NT, kTerms>;
   if (cudaError_t e = ensure_dynamic_smem((const void*)fn, smem); e != cudaSuccess) return e;
-  fn<<<p.ctas, kAttWarps * 32, smem, st>>>(p);
+  fn<<<p.ctas, att_warps(NT, kTerms) * 32, smem, st>>>(p);
   if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   cfg.gridDim = dim3(p.ctas);
-  cfg.blockDim = dim3(kAttWarps * 32);
+  cfg.blockDim = dim3(kMergeWarps * 32);
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -705,7 +782,8 @@ static cudaError_t att_launch(AttArgs& p, void* ws, cudaStream_t st) {
 
 template <int D, int kFmt>
 static cudaError_t att_pick(AttArgs& p, int rows, void* ws, cudaStream_t st) {
-  return rows > 8 ? att_launch<D, kFmt, 2>(p, ws, st) : att_launch<D, kFmt, 1>(p, ws, st);
+  if (p.a.dtype == CKV_BF16) return rows > 8 ? att_launch<D, kFmt, 2, 1>(p, ws, st) : att_launch<D, kFmt, 1, 1>(p, ws, st);
+  return rows > 8 ? att_launch<D, kFmt, 2, 2>(p, ws, st) : att_launch<D, kFmt, 1, 2>(p, ws, st);
 }
 
 cudaError_t launch_cache_attention(const ckv_cache& c, const ckv_attention_args& a, void* ws, cudaStream_t st) {

@@ -7,7 +7,10 @@ after the 64-bit reduction, cosine and sine to 2 ulp, two products and a sum: 8 
 norm.  Attention: operands in two fp16 terms (2^-22 relative), the tensor core's truncated sums over
 D / 16 + 1 steps and an approximate exp2 (2^-22) put a logit off by at most
     delta = 2^-20 * scale * sum_i |q_i k_i| + 2^-20,
-which moves the log-sum-exp by delta and the output by 2 delta max |v|.
+which moves the log-sum-exp by delta and the output by 2 delta max |v|.  For bf16 queries the weights
+are one fp16 term instead: each p_j is off by at most 2^-11 p_j (11 significant bits, to nearest;
+they stand at 2^9 or more for the largest, so what is subnormal, below 2^-14, is off by 2^-25, that is
+2^-34 of the largest), which moves the output by at most sum_j 2^-11 p_j |v_j| + n 2^-34 max |v|.
 """
 
 import math
@@ -429,7 +432,10 @@ def _attention_check(out, lse, q, k, v, lens, queries, scale, causal):
             mass = torch.einsum("mhd,nhd->mhn", qq.abs(), kk.abs().repeat_interleave(H // Hk, 1)).amax(-1)
             delta = 2.0 ** -20 * abs(scale) * mass + 2.0 ** -20
             top = vv.abs().amax((0, 2)).repeat_interleave(H // Hk)
-            tol = u * want.abs() + (2 * delta * top)[..., None]
+            tol = (2 * delta * top)[..., None]
+            if q.dtype == torch.bfloat16:
+                tol = tol + 2.0 ** -11 * ref.attention(qq, kk, vv.abs(), scale, causal)[0] + n * 2.0 ** -34 * top[:, None]
+            tol = u * want.abs() + tol * (1 + u)
         else:
             delta, tol = torch.zeros_like(wl), torch.zeros_like(want)
         got, gl = out[a:a + m].double(), lse[a:a + m].double()
