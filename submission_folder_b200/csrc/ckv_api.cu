@@ -967,6 +967,10 @@ int ckv_cache_attention(const ckv_cache* cache, const ckv_attention_args* a, voi
   rc = ckv_cache_attention_workspace(cache->head_dim, a->max_q, a->q_heads, cache->num_kv_heads, &need);
   if (rc) return rc;
   if ((int64_t)a->max_q * a->q_heads > 1 << 20) return fail(CKV_ERR_UNSUPPORTED, "too many query rows per sequence");
+  // the steps of the largest batch that the tables can hold are counted in 32 bits
+  const double most = (double)a->requests * (((double)a->table_width * cache->block_size) / 32 + 1) * cache->num_kv_heads *
+                      ((double)a->max_q * (a->q_heads / cache->num_kv_heads) / 8 + 1);
+  if (most > 4.0e9) return fail(CKV_ERR_UNSUPPORTED, "requests * table_width * block_size * heads too large");
   if (!workspace || (uintptr_t)workspace % 256 != 0) return fail(CKV_ERR_WORKSPACE, "workspace must be 256-byte aligned and non-null");
   if (workspace_bytes < need) return fail(CKV_ERR_WORKSPACE, "workspace too small (see ckv_cache_attention_workspace)");
   if (a->requests == 0 || a->tokens == 0) return CKV_OK;

@@ -52,8 +52,9 @@ struct AttArgs {
   ckv_cache c;
   ckv_attention_args a;
   float* ws;                     // [ctas][kAttMaxWarps + 2] partial results
-  int4* desc;                    // [ctas][2]: what k_attend_merge has to merge from this CTA on
+  int4* desc;                    // [ctas]: what k_attend_merge has to merge from this CTA on
   int block_log2, group, ctas;
+  float inv_group;
 };
 
 // A partial result: 8 * NT rows of (m, m', l, -) then of D sums.
@@ -131,13 +132,6 @@ CKV_DEV void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   lo = half2_bits(x - f.x, y - f.y);
 }
 
-// A position in the line of units.
-struct Place {
-  int r, n, nq, q0;        // sequence, its length, its query tokens and the first one's row
-  int unit, units, steps;  // (head, row tile) within the sequence, their count, steps of each
-  int step;
-};
-
 CKV_DEV int seq_len(const AttArgs& p, int r) {
   const long long cap = (long long)p.a.table_width << p.block_log2;
   return (int)min(min((long long)max(__ldg(p.a.lens + r), 0), cap), (long long)INT32_MAX - 2 * kAttStep);
@@ -151,14 +145,31 @@ CKV_DEV void seq_queries(const AttArgs& p, int r, int& q0, int& nq) {
     nq = 1;
   }
 }
-template <int NT> CKV_DEV int seq_units(const AttArgs& p, int nq) {
-  return p.c.num_kv_heads * ((nq * p.group + 8 * NT - 1) / (8 * NT));
+CKV_DEV uint32_t steps_of(int n) { return (uint32_t)(n + kAttStep - 1) / kAttStep; }
+template <int NT> CKV_DEV uint32_t seq_units(const AttArgs& p, int nq) {
+  return p.c.num_kv_heads * (uint32_t)((nq * p.group + 8 * NT - 1) / (8 * NT));
 }
-template <int NT> CKV_DEV long long seq_work(const AttArgs& p, int r) {
+template <int NT> CKV_DEV uint32_t seq_work(const AttArgs& p, int r) {
   int q0, nq;
   seq_queries(p, r, q0, nq);
-  return (long long)seq_units<NT>(p, nq) * ((seq_len(p, r) + kAttStep - 1) / kAttStep);
+  return seq_units<NT>(p, nq) * steps_of(seq_len(p, r));
 }
+// Query token and head within the group of row rho (rho < 2^20: the product cannot reach the
+// next whole number).
+CKV_DEV void row_split(const AttArgs& p, int rho, int& token, int& member) {
+  token = (int)((rho + 0.5f) * p.inv_group);
+  member = rho - token * p.group;
+}
+
+// The line of units cut in `parts`: the first `rem` parts have one step more.
+struct Cut {
+  uint32_t each, rem;
+  CKV_DEV uint32_t at(uint32_t part) const { return part * each + min(part, rem); }
+  CKV_DEV uint32_t of(uint32_t x) const {   // the part that holds step x
+    const uint32_t big = rem * (each + 1);
+    return x < big ? x / (each + 1) : rem + (x - big) / each;
+  }
+};
 
 // One query row of four floats at p + i in the query's type.
 CKV_DEV float4 load_q4(const void* p, int dtype, int64_t i) {
@@ -190,73 +201,60 @@ CKV_DEV void store_out4(void* p, int dtype, int64_t i, float4 v) {
 
 // Where row `rho` of a unit's sequence and head goes.
 CKV_DEV void row_home(const AttArgs& p, int q0, int head, int rho, int64_t& out, int64_t& lse) {
-  const int i = rho / p.group, hq = head * p.group + rho % p.group;
+  int i, member;
+  row_split(p, rho, i, member);
+  const int hq = head * p.group + member;
   out = (q0 + i) * p.a.out_tok_stride + hq * p.a.out_head_stride;
   lse = (int64_t)(q0 + i) * (p.c.num_kv_heads * p.group) + hq;
 }
-// The factor on a row's sums and its log-sum-exp, from its maxima (base 2) and its sum.
+// The factor on a row's sums and its log-sum-exp, from its references (base 2) and its sum.
 CKV_DEV float row_factor(float m, float mw, float l) { return l > 0.f || isnan(l) ? exp2f(mw - m - kTop) / l : 0.f; }
 CKV_DEV float row_lse(float m, float l) { return l > 0.f || isnan(l) ? (m + log2f(l)) * kLn2 : -INFINITY; }
 
-// Merge of `count` partial results of one unit, part(i) their places, by the warps of a CTA
-// [w0, w0 + nw): to the output (ctas_left == 0) or to `dst`.
+// Merge of `count` partial results of one unit, part(i) their places: to the output, or to `dst`.
+// A thread has four dimensions of a row.  kL2: other CTAs' results, read from L2.
 template <int D, int NT, bool kL2, typename F>
-CKV_DEV void merge_parts(const AttArgs& p, F part, int count, int w0, int nw, float* dst, int q0, int nq, int head, int tile) {
-  constexpr int PER = D / 32;
-  auto get = [](const float* x) { return kL2 ? __ldcg(x) : *x; };   // other CTAs' results come from L2
-  const int lane = threadIdx.x & 31;
-  for (int row = w0; row < 8 * NT; row += nw) {
+CKV_DEV void merge_parts(const AttArgs& p, F part, int count, int tid, int threads, float* dst, int q0, int rows, int head,
+                         int tile) {
+  auto get4 = [](const float* x) {
+    return kL2 ? __ldcg(reinterpret_cast<const float4*>(x)) : *reinterpret_cast<const float4*>(x);
+  };
+  for (int i = tid; i < 8 * NT * (D / 4); i += threads) {
+    const int row = i / (D / 4), d = i % (D / 4) * 4;
     const int rho = tile * 8 * NT + row;
-    if (!dst && rho >= nq * p.group) break;
+    if (rho >= rows) break;
     float m = kNone, mw = kNone;
-    for (int i = lane; i < count; i += 32) {
-      const float* s = part(i) + row * 4;
-      m = fmaxf(m, get(s));
-      mw = fmaxf(mw, get(s + 1));
-    }
-    m = warp_max(m);
-    mw = warp_max(mw);
-    float l = 0.f, o[PER] = {};
-    for (int i0 = 0; i0 < count; i0 += 32) {   // lane i weighs part i0 + i, then all lanes add up the parts
-      float f = 0.f;
-      if (i0 + lane < count) {
-        const float* s = part(i0 + lane) + row * 4;
-        l += get(s + 2) * exp2f(get(s) - m);
-        f = exp2f(get(s + 1) - mw);
-      }
-      const int nn = min(32, count - i0);
 #pragma unroll 4
-      for (int i = 0; i < nn; ++i) {
-        const float fi = __shfl_sync(0xffffffffu, f, i);
-        const float* x = part(i0 + i) + 8 * NT * 4 + row * D + lane * PER;
-#pragma unroll
-        for (int e = 0; e < PER; ++e) o[e] += get(x + e) * fi;
-      }
+    for (int k = 0; k < count; ++k) {
+      const float4 s = get4(part(k) + row * 4);
+      m = fmaxf(m, s.x);
+      mw = fmaxf(mw, s.y);
     }
-    l = warp_sum(l);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < count; ++k) {
+      const float4 s = get4(part(k) + row * 4), x = get4(part(k) + 8 * NT * 4 + row * D + d);
+      l += s.z * ex2(s.x - m);
+      const float f = ex2(s.y - mw);
+      o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
+    }
     if (dst) {
-      if (lane == 0) { dst[row * 4] = m; dst[row * 4 + 1] = mw; dst[row * 4 + 2] = l; }
-#pragma unroll
-      for (int e = 0; e < PER; ++e) dst[8 * NT * 4 + row * D + lane * PER + e] = o[e];
+      if (d == 0) *reinterpret_cast<float4*>(dst + row * 4) = make_float4(m, mw, l, 0.f);
+      *reinterpret_cast<float4*>(dst + 8 * NT * 4 + row * D + d) = o;
     } else {
       int64_t at, lat;
       row_home(p, q0, head, rho, at, lat);
       const float f = row_factor(m, mw, l);
-      if constexpr (PER == 4) {
-        store_out4(p.a.out, p.a.dtype, at + lane * 4, make_float4(o[0] * f, o[1] * f, o[2] * f, o[3] * f));
-      } else {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __shfl_sync(0xffffffffu, o[e & 1] * f, (2 * lane + (e >> 1)) & 31);
-        if (lane < 16) store_out4(p.a.out, p.a.dtype, at + lane * 4, make_float4(v[0], v[1], v[2], v[3]));
-      }
-      if (p.a.lse && lane == 0) p.a.lse[lat] = row_lse(m, l);
+      store_out4(p.a.out, p.a.dtype, at + d, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+      if (p.a.lse && d == 0) p.a.lse[lat] = row_lse(m, l);
     }
   }
 }
 
 struct Entry {     // a piece of a unit that ended in this CTA without being the whole unit
-  int used, r, unit, begins, ends;   // begins: the unit's first step is in this piece; ends: its last
+  int used, q0, rows, head, tile;
+  uint32_t begin, end;     // the unit in the line
   const float* part;
 };
 
@@ -268,84 +266,64 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
   constexpr int kTiles = D / 16;                 // m16 tiles of the output
   constexpr int kStageBytes = 2 * kAttStep * D;  // K then V
   constexpr int kRing = kStages * kStageBytes;
-  constexpr int kAhead = 2;                      // steps in flight: the ring's third stage is refilled before a step's
-                                                 // products, the second of two after them
-  static_assert(kStages == 2 || kStages == 3, "ring");
+  constexpr int kAhead = kStages - 1;            // steps in flight during a step's products
   constexpr int kPart = part_floats(D, 8 * NT);
   extern __shared__ __align__(128) char att_smem[];
   __shared__ float s_scale[kWarps][kStages][4];  // K, V of the step's first and second 16 tokens
   __shared__ Entry s_entry[2 * kWarps];
-  __shared__ Place s_place[kWarps];
-  __shared__ long long s_tot[kWarps];
+  __shared__ int s_order[2 * kWarps];            // its used ones
+  static_assert(2 * kWarps <= 32, "one ballot");
+  __shared__ uint2 s_place[kWarps];              // sequence of the warp's first step, and where it begins in the line
+  __shared__ uint32_t s_tot[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x, R = p.a.requests;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid < 2 * kWarps) s_entry[tid].used = 0;
-  if (tid < 2) p.desc[cta * 2 + tid] = make_int4(0, 0, 0, 0);
 
   // ---- the line of units: its length, and where this CTA's warps stand in it
-  const long long first = tid < R ? seq_work<NT>(p, tid) : 0;
-  long long total = first;
+  const uint32_t first = tid < R ? seq_work<NT>(p, tid) : 0;
+  uint32_t total = first;
   for (int r = tid + kWarps * 32; r < R; r += kWarps * 32) total += seq_work<NT>(p, r);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  total = __reduce_add_sync(0xffffffffu, total);
   if (lane == 0) s_tot[wid] = total;
   __syncthreads();
   total = 0;
+#pragma unroll
   for (int w = 0; w < kWarps; ++w) total += s_tot[w];
-  const int nctas = (int)min((long long)p.ctas, (total + kWarps - 1) / kWarps);
-  const long long c0 = cta < nctas ? total * cta / nctas : total, c1 = cta < nctas ? total * (cta + 1) / nctas : total;
-  auto warp_at = [&](int w) { return c0 + (c1 - c0) * w / kWarps; };
-  long long before = 0;   // work of the sequences before this chunk of threads
+  const uint32_t nctas = min((uint32_t)p.ctas, (total + kWarps - 1) / kWarps);
+  const Cut cut = {nctas ? total / nctas : 0u, nctas ? total % nctas : 0u};
+  const uint32_t c0 = cta < nctas ? cut.at(cta) : total, c1 = cta < nctas ? cut.at(cta + 1) : total;
+  const Cut warps = {(c1 - c0) / kWarps, (c1 - c0) % kWarps};
+  uint32_t before = 0;   // work of the sequences before this chunk of threads
   for (int base = 0; base < R && before < c1; base += kWarps * 32) {
     const int r = base + tid;
-    const long long mine = base == 0 ? first : r < R ? seq_work<NT>(p, r) : 0;
-    long long x = mine;
+    const uint32_t mine = base == 0 ? first : r < R ? seq_work<NT>(p, r) : 0;
+    uint32_t x = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
     __syncthreads();
     if (lane == 31) s_tot[wid] = x;
     __syncthreads();
-    long long at = before;
-    for (int w = 0; w < wid; ++w) at += s_tot[w];
-    for (int w = 0; w < kWarps; ++w) before += s_tot[w];
-    at += x - mine;
-    if (mine > 0 && at < c1 && at + mine > c0) {
-      Place pl;
-      pl.r = r;
-      pl.n = seq_len(p, r);
-      seq_queries(p, r, pl.q0, pl.nq);
-      pl.units = seq_units<NT>(p, pl.nq);
-      pl.steps = (pl.n + kAttStep - 1) / kAttStep;
-      for (int w = 0; w < kWarps; ++w) {
-        const long long a = warp_at(w);
-        if (a >= at && a < at + mine && a < c1) {
-          pl.unit = (int)((a - at) / pl.steps);
-          pl.step = (int)((a - at) % pl.steps);
-          s_place[w] = pl;
-        }
-      }
+    uint32_t at = before + x - mine;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < wid) at += s_tot[w];
+      before += s_tot[w];
     }
+    if (mine > 0 && at < c1 && at + mine > c0)
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const uint32_t a = c0 + warps.at(w);
+        if (a >= at && a < at + mine) s_place[w] = make_uint2(r, at);
+      }
   }
   __syncthreads();
-  // sequences with nothing to see: zeros
-  for (int r = cta; r < R; r += gridDim.x)
-    if (seq_len(p, r) == 0) {
-      int q0, nq;
-      seq_queries(p, r, q0, nq);
-      const int hq = p.c.num_kv_heads * p.group;
-      for (int i = tid; i < nq * hq * (D / 4); i += kWarps * 32) {
-        const int row = i / (D / 4), d = i % (D / 4) * 4, tok = q0 + row / hq, h = row % hq;
-        store_out4(p.a.out, p.a.dtype, tok * p.a.out_tok_stride + h * p.a.out_head_stride + d, make_float4(0.f, 0.f, 0.f, 0.f));
-        if (p.a.lse && d == 0) p.a.lse[(int64_t)tok * hq + h] = -INFINITY;
-      }
-    }
 
   // ---- this warp's piece
-  long long left = warp_at(wid + 1) - warp_at(wid);
+  uint32_t here = c0 + warps.at(wid), left = warps.at(wid + 1) - warps.at(wid);
   char* ring = att_smem + wid * kRing;
   const uint32_t ring_a = smem_u32(ring), scale_a = smem_u32(&s_scale[wid][0][0]);
   // 16-byte chunk of a row, so that neither reads by rows nor reads by columns meet in a bank
@@ -355,16 +333,21 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
   constexpr int kChunks = D / 16, kRows = 32 / kChunks;   // of one copy instruction
   const int crow = lane / kChunks, cchunk = lane % kChunks;
   if (left > 0) {
-    Place pl = s_place[wid];
+    uint32_t seq_at = s_place[wid].y;
+    int r = (int)s_place[wid].x;
+    int n = seq_len(p, r), q0, nq;
+    seq_queries(p, r, q0, nq);
+    uint32_t steps = steps_of(n);
+    uint32_t unit = (here - seq_at) / steps;
+    int step = (int)(here - seq_at - unit * steps);
     bool first_piece = true;
     while (left > 0) {
-      const int todo = (int)min(left, (long long)(pl.steps - pl.step));
-      const int s_begin = pl.step, s_end = pl.step + todo;
-      const int tiles = pl.units / p.c.num_kv_heads;
-      const int head = pl.unit / tiles, tile = pl.unit - head * tiles;
-      const int rows = pl.nq * p.group;
-      const int n = pl.n;
-      const int32_t* table = p.a.tables + pl.r * p.a.table_stride;
+      const int todo = (int)min(left, steps - step);
+      const int s_begin = step, s_end = step + todo;
+      const uint32_t tiles = (uint32_t)(nq * p.group + 8 * NT - 1) / (8 * NT);
+      const int head = unit / tiles, tile = unit - head * tiles;
+      const int rows = nq * p.group;
+      const int32_t* table = p.a.tables + r * p.a.table_stride;
       const int pages = (n + (1 << p.block_log2) - 1) >> p.block_log2;
       const char* kh = static_cast<const char*>(p.c.k) + head * p.c.k_head_stride + crow * p.c.k_tok_stride + cchunk * 16;
       const char* vh = static_cast<const char*>(p.c.v) + head * p.c.v_head_stride + crow * p.c.v_tok_stride + cchunk * 16;
@@ -374,7 +357,7 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
       auto page = [&](int i) { return i < pages ? __ldg(table + i) : 0; };
       int pcur = page(pbase + lane), pnext = page(pbase + 32 + lane);
       auto issue = [&](int s, int stage) {
-        if (s < s_end) {
+        {
           const uint32_t st = ring_a + stage * kStageBytes;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
@@ -413,61 +396,63 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
             }
           }
         }
-        cp_commit();
       };
 
-      // query rows: lane (g, t) loads row g's dimensions of its chunks
       uint32_t qf[NT][kTerms][kSteps16][2];
       float qs[NT][2];        // rows 2t, 2t + 1: scale * log2 e * the row's power of two
       int see[NT][2];         // tokens that they see
       int see_min = n;
-      float4 x[NT][kSteps16];
+      // query rows: lane (g, t) loads row g's dimensions of its chunks
+      auto load_queries = [&]() {
+        float4 x[NT][kSteps16];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int rho = (tile * NT + nt) * 8 + g;
-        const int i = rho / p.group, hq = head * p.group + rho % p.group;
+        for (int nt = 0; nt < NT; ++nt) {
+          const int rho = (tile * NT + nt) * 8 + g;
+          int i, member;
+          row_split(p, rho, i, member);
+          const int64_t at = (q0 + i) * p.a.q_tok_stride + (head * p.group + member) * p.a.q_head_stride;
 #pragma unroll
-        for (int k = 0; k < kSteps16; ++k) {
-          const int dim = D == 128 ? (2 * t + k / 4) * 16 + (k & 3) * 4 : t * 16 + k * 4;
-          x[nt][k] = rho < rows ? load_q4(p.a.q, p.a.dtype, (pl.q0 + i) * p.a.q_tok_stride + hq * p.a.q_head_stride + dim)
-                                : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) issue(s_begin + i, i);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int rho = (tile * NT + nt) * 8 + g;
-        float top = 0.f;
-#pragma unroll
-        for (int k = 0; k < kSteps16; ++k)
-          top = fmaxf(fmaxf(fmaxf(top, fabsf(x[nt][k].x)), fmaxf(fabsf(x[nt][k].y), fabsf(x[nt][k].z))), fabsf(x[nt][k].w));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the row times 2^(14 - exponent); exponents at the ends of the range are clamped
-        const int e = min(max((int)(__float_as_uint(top) >> 23), 16), 254);   // biased
-        const float up = __uint_as_float((uint32_t)(268 - e) << 23);
-        const float mine = p.a.scale * kLog2e / up;
-        const int sees = rho < rows && p.a.causal ? n - pl.nq + rho / p.group + 1 : n;
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          qs[nt][r] = __shfl_sync(0xffffffffu, mine, (2 * t + r) * 4);
-          see[nt][r] = __shfl_sync(0xffffffffu, sees, (2 * t + r) * 4);
-          see_min = min(see_min, see[nt][r]);
-        }
-#pragma unroll
-        for (int k = 0; k < kSteps16; ++k) {
-          const float4 v = x[nt][k];
-          if constexpr (kTerms == 1) {
-            qf[nt][0][k][0] = half2_bits(v.x * up, v.y * up);
-            qf[nt][0][k][1] = half2_bits(v.z * up, v.w * up);
-          } else {
-            split2(v.x * up, v.y * up, qf[nt][0][k][0], qf[nt][1][k][0]);
-            split2(v.z * up, v.w * up, qf[nt][0][k][1], qf[nt][1][k][1]);
+          for (int k = 0; k < kSteps16; ++k) {
+            const int dim = D == 128 ? (2 * t + k / 4) * 16 + (k & 3) * 4 : t * 16 + k * 4;
+            x[nt][k] = rho < rows ? load_q4(p.a.q, p.a.dtype, at + dim) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
         }
-      }
-      see_min = __reduce_min_sync(0xffffffffu, see_min);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int rho = (tile * NT + nt) * 8 + g;
+          float top = 0.f;
+#pragma unroll
+          for (int k = 0; k < kSteps16; ++k)
+            top = fmaxf(fmaxf(fmaxf(top, fabsf(x[nt][k].x)), fmaxf(fabsf(x[nt][k].y), fabsf(x[nt][k].z))), fabsf(x[nt][k].w));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          // the row times 2^(14 - exponent); exponents at the ends of the range are clamped
+          const int e = min(max((int)(__float_as_uint(top) >> 23), 16), 254);   // biased
+          const float up = __uint_as_float((uint32_t)(268 - e) << 23);
+          const float mine = p.a.scale * kLog2e / up;
+          int i, member;
+          row_split(p, rho, i, member);
+          const int sees = rho < rows && p.a.causal ? n - nq + i + 1 : n;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            qs[nt][r] = __shfl_sync(0xffffffffu, mine, (2 * t + r) * 4);
+            see[nt][r] = __shfl_sync(0xffffffffu, sees, (2 * t + r) * 4);
+            see_min = min(see_min, see[nt][r]);
+          }
+#pragma unroll
+          for (int k = 0; k < kSteps16; ++k) {
+            const float4 v = x[nt][k];
+            if constexpr (kTerms == 1) {
+              qf[nt][0][k][0] = half2_bits(v.x * up, v.y * up);
+              qf[nt][0][k][1] = half2_bits(v.z * up, v.w * up);
+            } else {
+              split2(v.x * up, v.y * up, qf[nt][0][k][0], qf[nt][1][k][0]);
+              split2(v.z * up, v.w * up, qf[nt][0][k][1], qf[nt][1][k][1]);
+            }
+          }
+        }
+        see_min = __reduce_min_sync(0xffffffffu, see_min);
+      };
 
       // out^T: tile i has dims (g * kTiles * 2 + 2 i, + 1) x rows (2t, 2t + 1)
       float o[NT][kTiles][4];
@@ -480,11 +465,16 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
         for (int j = 0; j < kTiles; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
       }
 
-      int stage = 0;
-      for (int s = s_begin; s < s_end; ++s) {
-        cp_wait<kAhead - 1>();
+      int fill = 0, stage = 0;   // ring stages to fill and to use next
+#pragma unroll 1
+      for (int s = s_begin - kAhead; s < s_end; ++s) {   // one copy of the code for the ring's filling and its use
+        if (s + kAhead < s_end) issue(s + kAhead, fill);
+        cp_commit();
+        fill = fill == kStages - 1 ? 0 : fill + 1;
+        if (s + kAhead == s_begin) load_queries();
+        if (s < s_begin) continue;
+        cp_wait<kAhead>();
         __syncwarp();
-        if constexpr (kStages > 2) issue(s + kStages - 1, stage == 0 ? kStages - 1 : stage - 1);
         const uint32_t kst = ring_a + stage * kStageBytes, vst = kst + kAttStep * D;
         // logits^T: lane holds tokens g, g + 8 of each 16 x rows 2t, 2t + 1
         float sc[NT][2][4];
@@ -635,7 +625,6 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
             }
         }
         __syncwarp();   // the stage may be filled again
-        if constexpr (kStages == 2) issue(s + 2, stage);
         stage = stage == kStages - 1 ? 0 : stage + 1;
       }
       cp_wait<0>();
@@ -643,14 +632,15 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
 
       // ---- the piece's end: the whole unit goes out, a part of one is kept for merging
       left -= todo;
-      const bool begins = s_begin == 0, ends = s_end == pl.steps;
       float* part = nullptr;
-      if (!(begins && ends)) {
+      if (todo != (int)steps) {
         // the ring is free once the warp has no further piece
         part = left > 0 ? p.ws + ((size_t)cta * (kAttMaxWarps + 2) + wid) * kPart : reinterpret_cast<float*>(ring);
         if (lane == 0) {
           Entry& en = s_entry[2 * wid + (first_piece ? 0 : 1)];
-          en.used = 1; en.r = pl.r; en.unit = pl.unit; en.begins = begins; en.ends = ends; en.part = part;
+          en.used = 1; en.q0 = q0; en.rows = rows; en.head = head; en.tile = tile; en.part = part;
+          en.begin = seq_at + unit * steps;
+          en.end = en.begin + steps;
         }
       }
 #pragma unroll
@@ -662,7 +652,7 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
           for (int d = 4; d < 32; d <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, d);
           const int row = nt * 8 + 2 * t + r;
           if (part) {
-            if (g == 0) { part[row * 4] = m[nt][r]; part[row * 4 + 1] = mw[nt][r]; part[row * 4 + 2] = lt; }
+            if (g == 0) *reinterpret_cast<float4*>(part + row * 4) = make_float4(m[nt][r], mw[nt][r], lt, 0.f);
             float4* d = reinterpret_cast<float4*>(part + 8 * NT * 4 + row * D + g * 2 * kTiles);
 #pragma unroll
             for (int j = 0; j < kTiles; j += 2)
@@ -671,7 +661,7 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
             const int rho = tile * NT * 8 + row;
             if (rho < rows) {
               int64_t at, lat;
-              row_home(p, pl.q0, head, rho, at, lat);
+              row_home(p, q0, head, rho, at, lat);
               const float f = row_factor(m[nt][r], mw[nt][r], lt);
 #pragma unroll
               for (int j = 0; j < kTiles; j += 2)
@@ -683,78 +673,79 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
         }
       first_piece = false;
       if (left > 0) {   // on to the next unit
-        pl.step = 0;
-        if (++pl.unit == pl.units) {
-          pl.unit = 0;
+        step = 0;
+        if (++unit == p.c.num_kv_heads * tiles) {
+          seq_at += unit * steps;
+          unit = 0;
           do {
-            if (++pl.r >= R) { left = 0; break; }   // never expected: keeps the reads in bounds
-            pl.n = seq_len(p, pl.r);
-            seq_queries(p, pl.r, pl.q0, pl.nq);
-            pl.units = seq_units<NT>(p, pl.nq);
-            pl.steps = (pl.n + kAttStep - 1) / kAttStep;
-          } while (pl.units * pl.steps == 0);
+            if (++r >= R) { left = 0; break; }   // never expected: keeps the reads in bounds
+            n = seq_len(p, r);
+            seq_queries(p, r, q0, nq);
+            steps = steps_of(n);
+          } while (nq * steps == 0);
         }
       }
     }
   }
   __syncthreads();
 
-  // ---- merge the pieces of each unit within the CTA
-  const float* list[kWarps + 1];
-  for (int i = 0; i < 2 * kWarps;) {
-    if (!s_entry[i].used) { ++i; continue; }
-    const int r = s_entry[i].r, unit = s_entry[i].unit;
-    const bool begins = s_entry[i].begins;
-    bool ends = false;
-    int count = 0;
-    for (; i < 2 * kWarps; ++i) {
-      if (!s_entry[i].used) continue;
-      if (s_entry[i].r != r || s_entry[i].unit != unit) break;
-      list[count++] = s_entry[i].part;
-      ends = s_entry[i].ends;
+  // ---- merge the pieces of each unit within the CTA; a unit that reaches past the CTA leaves its
+  // part in slot 0 (begun in a CTA before) or 1 (begun here)
+  if (c1 > c0) {
+    int4 todo = make_int4(0, 0, 0, 0);
+    const bool used = lane < 2 * kWarps && s_entry[lane].used;   // each warp for itself
+    const uint32_t mask = __ballot_sync(0xffffffffu, used);
+    if (wid == 0 && used) s_order[__popc(mask & ((1u << lane) - 1))] = lane;
+    __syncthreads();
+    const int entries = __popc(mask);
+    for (int i = 0; i < entries;) {
+      const Entry e = s_entry[s_order[i]];
+      const int from = i;
+      while (i < entries && s_entry[s_order[i]].begin == e.begin) ++i;
+      const bool begins = e.begin >= c0, ends = e.end <= c1;
+      float* dst = begins && ends ? nullptr : p.ws + ((size_t)cta * (kAttMaxWarps + 2) + kAttMaxWarps + (begins ? 1 : 0)) * kPart;
+      merge_parts<D, NT, false>(p, [&](int j) { return s_entry[s_order[from + j]].part; }, i - from, tid, kWarps * 32, dst, e.q0,
+                                e.rows, e.head, e.tile);
+      if (begins && !ends) todo = make_int4((int)(cut.of(e.end - 1) - cta + 1) | e.head << 8, e.q0, e.rows, e.tile);
     }
-    int q0, nq;
-    seq_queries(p, r, q0, nq);
-    const int tiles = seq_units<NT>(p, nq) / p.c.num_kv_heads;
-    const int head = unit / tiles, tile = unit - head * tiles;
-    // a unit that reaches past this CTA leaves its part in slot 0 (begun before) or 1
-    float* dst = begins && ends ? nullptr : p.ws + ((size_t)cta * (kAttMaxWarps + 2) + kAttMaxWarps + (begins ? 1 : 0)) * kPart;
-    merge_parts<D, NT, false>(p, [&](int k) { return list[k]; }, count, wid, kWarps, dst, q0, nq, head, tile);
-    if (begins && !ends && tid == 0) {
-      p.desc[cta * 2] = make_int4(1, r, head, tile);
-    }
-    if (!begins && tid == 0) p.desc[cta * 2 + 1] = make_int4(1, ends ? 1 : 0, 0, 0);
+    if (tid == 0) p.desc[cta] = todo;
+  } else if (tid == 0) {
+    p.desc[cta] = make_int4(0, 0, 0, 0);
   }
+
+  // sequences with nothing to see: zeros
+  for (int r = cta; r < R; r += gridDim.x)
+    if (seq_len(p, r) == 0) {
+      int q0, nq;
+      seq_queries(p, r, q0, nq);
+      const int hq = p.c.num_kv_heads * p.group;
+      for (int i = tid; i < nq * hq * (D / 4); i += kWarps * 32) {
+        const int row = i / (D / 4), d = i % (D / 4) * 4, tok = q0 + row / hq, h = row % hq;
+        store_out4(p.a.out, p.a.dtype, tok * p.a.out_tok_stride + h * p.a.out_head_stride + d, make_float4(0.f, 0.f, 0.f, 0.f));
+        if (p.a.lse && d == 0) p.a.lse[(int64_t)tok * hq + h] = -INFINITY;
+      }
+    }
 }
 
 // CTA c merges the unit that begins in CTA c of k_attend and reaches past it: its slot 1 and
 // slot 0 of the CTAs that follow, up to the one where it ends.
-constexpr int kMergeWarps = 8;
+constexpr int kMergeThreads = 256;
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kMergeWarps * 32) k_attend_merge(const AttArgs p) {
+__global__ void __launch_bounds__(kMergeThreads) k_attend_merge(const AttArgs p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int kPart = part_floats(D, 8 * NT);
   const int cta = blockIdx.x;
-  const int4 d = __ldcg(p.desc + cta * 2);
+  const int4 d = __ldcg(p.desc + cta);
   if (!d.x) return;
-  int count = 1;
-  for (int c = cta + 1; c < p.ctas; ++c) {
-    const int4 f = __ldcg(p.desc + c * 2 + 1);
-    if (!f.x) break;
-    ++count;
-    if (f.y) break;
-  }
-  int q0, nq;
-  seq_queries(p, d.y, q0, nq);
-  merge_parts<D, NT, true>(p, [&](int k) {
-    return p.ws + ((size_t)(cta + k) * (kAttMaxWarps + 2) + kAttMaxWarps + (k == 0 ? 1 : 0)) * kPart;
-  }, count, threadIdx.x >> 5, kMergeWarps, nullptr, q0, nq, d.z, d.w);
+  const float* base = p.ws + ((size_t)cta * (kAttMaxWarps + 2) + kAttMaxWarps) * kPart;
+  merge_parts<D, NT, true>(p, [&](int k) { return k ? base + (size_t)k * (kAttMaxWarps + 2) * kPart : base + kPart; }, d.x & 255,
+                           threadIdx.x, kMergeThreads, nullptr, d.y, d.z, d.x >> 8, d.w);
 }
 
 size_t attention_workspace_bytes(int head_dim, int rows) {
   const int nt = rows > 8 ? 2 : 1;
-  return (size_t)kAttMaxCtas * ((kAttMaxWarps + 2) * part_floats(head_dim, 8 * nt) * sizeof(float) + 2 * sizeof(int4));
+  return (size_t)kAttMaxCtas * ((kAttMaxWarps + 2) * part_floats(head_dim, 8 * nt) * sizeof(float) + sizeof(int4));
 }
 
 template <int D, int kFmt, int NT, int kTerms>
@@ -771,7 +762,7 @@ static cudaError_t att_launch(AttArgs& p, void* ws, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   cfg.gridDim = dim3(p.ctas);
-  cfg.blockDim = dim3(kMergeWarps * 32);
+  cfg.blockDim = dim3(kMergeThreads);
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -794,6 +785,7 @@ cudaError_t launch_cache_attention(const ckv_cache& c, const ckv_attention_args&
   while ((1 << p.block_log2) < c.block_size) ++p.block_log2;
   p.group = a.q_heads / c.num_kv_heads;
   p.ctas = kAttMaxCtas;
+  p.inv_group = 1.f / p.group;
   const int rows = a.max_q * p.group;
   const bool e4 = c.format == CKV_CACHE_E4M3;
   if (c.head_dim == 64)
