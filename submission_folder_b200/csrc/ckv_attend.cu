@@ -171,10 +171,14 @@ struct Cut {
   }
 };
 
-// One query row of four floats at p + i in the query's type.
-CKV_DEV float4 load_q4(const void* p, int dtype, int64_t i) {
-  if (dtype == CKV_FP32) return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
-  const uint2 v = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i));
+// Four elements, from `dim` on, of a query row in shared memory (chunks of 16 bytes, their
+// place turned by the row's low bits g).
+CKV_DEV float4 load_q4(uint32_t row, int g, int dtype, int dim) {
+  if (dtype == CKV_FP32) {
+    const uint4 v = lds4(row + (((dim >> 2) ^ g) << 4));
+    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+  }
+  const uint2 v = lds2(row + (((dim >> 3) ^ g) << 4) + (dim & 4) * 2);
   float2 x, y;
   if (dtype == CKV_BF16) {
     x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.x));
@@ -211,10 +215,11 @@ CKV_DEV void row_home(const AttArgs& p, int q0, int head, int rho, int64_t& out,
 CKV_DEV float row_factor(float m, float mw, float l) { return l > 0.f || isnan(l) ? exp2f(mw - m - kTop) / l : 0.f; }
 CKV_DEV float row_lse(float m, float l) { return l > 0.f || isnan(l) ? (m + log2f(l)) * kLn2 : -INFINITY; }
 
-// Merge of `count` partial results of one unit, part(i) their places: to the output, or to `dst`.
-// A thread has four dimensions of a row.  kL2: other CTAs' results, read from L2.
-template <int D, int NT, bool kL2, typename F>
-CKV_DEV void merge_parts(const AttArgs& p, F part, int count, int tid, int threads, float* dst, int q0, int rows, int head,
+// Merge of `count` partial results of one unit, next() their places in turn: to the output, or to
+// `dst`.  A thread has four dimensions of a row; kBatch parts are read at a time.  kL2: other
+// CTAs' results, read from L2.
+template <int D, int NT, bool kL2, int kBatch, typename F>
+CKV_DEV void merge_parts(const AttArgs& p, F parts, int count, int tid, int threads, float* dst, int q0, int rows, int head,
                          int tile) {
   auto get4 = [](const float* x) {
     return kL2 ? __ldcg(reinterpret_cast<const float4*>(x)) : *reinterpret_cast<const float4*>(x);
@@ -223,21 +228,35 @@ CKV_DEV void merge_parts(const AttArgs& p, F part, int count, int tid, int threa
     const int row = i / (D / 4), d = i % (D / 4) * 4;
     const int rho = tile * 8 * NT + row;
     if (rho >= rows) break;
-    float m = kNone, mw = kNone;
-#pragma unroll 4
-    for (int k = 0; k < count; ++k) {
-      const float4 s = get4(part(k) + row * 4);
-      m = fmaxf(m, s.x);
-      mw = fmaxf(mw, s.y);
-    }
-    float l = 0.f;
+    auto next = parts;
+    float m = kNone, mw = kNone, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int k = 0; k < count; ++k) {
-      const float4 s = get4(part(k) + row * 4), x = get4(part(k) + 8 * NT * 4 + row * D + d);
-      l += s.z * ex2(s.x - m);
-      const float f = ex2(s.y - mw);
-      o.x += x.x * f; o.y += x.y * f; o.z += x.z * f; o.w += x.w * f;
+    for (int k = 0; k < count; k += kBatch) {
+      float4 s[kBatch], x[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        s[j] = make_float4(kNone, kNone, 0.f, 0.f);
+        x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k + j < count) {
+          const float* q = next();
+          s[j] = get4(q + row * 4);
+          x[j] = get4(q + 8 * NT * 4 + row * D + d);
+        }
+      }
+      float nm = m, nw = mw;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) { nm = fmaxf(nm, s[j].x); nw = fmaxf(nw, s[j].y); }
+      l *= ex2(m - nm);
+      const float f0 = ex2(mw - nw);
+      o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        l += s[j].z * ex2(s[j].x - nm);
+        const float f = ex2(s[j].y - nw);
+        o.x += x[j].x * f; o.y += x[j].y * f; o.z += x[j].z * f; o.w += x[j].w * f;
+      }
+      m = nm;
+      mw = nw;
     }
     if (dst) {
       if (d == 0) *reinterpret_cast<float4*>(dst + row * 4) = make_float4(m, mw, l, 0.f);
@@ -271,59 +290,45 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
   extern __shared__ __align__(128) char att_smem[];
   __shared__ float s_scale[kWarps][kStages][4];  // K, V of the step's first and second 16 tokens
   __shared__ Entry s_entry[2 * kWarps];
-  __shared__ int s_order[2 * kWarps];            // its used ones
   static_assert(2 * kWarps <= 32, "one ballot");
-  __shared__ uint2 s_place[kWarps];              // sequence of the warp's first step, and where it begins in the line
-  __shared__ uint32_t s_tot[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x, R = p.a.requests;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid < 2 * kWarps) s_entry[tid].used = 0;
 
-  // ---- the line of units: its length, and where this CTA's warps stand in it
-  const uint32_t first = tid < R ? seq_work<NT>(p, tid) : 0;
+  // ---- the line of units: its length, and where this warp stands in it (each warp for itself)
+  const uint32_t first = lane < R ? seq_work<NT>(p, lane) : 0;
   uint32_t total = first;
-  for (int r = tid + kWarps * 32; r < R; r += kWarps * 32) total += seq_work<NT>(p, r);
+#pragma unroll 4
+  for (int r = lane + 32; r < R; r += 32) total += seq_work<NT>(p, r);
   total = __reduce_add_sync(0xffffffffu, total);
-  if (lane == 0) s_tot[wid] = total;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) total += s_tot[w];
   const uint32_t nctas = min((uint32_t)p.ctas, (total + kWarps - 1) / kWarps);
   const Cut cut = {nctas ? total / nctas : 0u, nctas ? total % nctas : 0u};
   const uint32_t c0 = cta < nctas ? cut.at(cta) : total, c1 = cta < nctas ? cut.at(cta + 1) : total;
   const Cut warps = {(c1 - c0) / kWarps, (c1 - c0) % kWarps};
-  uint32_t before = 0;   // work of the sequences before this chunk of threads
-  for (int base = 0; base < R && before < c1; base += kWarps * 32) {
-    const int r = base + tid;
-    const uint32_t mine = base == 0 ? first : r < R ? seq_work<NT>(p, r) : 0;
-    uint32_t x = mine;
+  const uint32_t here = c0 + warps.at(wid);
+  uint32_t left = warps.at(wid + 1) - warps.at(wid);
+  int r = 0;
+  uint32_t seq_at = 0;   // where sequence r begins in the line
+  if (left > 0) {
+    for (int base = 0; base < R; base += 32) {
+      const uint32_t mine = base == 0 ? first : base + lane < R ? seq_work<NT>(p, base + lane) : 0;
+      const uint32_t sum = __reduce_add_sync(0xffffffffu, mine);
+      if (here >= seq_at + sum) { seq_at += sum; continue; }
+      uint32_t x = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) s_tot[wid] = x;
-    __syncthreads();
-    uint32_t at = before + x - mine;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < wid) at += s_tot[w];
-      before += s_tot[w];
-    }
-    if (mine > 0 && at < c1 && at + mine > c0)
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const uint32_t a = c0 + warps.at(w);
-        if (a >= at && a < at + mine) s_place[w] = make_uint2(r, at);
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
       }
+      const int at = __ffs(__ballot_sync(0xffffffffu, here < seq_at + x)) - 1;
+      r = base + at;
+      seq_at += __shfl_sync(0xffffffffu, x - mine, at);
+      break;
+    }
   }
-  __syncthreads();
 
   // ---- this warp's piece
-  uint32_t here = c0 + warps.at(wid), left = warps.at(wid + 1) - warps.at(wid);
   char* ring = att_smem + wid * kRing;
   const uint32_t ring_a = smem_u32(ring), scale_a = smem_u32(&s_scale[wid][0][0]);
   // 16-byte chunk of a row, so that neither reads by rows nor reads by columns meet in a bank
@@ -333,8 +338,6 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
   constexpr int kChunks = D / 16, kRows = 32 / kChunks;   // of one copy instruction
   const int crow = lane / kChunks, cchunk = lane % kChunks;
   if (left > 0) {
-    uint32_t seq_at = s_place[wid].y;
-    int r = (int)s_place[wid].x;
     int n = seq_len(p, r), q0, nq;
     seq_queries(p, r, q0, nq);
     uint32_t steps = steps_of(n);
@@ -402,21 +405,28 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
       float qs[NT][2];        // rows 2t, 2t + 1: scale * log2 e * the row's power of two
       int see[NT][2];         // tokens that they see
       int see_min = n;
-      // query rows: lane (g, t) loads row g's dimensions of its chunks
+      // the query rows come through the ring's last stage, ahead of the first codes
+      const uint32_t q_a = ring_a + kAhead * kStageBytes;
+      const int q_log2 = (D == 128 ? 4 : 3) + (p.a.dtype == CKV_FP32 ? 1 : 0);   // 16-byte chunks of a row
+      for (int i = lane; i < 8 * NT << q_log2; i += 32) {
+        const int row = i >> q_log2, chunk = i & ((1 << q_log2) - 1), rho = tile * NT * 8 + row;
+        int tok, member;
+        row_split(p, rho, tok, member);
+        const char* src = static_cast<const char*>(p.a.q) +
+                          ((q0 + tok) * p.a.q_tok_stride + (head * p.group + member) * p.a.q_head_stride) * (p.a.dtype == CKV_FP32 ? 4 : 2);
+        cp16_or_zero(q_a + (row << q_log2 << 4) + ((chunk ^ (row & 7)) << 4), rho < rows ? src + chunk * 16 : p.a.q, rho < rows ? 16u : 0u);
+      }
+      cp_commit();
+      // lane (g, t) has row g's dimensions of its chunks
       auto load_queries = [&]() {
         float4 x[NT][kSteps16];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const int rho = (tile * NT + nt) * 8 + g;
-          int i, member;
-          row_split(p, rho, i, member);
-          const int64_t at = (q0 + i) * p.a.q_tok_stride + (head * p.group + member) * p.a.q_head_stride;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int k = 0; k < kSteps16; ++k) {
             const int dim = D == 128 ? (2 * t + k / 4) * 16 + (k & 3) * 4 : t * 16 + k * 4;
-            x[nt][k] = rho < rows ? load_q4(p.a.q, p.a.dtype, at + dim) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[nt][k] = load_q4(q_a + ((nt * 8 + g) << q_log2 << 4), g, p.a.dtype, dim);
           }
-        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const int rho = (tile * NT + nt) * 8 + g;
@@ -471,7 +481,12 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
         if (s + kAhead < s_end) issue(s + kAhead, fill);
         cp_commit();
         fill = fill == kStages - 1 ? 0 : fill + 1;
-        if (s + kAhead == s_begin) load_queries();
+        if (s + kAhead == s_begin) {
+          cp_wait<1>();
+          __syncwarp();
+          load_queries();
+          __syncwarp();
+        }
         if (s < s_begin) continue;
         cp_wait<kAhead>();
         __syncwarp();
@@ -693,20 +708,26 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
   // part in slot 0 (begun in a CTA before) or 1 (begun here)
   if (c1 > c0) {
     int4 todo = make_int4(0, 0, 0, 0);
-    const bool used = lane < 2 * kWarps && s_entry[lane].used;   // each warp for itself
-    const uint32_t mask = __ballot_sync(0xffffffffu, used);
-    if (wid == 0 && used) s_order[__popc(mask & ((1u << lane) - 1))] = lane;
-    __syncthreads();
-    const int entries = __popc(mask);
-    for (int i = 0; i < entries;) {
-      const Entry e = s_entry[s_order[i]];
-      const int from = i;
-      while (i < entries && s_entry[s_order[i]].begin == e.begin) ++i;
+    // the used entries in order, and the first of each unit (each warp for itself)
+    const bool used = lane < 2 * kWarps && s_entry[lane].used;
+    const uint32_t mask = __ballot_sync(0xffffffffu, used), below = mask & ((1u << lane) - 1);
+    const uint32_t mine = used ? s_entry[lane].begin : 0;
+    const uint32_t prev = __shfl_sync(0xffffffffu, mine, below ? 31 - __clz(below) : 0);
+    uint32_t firsts = __ballot_sync(0xffffffffu, used && (!below || prev != mine));
+    while (firsts) {
+      const Entry& e = s_entry[__ffs(firsts) - 1];
+      const uint32_t later = firsts & (firsts - 1);
+      uint32_t list = mask & (0u - (firsts & -firsts)) & (later ? (later & -later) - 1 : 0xffffffffu);
+      const int count = __popc(list);
       const bool begins = e.begin >= c0, ends = e.end <= c1;
       float* dst = begins && ends ? nullptr : p.ws + ((size_t)cta * (kAttMaxWarps + 2) + kAttMaxWarps + (begins ? 1 : 0)) * kPart;
-      merge_parts<D, NT, false>(p, [&](int j) { return s_entry[s_order[from + j]].part; }, i - from, tid, kWarps * 32, dst, e.q0,
-                                e.rows, e.head, e.tile);
+      merge_parts<D, NT, false, 4>(p, [list]() mutable {
+        const float* part = s_entry[__ffs(list) - 1].part;
+        list &= list - 1;
+        return part;
+      }, count, tid, kWarps * 32, dst, e.q0, e.rows, e.head, e.tile);
       if (begins && !ends) todo = make_int4((int)(cut.of(e.end - 1) - cta + 1) | e.head << 8, e.q0, e.rows, e.tile);
+      firsts = later;
     }
     if (tid == 0) p.desc[cta] = todo;
   } else if (tid == 0) {
@@ -738,9 +759,13 @@ __global__ void __launch_bounds__(kMergeThreads) k_attend_merge(const AttArgs p)
   const int cta = blockIdx.x;
   const int4 d = __ldcg(p.desc + cta);
   if (!d.x) return;
-  const float* base = p.ws + ((size_t)cta * (kAttMaxWarps + 2) + kAttMaxWarps) * kPart;
-  merge_parts<D, NT, true>(p, [&](int k) { return k ? base + (size_t)k * (kAttMaxWarps + 2) * kPart : base + kPart; }, d.x & 255,
-                           threadIdx.x, kMergeThreads, nullptr, d.y, d.z, d.x >> 8, d.w);
+  const float* part = p.ws + ((size_t)cta * (kAttMaxWarps + 2) + kAttMaxWarps + 1) * kPart;
+  merge_parts<D, NT, true, 8>(p, [part, first = true]() mutable {
+    const float* now = part;
+    part += ((size_t)(kAttMaxWarps + 2) - (first ? 1 : 0)) * kPart;
+    first = false;
+    return now;
+  }, d.x & 255, threadIdx.x, kMergeThreads, nullptr, d.y, d.z, d.x >> 8, d.w);
 }
 
 size_t attention_workspace_bytes(int head_dim, int rows) {
