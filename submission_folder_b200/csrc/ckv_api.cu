@@ -882,7 +882,7 @@ static int check_cache(const ckv_cache* c) {
 
 int ckv_block_tables(const ckv_table_step* s, ckv_stream_t stream) {
   if (!s || !s->lens || !s->new_tokens || !s->tables || !s->free_list || !s->free_count || !s->out_lens ||
-      !s->out_free_count || !s->out_cu || !s->out_granted || (s->total > 0 && (!s->out_slots || !s->out_positions)))
+      !s->out_free_count || !s->out_cu || !s->out_granted || !s->work || (s->total > 0 && (!s->out_slots || !s->out_positions)))
     return fail(CKV_ERR_ARG, "null argument");
   if (s->requests < 1 || s->requests > kMaxRequests) return fail(CKV_ERR_ARG, "1 to 8192 requests");
   if (s->total < 0 || s->table_width < 1 || s->table_stride < s->table_width || s->free_capacity < 0)
@@ -937,6 +937,8 @@ int ckv_cache_read(const ckv_cache* cache, void* k, void* v, int32_t dtype, cons
   const int64_t hs = cache ? cache->head_dim : 0, ts = cache ? hs * cache->num_kv_heads : 0;
   const int rc = cache_rows(cache, k, ts, hs, v, ts, hs, dtype, slots, tokens, &r);
   if (rc || tokens == 0) return rc;
+  if ((int64_t)tokens * cache->num_kv_heads * (cache->head_dim / 16) >= (int64_t)1 << 32)
+    return fail(CKV_ERR_UNSUPPORTED, "too many tokens in one read");
   const cudaError_t e = launch_cache_read(*cache, r, (cudaStream_t)stream);
   return e == cudaSuccess ? CKV_OK : cuda_fail(e, "cache read");
 }

@@ -17,6 +17,8 @@
 // result every time.
 //
 // Bound: HBM; (element size + 1) bytes per element.
+#include <type_traits>
+
 #include "ckv_cache.h"
 #include "ckv_common.cuh"
 
@@ -62,21 +64,60 @@ template <int kFmt> CKV_DEV void decode4(uint32_t w, float (&o)[4]) {
   }
 }
 
-// 16 elements of a row as fp32, and back.
-CKV_DEV void load16(const float* p, float (&x)[16]) {
+// 16 elements of a row as they are, their largest magnitude, and four of them as fp32.
+template <typename T> struct Row16;
+template <> struct Row16<float> {
+  float4 x[4];
+  CKV_DEV void load(const float* p) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float4 v = __ldg(reinterpret_cast<const float4*>(p) + i);
-    x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+    for (int i = 0; i < 4; ++i) x[i] = __ldg(reinterpret_cast<const float4*>(p) + i);
   }
-}
-template <typename H> CKV_DEV void load16(const H* p, float (&x)[16]) {
-  H h[16];
-  *reinterpret_cast<uint4*>(h) = __ldg(reinterpret_cast<const uint4*>(p));
-  *reinterpret_cast<uint4*>(h + 8) = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+  CKV_DEV void clear() {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = to_f32(h[i]);
-}
+    for (int i = 0; i < 4; ++i) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  CKV_DEV float4 get(int i) const { return x[i]; }
+  CKV_DEV uint32_t amax(uint32_t top) const {   // magnitudes are ordered as their bits, NaN above infinity
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      top = max(top, __float_as_uint(x[i].x) & 0x7fffffffu);
+      top = max(top, __float_as_uint(x[i].y) & 0x7fffffffu);
+      top = max(top, __float_as_uint(x[i].z) & 0x7fffffffu);
+      top = max(top, __float_as_uint(x[i].w) & 0x7fffffffu);
+    }
+    return top;
+  }
+  static CKV_DEV uint32_t fp32_bits(uint32_t top) { return top; }
+};
+template <typename H> struct Row16 {
+  uint32_t w[8];
+  CKV_DEV void load(const H* p) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+  }
+  CKV_DEV void clear() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 0;
+  }
+  CKV_DEV float4 get(int i) const {
+    const float2 a = f2(w[2 * i]), b = f2(w[2 * i + 1]);
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+  CKV_DEV uint32_t amax(uint32_t top) const {   // of both halves of the words
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+    return top;
+  }
+  static CKV_DEV uint32_t fp32_bits(uint32_t top) {
+    const uint32_t m = max(top & 0xffffu, top >> 16);
+    return __float_as_uint(f2(m).x);
+  }
+  static CKV_DEV float2 f2(uint32_t v) {
+    if constexpr (sizeof(H) == 2 && std::is_same<H, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+    else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+  }
+};
 CKV_DEV void store16(float* p, const float (&x)[16]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -152,33 +193,30 @@ __global__ void __launch_bounds__(kCacheMaxBlock / kRowsPerWarp * 32) k_cache_wr
     }
     const int64_t sidx = blk * a.c.num_kv_heads + h;
     const float old = anew ? 0.f : scales[sidx];
-    if (threadIdx.x < kCacheMaxBlock / 32) s_new[threadIdx.x] = 0;
     const int rows_per_round = nw * kRowsPerWarp;
     const bool once = end - t <= rows_per_round;
-    float x[kSteps][16];
+    Row16<T> x[kSteps];
     uint32_t top = 0;
     for (int r0 = t; r0 < end; r0 += rows_per_round) {
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         const int i = r0 + wid * kRowsPerWarp + s * kRowsPerStep + lane / kLanesPerRow;
-        if (i < end) load16(src + i * ts + (lane % kLanesPerRow) * 16, x[s]);
-        else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[s][e] = 0.f;
-        }
+        if (i < end) x[s].load(src + i * ts + (lane % kLanesPerRow) * 16);
+        else x[s].clear();
       }
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = max(top, __float_as_uint(x[s][e]) & 0x7fffffffu);
+      for (int s = 0; s < kSteps; ++s) top = x[s].amax(top);
     }
-    top = __reduce_max_sync(0xffffffffu, top);
-    __syncthreads();   // s_new cleared, the last run's s_max read
+    top = __reduce_max_sync(0xffffffffu, Row16<T>::fp32_bits(top));
+    if (!anew) {   // which places of the block this run writes
+      if (threadIdx.x < kCacheMaxBlock / 32) s_new[threadIdx.x] = 0;
+      __syncthreads();
+      for (int i = t + threadIdx.x; i < end; i += blockDim.x) {
+        const int o = (int)(__ldg(slots + i) & (bs - 1));
+        atomicOr(&s_new[o >> 5], 1u << (o & 31));
+      }
+    }
     if (lane == 0) s_max[wid] = top;
-    for (int i = t + threadIdx.x; i < end; i += blockDim.x) {
-      const int o = (int)(__ldg(slots + i) & (bs - 1));
-      atomicOr(&s_new[o >> 5], 1u << (o & 31));
-    }
     __syncthreads();
     for (int w = 0; w < nw; ++w) top = max(top, s_max[w]);
     float scale = scale_for<kFmt>(top);
@@ -198,18 +236,20 @@ __global__ void __launch_bounds__(kCacheMaxBlock / kRowsPerWarp * 32) k_cache_wr
           for (int j = i + 1; j < end; ++j) again = again || __ldg(slots + j) == slot;
           if (again) continue;
         }
-        if (!once) load16(src + i * ts + (lane % kLanesPerRow) * 16, x[s]);
+        if (!once) x[s].load(src + i * ts + (lane % kLanesPerRow) * 16);
         uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          w[e] = bad ? 0u : encode4<kFmt>(x[s][4 * e] * inv, x[s][4 * e + 1] * inv, x[s][4 * e + 2] * inv, x[s][4 * e + 3] * inv);
+        for (int e = 0; e < 4; ++e) {
+          const float4 f = x[s].get(e);
+          w[e] = bad ? 0u : encode4<kFmt>(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
+        }
         *reinterpret_cast<uint4*>(blk_dst + (slot & (bs - 1)) * tstr + (lane % kLanesPerRow) * 16) =
             make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
     if (!anew && !bad && scale > old) {   // the tokens that stay, in the new scale
       const float ratio = old * inv;
-#pragma unroll
+#pragma unroll 1
       for (int s = 0; s < kSteps; ++s) {
         const int o = wid * kRowsPerWarp + s * kRowsPerStep + lane / kLanesPerRow;
         if (o >= bs || (s_new[o >> 5] >> (o & 31) & 1u)) continue;
@@ -231,39 +271,54 @@ __global__ void __launch_bounds__(kCacheMaxBlock / kRowsPerWarp * 32) k_cache_wr
   }
 }
 
-// One thread per 16 codes: grid over tokens * heads * D / 16, z = K / V.
+// A thread has 16 codes of K and of V of kReadTokens tokens (two of them half the list apart):
+// the slots first, then all codes and scales, then the stores, so that four loads of 16 bytes
+// are in flight.
+constexpr int kReadTokens = 2;
 template <typename T, int kFmt>
 __global__ void __launch_bounds__(256) k_cache_read(const ckv_cache c, const CacheRows r, int block_log2) {
-  const int per_row = c.head_dim / 16;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int v16 = (int)(i % per_row);
-  const int64_t th = i / per_row;
-  const int h = (int)(th % c.num_kv_heads);
-  const int64_t t = th / c.num_kv_heads;
-  if (t >= r.tokens) return;
-  const bool isv = blockIdx.y != 0;
-  const int64_t s = __ldg(r.slots + t);
-  float x[16];
-  if (s >= 0 && s < ((int64_t)c.num_blocks << block_log2)) {
-    const int64_t blk = s >> block_log2, o = s & (c.block_size - 1);
-    const char* p = isv ? static_cast<const char*>(c.v) + blk * c.v_block_stride + h * c.v_head_stride + o * c.v_tok_stride
+  const uint32_t per_row = c.head_dim / 16, per_tok = per_row * c.num_kv_heads;
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x, half = (r.tokens + kReadTokens - 1) / kReadTokens;
+  const uint32_t t = i / per_tok;
+  if (t >= half) return;
+  const uint32_t h = (i - t * per_tok) / per_row, v16 = i - t * per_tok - h * per_row;
+  const int64_t pool = (int64_t)c.num_blocks << block_log2;
+  int64_t slot[kReadTokens];
+#pragma unroll
+  for (int j = 0; j < kReadTokens; ++j) slot[j] = t + j * half < (uint32_t)r.tokens ? __ldg(r.slots + t + j * half) : -1;
+  uint4 q[kReadTokens][2];
+  float sc[kReadTokens][2];
+#pragma unroll
+  for (int j = 0; j < kReadTokens; ++j)
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      q[j][v] = make_uint4(0, 0, 0, 0);
+      sc[j][v] = 0.f;
+      if (slot[j] < 0 || slot[j] >= pool) continue;
+      const int64_t blk = slot[j] >> block_log2, o = slot[j] & (c.block_size - 1);
+      const char* p = v ? static_cast<const char*>(c.v) + blk * c.v_block_stride + h * c.v_head_stride + o * c.v_tok_stride
                         : static_cast<const char*>(c.k) + blk * c.k_block_stride + h * c.k_head_stride + o * c.k_tok_stride;
-    const uint4 q = *(reinterpret_cast<const uint4*>(p) + v16);
-    const float sc = (isv ? c.v_scale : c.k_scale)[blk * c.num_kv_heads + h];
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float f[4];
-      decode4<kFmt>(w[e], f);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[4 * e + k] = f[k] * sc;
+      q[j][v] = *(reinterpret_cast<const uint4*>(p) + v16);
+      sc[j][v] = (v ? c.v_scale : c.k_scale)[blk * c.num_kv_heads + h];
     }
-  } else {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = 0.f;
-  }
-  T* out = isv ? static_cast<T*>(r.v) + t * r.vts + h * r.vhs : static_cast<T*>(r.k) + t * r.kts + h * r.khs;
-  store16(out + v16 * 16, x);
+  for (int j = 0; j < kReadTokens; ++j)
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      if (t + j * half >= (uint32_t)r.tokens) continue;
+      const uint32_t w[4] = {q[j][v].x, q[j][v].y, q[j][v].z, q[j][v].w};
+      float x[16];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float f[4];
+        decode4<kFmt>(w[e], f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[4 * e + k] = f[k] * sc[j][v];
+      }
+      T* out = v ? static_cast<T*>(r.v) + (int64_t)(t + j * half) * r.vts + h * r.vhs
+                 : static_cast<T*>(r.k) + (int64_t)(t + j * half) * r.kts + h * r.khs;
+      store16(out + v16 * 16, x);
+    }
 }
 
 static int log2_of(int x) {
@@ -302,8 +357,8 @@ cudaError_t launch_cache_write(const ckv_cache& c, const CacheRows& r, cudaStrea
 }
 
 cudaError_t launch_cache_read(const ckv_cache& c, const CacheRows& r, cudaStream_t st) {
-  const int64_t n = (int64_t)r.tokens * c.num_kv_heads * (c.head_dim / 16);
-  const dim3 grid((unsigned)((n + 255) / 256), 2);
+  const int64_t n = ((int64_t)r.tokens + kReadTokens - 1) / kReadTokens * c.num_kv_heads * (c.head_dim / 16);
+  const dim3 grid((unsigned)((n + 255) / 256));
   const int bl = log2_of(c.block_size);
   const bool e4 = c.format == CKV_CACHE_E4M3;
   switch (r.dtype) {

@@ -17,7 +17,6 @@
 namespace ckv {
 
 constexpr int kRotThreads = 256;
-constexpr int kRotMaxDim = 512;
 
 template <typename T> CKV_DEV T from_f32(float x);
 template <> CKV_DEV float from_f32<float>(float x) { return x; }
@@ -26,8 +25,8 @@ template <> CKV_DEV __half from_f32<__half>(float x) { return __float2half_rn(x)
 
 template <typename T, int N> struct alignas(sizeof(T) * N) Vec { T x[N]; };
 
-// One unit = N elements of the first halves and their N partners (half layout), 2N adjacent
-// elements (interleaved), or N elements past the rotated part.
+// A unit is 2N elements: N of the first half and their N partners (half layout), or 2N adjacent
+// ones (interleaved), or 2N past the rotated part (N at its end, where that is odd).
 template <typename T, int N, bool kInter>
 __global__ void __launch_bounds__(kRotThreads) k_rotary(const ckv_rotary_args a, int tokens_per_cta) {
   extern __shared__ float2 rot_cs[];   // [tokens_per_cta][pairs]
@@ -46,7 +45,7 @@ __global__ void __launch_bounds__(kRotThreads) k_rotary(const ckv_rotary_args a,
   }
   __syncthreads();
   const int turn_units = pairs / N;                                   // per head
-  const int rest_units = (a.head_dim - a.rotary_dim) / N;
+  const int rest_units = (a.head_dim - a.rotary_dim + 2 * N - 1) / (2 * N);
   const int units = turn_units + rest_units;
   const int heads = a.q_heads + a.k_heads;
   const int h0 = blockIdx.y * a.heads_per_cta, h1 = min(heads, h0 + a.heads_per_cta);
@@ -90,8 +89,10 @@ __global__ void __launch_bounds__(kRotThreads) k_rotary(const ckv_rotary_args a,
       *reinterpret_cast<V*>(dst + i0) = ox;
       *reinterpret_cast<V*>(dst + i1) = oy;
     } else if (src != dst) {
-      const int i0 = a.rotary_dim + (u - turn_units) * N;
-      *reinterpret_cast<V*>(dst + i0) = *reinterpret_cast<const V*>(src + i0);
+      const int i0 = a.rotary_dim + (u - turn_units) * 2 * N, i1 = i0 + N;
+      const V x = *reinterpret_cast<const V*>(src + i0);
+      if (i1 < a.head_dim) *reinterpret_cast<V*>(dst + i1) = *reinterpret_cast<const V*>(src + i1);
+      *reinterpret_cast<V*>(dst + i0) = x;
     }
   }
 }

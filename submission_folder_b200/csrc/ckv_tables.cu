@@ -6,20 +6,16 @@
 // ceil((len + new) / b) - ceil(len / b) more; new < 0 ends it and gives its blocks back.
 // The free blocks are a stack.  Blocks given back go on top (requests in order, blocks in
 // order); fresh blocks come off the top (requests in order, blocks in order).  All of it is
-// three prefix sums over the requests (tokens, blocks back, blocks needed), held in shared
-// memory by every CTA, after which each token and each block finds its request by binary
-// search and is written independently.
+// three prefix sums over the requests (tokens, blocks back, blocks needed); after them each
+// token and each block finds its request by binary search and its block by arithmetic on the
+// sums, independently of all others (a block that is given back and taken in the same step is
+// looked up where it was given back, not where it is put down).
 //
-// Bound: latency (a few loads per request, one dependent scan, one round of stores).  One
-// CTA handles a decode step; above kOneCta tokens a cluster of 8 CTAs shares the stores
-// (the cluster, because the new lengths may overwrite the old ones in place: every CTA has
-// to have read them before any CTA writes).
-#include <cooperative_groups.h>
-
+// Bound: latency.  A small step is one CTA: scan, then stores.  Above kOneCta tokens and
+// requests the stores go to a second launch over the whole GPU (one CTA's search and stores of
+// 630,000 tokens took 126 us on a cluster of 8 CTAs; in two launches the step takes 9).
 #include "ckv_cache.h"
 #include "ckv_common.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace ckv {
 
@@ -63,17 +59,72 @@ CKV_DEV Sum3 scan3(Sum3 v, Sum3* scratch, Sum3* total) {
   return {base.tok + x.tok - v.tok, base.back + x.back - v.back, base.need + x.need - v.need};
 }
 
+// p[i]; kL2: written by the launch before, read from L2.
+template <bool kL2> CKV_DEV int get(const int* p, int i) { return kL2 ? __ldcg(p + i) : p[i]; }
+
 // Last row in [lo, hi] whose prefix p[row] is <= x (p ascending, p[lo] <= x).
-CKV_DEV int row_of(const int* p, int lo, int hi, int x) {
+template <bool kL2> CKV_DEV int row_of(const int* p, int lo, int hi, int x) {
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (p[mid] <= x) lo = mid;
+    if (get<kL2>(p, mid) <= x) lo = mid;
     else hi = mid - 1;
   }
   return lo;
 }
 
-__global__ void __launch_bounds__(kTabThreads) k_block_tables(const ckv_table_step s) {
+// What the scan leaves for the stores: prefixes over the requests, and per request the old length
+// and the tokens granted; the stack's height before (count), with what came back (have), and the
+// blocks taken.
+struct StepView {
+  const int *cu, *back, *fresh, *len, *give;
+  int count, have, taken;
+};
+
+// Stores of the threads gt of gn: blocks given back, table entries, slots and positions.  cu is in
+// shared memory; kL2: the rest of the view is the scan's, in global memory.
+template <bool kL2> CKV_DEV void fill_step(const ckv_table_step& s, const StepView& v, int gt, int gn) {
+  const int R = s.requests, lane = threadIdx.x & 31;
+  const uint32_t b = s.block_size;
+  // the j-th block from the bottom of the stack, after the blocks given back went on top
+  auto stack = [&](int j) -> int {
+    if (j < v.count) return __ldcg(s.free_list + j);
+    const int e = j - v.count, r = row_of<kL2>(v.back, 0, R - 1, e);
+    return __ldcg(s.tables + r * s.table_stride + (e - get<kL2>(v.back, r)));
+  };
+  for (int i = gt; i < v.have - v.count; i += gn) s.free_list[v.count + i] = stack(v.count + i);
+  for (int i = gt; i < v.taken; i += gn) {
+    const int r = row_of<kL2>(v.fresh, 0, R - 1, i);
+    s.tables[r * s.table_stride + ((uint32_t)get<kL2>(v.len, r) + b - 1) / b + (i - get<kL2>(v.fresh, r))] = stack(v.have - 1 - i);
+  }
+  // tokens: a warp takes 128 at a time, its rows bracketed by two searches
+  const int asked = v.cu[R], warp = gt >> 5, warps = gn >> 5;
+  for (int t0 = warp * 128; t0 < s.total; t0 += warps * 128) {
+    const int first = row_of<false>(v.cu, 0, R - 1, min(t0, max(asked - 1, 0)));
+    const int last = row_of<false>(v.cu, first, R - 1, min(t0 + 127, max(asked - 1, 0)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = t0 + i * 32 + lane;
+      if (t >= s.total) break;
+      long long slot = -1, where = 0;
+      if (t < asked) {
+        const int r = row_of<false>(v.cu, first, last, t);
+        const uint32_t n = get<kL2>(v.len, r), pos = n + (uint32_t)(t - v.cu[r]);
+        where = (long long)pos + (s.shift ? s.shift[r] : 0);
+        if (get<kL2>(v.give, r) > 0) {
+          const uint32_t bi = pos / b, held = (n + b - 1) / b;
+          const int block = bi < held ? __ldcg(s.tables + r * s.table_stride + bi)
+                                      : stack(v.have - 1 - (get<kL2>(v.fresh, r) + (int)(bi - held)));
+          slot = (long long)block * b + (pos - bi * b);
+        }
+      }
+      s.out_slots[t] = slot;
+      s.out_positions[t] = where;
+    }
+  }
+}
+
+// The scan, by one CTA; and the stores, when they are few.
+__global__ void __launch_bounds__(kTabThreads) k_block_tables(const ckv_table_step s, int solo) {
   extern __shared__ int tab_smem[];
   __shared__ Sum3 scratch[32];
   __shared__ int s_taken;
@@ -82,25 +133,27 @@ __global__ void __launch_bounds__(kTabThreads) k_block_tables(const ckv_table_st
   int* back = cu + R + 1;         // [R + 1] blocks given back before request r
   int* fresh = back + R + 1;      // [R + 1] fresh blocks wanted before request r
   int* len = fresh + R + 1;       // [R] old length
-  int* ok = len + R;              // [R] 1: the request's tokens are granted
+  int* give = len + R;            // [R] tokens granted; before that -2: ended, -1: does not fit its row
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) s_taken = 0;
-  const int count = min(max(__ldcg(s.free_count), 0), s.free_capacity);
+  const int count = min(max(*s.free_count, 0), s.free_capacity);
   Sum3 run = {0, 0, 0};
   for (int base = 0; base < R; base += blockDim.x) {
     const int r = base + tid;
     Sum3 v = {0, 0, 0};
     if (r < R) {
-      const int n = max(__ldcg(s.lens + r), 0), nw = __ldcg(s.new_tokens + r);
-      const int held = (int)(((long long)n + b - 1) / b);
+      const int n = max(s.lens[r], 0), nw = s.new_tokens[r];
+      const int held = (int)(((uint32_t)n + b - 1) / b);
       len[r] = n;
       if (nw < 0) {
         v.back = min(held, s.table_width);
-        ok[r] = 2;                // ended
+        give[r] = -2;
       } else {
         v.tok = nw;
-        const long long want = ((long long)n + nw + b - 1) / b;
-        ok[r] = want <= s.table_width ? 1 : 0;
-        v.need = ok[r] ? (int)want - held : 0;
+        const uint32_t want = (uint32_t)n + nw == 0 ? 0u : ((uint32_t)n + nw - 1) / b + 1;
+        const bool fits = want <= (uint32_t)s.table_width && (uint32_t)n + nw <= (uint32_t)INT32_MAX;
+        give[r] = fits ? nw : -1;
+        v.need = fits ? (int)want - held : 0;
       }
     }
     Sum3 total;
@@ -120,84 +173,69 @@ __global__ void __launch_bounds__(kTabThreads) k_block_tables(const ckv_table_st
   __syncthreads();
   const int have = (int)min((long long)count + run.back, (long long)s.free_capacity);
   for (int r = tid; r < R; r += blockDim.x) {   // fresh blocks go to the requests in order while they last
-    const int need = fresh[r + 1] - fresh[r];
-    if (ok[r] == 1 && need > 0) {
+    const int need = fresh[r + 1] - fresh[r], was = give[r];
+    if (was >= 0 && need > 0) {
       if (fresh[r + 1] <= have) atomicMax(&s_taken, fresh[r + 1]);
-      else ok[r] = 0;
+      else give[r] = -1;
     }
-  }
-  cg::cluster_group cl = cg::this_cluster();
-  cl.sync();   // every CTA has read the old lengths and the old count
-  const int rank = (int)cl.block_rank(), nranks = (int)cl.num_blocks();
-  const int gt = rank * blockDim.x + tid, gn = nranks * blockDim.x;
-  const int taken = s_taken;
-
-  // the j-th block from the bottom of the stack, after the blocks given back went on top
-  auto stack = [&](int j) -> int {
-    if (j < count) return __ldcg(s.free_list + j);
-    const int e = j - count, r = row_of(back, 0, R - 1, e);
-    return __ldcg(s.tables + r * s.table_stride + (e - back[r]));
-  };
-  for (int i = gt; i < have - count; i += gn) s.free_list[count + i] = stack(count + i);
-  for (int i = gt; i < taken; i += gn) {
-    const int r = row_of(fresh, 0, R - 1, i);
-    s.tables[r * s.table_stride + (len[r] + b - 1) / b + (i - fresh[r])] = stack(have - 1 - i);
-  }
-  for (int r = gt; r <= R; r += gn) {
+    const int granted = max(give[r], 0);
+    give[r] = granted;
     s.out_cu[r] = cu[r];
-    if (r == R) break;
-    const int give = ok[r] == 1 ? cu[r + 1] - cu[r] : 0;
-    s.out_granted[r] = give;
-    s.out_lens[r] = ok[r] == 2 ? 0 : len[r] + give;
+    s.out_granted[r] = granted;
+    s.out_lens[r] = was == -2 ? 0 : len[r] + granted;
   }
-  if (gt == 0) s.out_free_count[0] = have - taken;
-
-  // tokens: a warp takes 128 at a time, its rows bracketed by two searches
-  const int lane = tid & 31, asked = cu[R];
-  for (int t0 = (gt >> 5) * 128; t0 < s.total; t0 += (gn >> 5) * 128) {
-    const int first = row_of(cu, 0, R - 1, min(t0, max(asked - 1, 0)));
-    const int last = row_of(cu, first, R - 1, min(t0 + 127, max(asked - 1, 0)));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = t0 + i * 32 + lane;
-      if (t >= s.total) break;
-      long long slot = -1, where = 0;
-      if (t < asked) {
-        const int r = row_of(cu, first, last, t);
-        const long long pos = (long long)len[r] + (t - cu[r]);
-        where = pos + (s.shift ? s.shift[r] : 0);
-        if (ok[r] == 1) {
-          const int bi = (int)(pos / b), held = (len[r] + b - 1) / b;
-          const int block = bi < held ? __ldcg(s.tables + r * s.table_stride + bi)
-                                      : stack(have - 1 - (fresh[r] + bi - held));
-          slot = (long long)block * b + pos % b;
-        }
-      }
-      s.out_slots[t] = slot;
-      s.out_positions[t] = where;
-    }
+  __syncthreads();
+  const int taken = s_taken;
+  if (tid == 0) {
+    s.out_cu[R] = cu[R];
+    s.out_free_count[0] = have - taken;
   }
+  if (solo) {
+    fill_step<false>(s, StepView{cu, back, fresh, len, give, count, have, taken}, tid, blockDim.x);
+    return;
+  }
+  int* w = s.work;                // [3 * (R + 1)]: back, fresh, old length, then count, have, taken
+  for (int r = tid; r <= R; r += blockDim.x) {
+    w[r] = back[r];
+    w[R + 1 + r] = fresh[r];
+    if (r < R) w[2 * (R + 1) + r] = len[r];
+  }
+  if (tid == 0) { w[3 * (R + 1)] = count; w[3 * (R + 1) + 1] = have; w[3 * (R + 1) + 2] = taken; }
 }
 
-constexpr int kOneCta = 8192;   // tokens up to which one CTA makes the step
+constexpr int kFillThreads = 512;
+
+__global__ void __launch_bounds__(kFillThreads) k_block_tables_fill(const ckv_table_step s) {
+  extern __shared__ int tab_smem[];   // [R + 1] cu: searched most
+  const int R = s.requests;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int r = threadIdx.x; r <= R; r += kFillThreads) tab_smem[r] = __ldcg(s.out_cu + r);
+  const int* w = s.work;
+  const int count = __ldcg(w + 3 * (R + 1)), have = __ldcg(w + 3 * (R + 1) + 1), taken = __ldcg(w + 3 * (R + 1) + 2);
+  __syncthreads();
+  fill_step<true>(s, StepView{tab_smem, w, w + R + 1, w + 2 * (R + 1), s.out_granted, count, have, taken},
+            blockIdx.x * kFillThreads + threadIdx.x, gridDim.x * kFillThreads);
+}
+
+constexpr int kOneCta = 4096;   // tokens and requests up to which one CTA makes the step
 
 cudaError_t launch_block_tables(const ckv_table_step& s, cudaStream_t st) {
   const size_t smem = (size_t)(5 * s.requests + 3) * sizeof(int);
   if (cudaError_t e = ensure_dynamic_smem((const void*)k_block_tables, smem); e != cudaSuccess) return e;
+  const bool solo = (int64_t)s.total + s.requests <= kOneCta;
+  k_block_tables<<<1, kTabThreads, smem, st>>>(s, solo ? 1 : 0);
+  if (cudaError_t e = cudaGetLastError(); solo || e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  const int ctas = s.total > kOneCta ? 8 : 1;
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(kTabThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3(2 * 148);
+  cfg.blockDim = dim3(kFillThreads);
+  cfg.dynamicSmemBytes = (size_t)(s.requests + 1) * sizeof(int);
   cfg.stream = st;
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_block_tables, s);
+  return cudaLaunchKernelEx(&cfg, k_block_tables_fill, s);
 }
 
 }  // namespace ckv

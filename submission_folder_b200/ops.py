@@ -503,7 +503,8 @@ def block_tables(lens: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, fr
         _need(total >= 0, "total must not be negative")
         raise ValueError("tables must be an int32 tensor [requests, width] with contiguous rows")
     dev, width = lens.device, tables.shape[1]
-    cu = torch.empty(R + 1, dtype=i32, device=dev)
+    small = torch.empty(4 * R + 7, dtype=i32, device=dev)   # cu, then scratch
+    cu = small[:R + 1]
     granted = torch.empty(R, dtype=i32, device=dev)
     slots = torch.empty(total, dtype=torch.int64, device=dev)
     positions = torch.empty(total, dtype=torch.int64, device=dev)
@@ -511,7 +512,7 @@ def block_tables(lens: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, fr
         lens.data_ptr(), new.data_ptr(), 0 if shift is None else shift.data_ptr(), tables.data_ptr(),
         max(tables.stride(0), width), width, free_list.data_ptr(), free_list.shape[0], free_count.data_ptr(), block_size, R,
         total, lens_out.data_ptr(), free_count_out.data_ptr(), cu.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-        granted.data_ptr()))
+        granted.data_ptr(), small.data_ptr() + 4 * (R + 1)))
     return TableStep(lens_out, free_count_out, cu, slots, positions, granted)
 
 

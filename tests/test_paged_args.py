@@ -74,13 +74,13 @@ def test_attention_workspace_is_checked():
     assert lib.ckv_cache_attention_workspace(128, 1, 8, 2, None) == -1
 
 
-@pytest.mark.parametrize("over", [dict(lens=None), dict(out_slots=None), dict(out_granted=None), dict(requests=0), dict(requests=8193),
+@pytest.mark.parametrize("over", [dict(lens=None), dict(out_slots=None), dict(out_granted=None), dict(work=None), dict(requests=0), dict(requests=8193),
                                   dict(total=-1), dict(table_width=0), dict(table_stride=1), dict(block_size=0),
                                   dict(free_capacity=-1)])
 def test_bad_table_steps_are_refused(over):
     a = dict(lens=P, new_tokens=P, tables=P, table_stride=4, table_width=4, free_list=P, free_capacity=8, free_count=P,
              block_size=16, requests=2, total=2, out_lens=P, out_free_count=P, out_cu=P, out_slots=P, out_positions=P,
-             out_granted=P)
+             out_granted=P, work=P)
     a.update(over)
     s = _lib.TableStep(**a)
     assert _lib.load().ckv_block_tables(ctypes.byref(s), None) == -1
