@@ -872,8 +872,8 @@ static int check_cache(const ckv_cache* c) {
   if (c->head_dim != 64 && c->head_dim != 128) return fail(CKV_ERR_UNSUPPORTED, "cache head_dim must be 64 or 128");
   if (c->block_size != 16 && c->block_size != 32 && c->block_size != 64 && c->block_size != 128)
     return fail(CKV_ERR_UNSUPPORTED, "cache block_size must be 16, 32, 64 or 128");
-  if (c->num_blocks < 1 || c->num_kv_heads < 1 || c->num_kv_heads > 65535)
-    return fail(CKV_ERR_ARG, "cache needs at least one block and 1 to 65535 heads");
+  if (c->num_blocks < 1 || c->num_kv_heads < 1 || c->num_kv_heads > 32767)
+    return fail(CKV_ERR_ARG, "cache needs at least one block and 1 to 32767 heads");
   if (!aligned16(c->k, c->k_block_stride, c->k_head_stride, 1) || c->k_tok_stride % 16 ||
       !aligned16(c->v, c->v_block_stride, c->v_head_stride, 1) || c->v_tok_stride % 16)
     return fail(CKV_ERR_ARG, "cache pointers and strides must be multiples of 16 bytes");

@@ -39,15 +39,18 @@ template <int kFmt> CKV_DEV float scale_for(uint32_t amax_bits) {
 // 1 / scale of a power of two in [2^-126, 2^121].
 CKV_DEV float inv_pow2(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
-// Four codes from four values already divided by the scale.
-template <int kFmt> CKV_DEV uint32_t encode4(float a, float b, float c, float d) {
+// Four codes from four values times the inverse scale (a power of two: the product is exact).
+// int8: adding 1.5 2^23 leaves the nearest whole number, ties to even, in the low byte.
+template <int kFmt> CKV_DEV uint32_t encode4(float a, float b, float c, float d, float inv) {
   uint32_t r;
   if constexpr (kFmt == CKV_CACHE_E4M3) {
     asm("{\n.reg .b16 lo, hi;\ncvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\ncvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n"
-        "mov.b32 %0, {lo, hi};\n}\n" : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
+        "mov.b32 %0, {lo, hi};\n}\n" : "=r"(r) : "f"(a * inv), "f"(b * inv), "f"(c * inv), "f"(d * inv));
   } else {
-    const int x = __float2int_rn(a), y = __float2int_rn(b), z = __float2int_rn(c), w = __float2int_rn(d);
-    r = (uint32_t)(x & 255) | (uint32_t)(y & 255) << 8 | (uint32_t)(z & 255) << 16 | (uint32_t)(w & 255) << 24;
+    constexpr float kMagic = 12582912.f;
+    const uint32_t x = __float_as_uint(fmaf(a, inv, kMagic)), y = __float_as_uint(fmaf(b, inv, kMagic));
+    const uint32_t z = __float_as_uint(fmaf(c, inv, kMagic)), w = __float_as_uint(fmaf(d, inv, kMagic));
+    r = __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
   }
   return r;
 }
@@ -144,128 +147,152 @@ struct WriteArgs {
   CacheRows r;
   int piece;       // tokens of the list whose runs a CTA owns
   int block_log2;
+  int items;       // of the 2 * heads (head, K / V) pairs, how many a CTA writes
 };
 
-// grid (pieces, heads, 2); block_size / 16 warps.
+// grid (pieces, 2 * heads / items); block_size / 16 warps.
 template <typename T, int kFmt, int D>
 __global__ void __launch_bounds__(kCacheMaxBlock / kRowsPerWarp * 32) k_cache_write(const WriteArgs a) {
   constexpr int kLanesPerRow = D / 16, kRowsPerStep = 32 / kLanesPerRow, kSteps = kRowsPerWarp / kRowsPerStep;
-  __shared__ uint32_t s_max[kCacheMaxBlock / kRowsPerWarp];
-  __shared__ uint32_t s_new[kCacheMaxBlock / 32];   // offsets of the block that this run writes
+  __shared__ uint32_t s_max[2][kCacheMaxBlock / kRowsPerWarp];   // of this item and the next
+  __shared__ uint32_t s_new[kCacheMaxBlock / 32];                // places of the block that this run writes
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  const int h = blockIdx.y;
-  const bool isv = blockIdx.z != 0;
   const int bs = a.c.block_size, T0 = blockIdx.x * a.piece, T1 = min(a.r.tokens, T0 + a.piece);
+  const int item0 = blockIdx.y * a.items, item1 = min(2 * a.c.num_kv_heads, item0 + a.items);
   const int64_t pool = (int64_t)a.c.num_blocks << a.block_log2;
-  const T* src = static_cast<const T*>(isv ? a.r.v : a.r.k) + h * (isv ? a.r.vhs : a.r.khs);
-  const int64_t ts = isv ? a.r.vts : a.r.kts;
-  char* dst = static_cast<char*>(isv ? a.c.v : a.c.k) + h * (isv ? a.c.v_head_stride : a.c.k_head_stride);
-  const int64_t bstr = isv ? a.c.v_block_stride : a.c.k_block_stride, tstr = isv ? a.c.v_tok_stride : a.c.k_tok_stride;
-  float* scales = isv ? a.c.v_scale : a.c.k_scale;
   const int64_t* slots = a.r.slots;
-  auto block_of = [&](int t) -> int64_t {
+  auto block_of = [&](int t) -> int {
     const int64_t s = __ldg(slots + t);
-    return s >= 0 && s < pool ? s >> a.block_log2 : -1;
+    return s >= 0 && s < pool ? (int)(s >> a.block_log2) : -1;
   };
   int t = T0;
   while (t < T1) {   // every warp takes the same path
     // the next token that begins a run: its block is not the token's before it
     const int cand = t + lane;
-    const int64_t mine = cand < T1 ? block_of(cand) : -1;
+    const int mine = cand < T1 ? block_of(cand) : -1;
     const uint32_t begins = __ballot_sync(0xffffffffu, mine >= 0 && (cand == 0 || block_of(cand - 1) != mine));
     if (begins == 0) { t += 32; continue; }
     t += __ffs(begins) - 1;
-    const int64_t blk = __shfl_sync(0xffffffffu, mine, __ffs(begins) - 1);
+    const int blk = __shfl_sync(0xffffffffu, mine, __ffs(begins) - 1);
     // the run's end, and whether it has the block's first token and rising slots
     int end = t;
     bool rising = true, anew = false;
     for (bool more = true; more;) {
       const int i = end + lane;
-      const bool in = i < a.r.tokens && block_of(i) == blk;
+      const int64_t s = i < a.r.tokens ? __ldg(slots + i) : -1;
+      const bool in = s >= 0 && s < pool && (int)(s >> a.block_log2) == blk;
       const uint32_t m = __ballot_sync(0xffffffffu, in);
       const int n = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
       const bool own = lane < n;
-      const int64_t s = own ? __ldg(slots + i) : 0;
       rising = rising && __all_sync(0xffffffffu, !own || i == t || __ldg(slots + i - 1) < s);
-      anew = anew || __any_sync(0xffffffffu, own && (s & (bs - 1)) == 0);
+      anew = anew || __any_sync(0xffffffffu, own && ((int)s & (bs - 1)) == 0);
       end += n;
       more = n == 32;
     }
-    const int64_t sidx = blk * a.c.num_kv_heads + h;
-    const float old = anew ? 0.f : scales[sidx];
-    const int rows_per_round = nw * kRowsPerWarp;
-    const bool once = end - t <= rows_per_round;
-    Row16<T> x[kSteps];
-    uint32_t top = 0;
-    for (int r0 = t; r0 < end; r0 += rows_per_round) {
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int i = r0 + wid * kRowsPerWarp + s * kRowsPerStep + lane / kLanesPerRow;
-        if (i < end) x[s].load(src + i * ts + (lane % kLanesPerRow) * 16);
-        else x[s].clear();
-      }
-#pragma unroll
-      for (int s = 0; s < kSteps; ++s) top = x[s].amax(top);
-    }
-    top = __reduce_max_sync(0xffffffffu, Row16<T>::fp32_bits(top));
-    if (!anew) {   // which places of the block this run writes
+    if (!anew) {
       if (threadIdx.x < kCacheMaxBlock / 32) s_new[threadIdx.x] = 0;
       __syncthreads();
       for (int i = t + threadIdx.x; i < end; i += blockDim.x) {
-        const int o = (int)(__ldg(slots + i) & (bs - 1));
+        const int o = (int)__ldg(slots + i) & (bs - 1);
         atomicOr(&s_new[o >> 5], 1u << (o & 31));
       }
     }
-    if (lane == 0) s_max[wid] = top;
-    __syncthreads();
-    for (int w = 0; w < nw; ++w) top = max(top, s_max[w]);
-    float scale = scale_for<kFmt>(top);
-    if (isnan(old) || isnan(scale)) scale = __uint_as_float(0x7fffffffu);
-    else scale = fmaxf(scale, old);
-    const bool bad = isnan(scale);
-    const float inv = bad ? 0.f : inv_pow2(scale);
-    char* blk_dst = dst + blk * bstr;
-    for (int r0 = t; r0 < end; r0 += rows_per_round) {
+    // the rows of this thread in the first round (a longer run names slots twice)
+    const int rows_per_round = nw * kRowsPerWarp;
+    const bool once = end - t <= rows_per_round;
+    const int row0 = t + wid * kRowsPerWarp + lane / kLanesPerRow, col = (lane % kLanesPerRow) * 16;
+    // where row i goes; -1: past the run, or its slot is named again later (its last token stays)
+    auto place_of = [&](int i) -> int {
+      if (i >= end) return -1;
+      const int64_t slot = __ldg(slots + i);
+      if (!rising)
+        for (int j = i + 1; j < end; ++j)
+          if (__ldg(slots + j) == slot) return -1;
+      return (int)slot & (bs - 1);
+    };
+    int place[kSteps];
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const int i = r0 + wid * kRowsPerWarp + s * kRowsPerStep + lane / kLanesPerRow;
-        if (i >= end) continue;
-        const int64_t slot = __ldg(slots + i);
-        if (!rising) {   // a slot named again later in the run: its last token stays
-          bool again = false;
-          for (int j = i + 1; j < end; ++j) again = again || __ldg(slots + j) == slot;
-          if (again) continue;
+    for (int s = 0; s < kSteps; ++s) place[s] = place_of(row0 + s * kRowsPerStep);
+#pragma unroll 1
+    for (int item = item0; item < item1; ++item) {
+      const int h = item >> 1;
+      const bool isv = item & 1;
+      const T* src = static_cast<const T*>(isv ? a.r.v : a.r.k) + h * (isv ? a.r.vhs : a.r.khs) + col;
+      const int64_t ts = isv ? a.r.vts : a.r.kts;
+      char* dst = static_cast<char*>(isv ? a.c.v : a.c.k) + blk * (isv ? a.c.v_block_stride : a.c.k_block_stride) +
+                  h * (isv ? a.c.v_head_stride : a.c.k_head_stride) + col;
+      const int64_t tstr = isv ? a.c.v_tok_stride : a.c.k_tok_stride;
+      float* at = (isv ? a.c.v_scale : a.c.k_scale) + (int64_t)blk * a.c.num_kv_heads + h;
+      const float old = anew ? 0.f : *at;
+      Row16<T> x[kSteps];
+      uint32_t top = 0;
+#pragma unroll 1
+      for (int r0 = row0; r0 - row0 < end - t; r0 += rows_per_round) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const int i = r0 + s * kRowsPerStep;
+          if (i < end) x[s].load(src + i * ts);
+          else x[s].clear();
         }
-        if (!once) x[s].load(src + i * ts + (lane % kLanesPerRow) * 16);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) top = x[s].amax(top);
+      }
+      top = __reduce_max_sync(0xffffffffu, Row16<T>::fp32_bits(top));
+      if (nw > 1 || !anew) {
+        uint32_t* all = s_max[item & 1];
+        if (lane == 0) all[wid] = top;
+        __syncthreads();   // s_new is whole, and every warp has read the item's old scale
+        for (int w = 0; w < nw; ++w) top = max(top, all[w]);
+      }
+      float scale = scale_for<kFmt>(top);
+      if (isnan(old) || isnan(scale)) scale = __uint_as_float(0x7fffffffu);
+      else scale = fmaxf(scale, old);
+      const bool bad = isnan(scale);
+      const float inv = bad ? 0.f : inv_pow2(scale);
+      auto put = [&](const Row16<T>& row, int o) {
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float4 f = x[s].get(e);
-          w[e] = bad ? 0u : encode4<kFmt>(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
+          const float4 f = row.get(e);
+          w[e] = encode4<kFmt>(f.x, f.y, f.z, f.w, inv);
         }
-        *reinterpret_cast<uint4*>(blk_dst + (slot & (bs - 1)) * tstr + (lane % kLanesPerRow) * 16) =
-            make_uint4(w[0], w[1], w[2], w[3]);
-      }
-    }
-    if (!anew && !bad && scale > old) {   // the tokens that stay, in the new scale
-      const float ratio = old * inv;
-#pragma unroll 1
-      for (int s = 0; s < kSteps; ++s) {
-        const int o = wid * kRowsPerWarp + s * kRowsPerStep + lane / kLanesPerRow;
-        if (o >= bs || (s_new[o >> 5] >> (o & 31) & 1u)) continue;
-        uint4* p = reinterpret_cast<uint4*>(blk_dst + o * tstr + (lane % kLanesPerRow) * 16);
-        const uint4 v = *p;
-        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        if (bad) w[0] = w[1] = w[2] = w[3] = 0;
+        *reinterpret_cast<uint4*>(dst + o * tstr) = make_uint4(w[0], w[1], w[2], w[3]);
+      };
+      if (once) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float f[4];
-          decode4<kFmt>(w[e], f);
-          w[e] = encode4<kFmt>(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
-        }
-        *p = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int s = 0; s < kSteps; ++s)
+          if (place[s] >= 0) put(x[s], place[s]);
+      } else {
+        for (int r0 = row0; r0 - row0 < end - t; r0 += rows_per_round)
+#pragma unroll 1
+          for (int s = 0; s < kSteps; ++s) {
+            const int i = r0 + s * kRowsPerStep, o = place_of(i);
+            if (o < 0) continue;
+            x[0].load(src + i * ts);
+            put(x[0], o);
+          }
       }
+      if (!anew && !bad && scale > old) {   // the tokens that stay, in the new scale
+        const float ratio = old * inv;
+#pragma unroll 1
+        for (int s = 0; s < kSteps; ++s) {
+          const int o = wid * kRowsPerWarp + s * kRowsPerStep + lane / kLanesPerRow;
+          if (s_new[o >> 5] >> (o & 31) & 1u) continue;
+          uint4* p = reinterpret_cast<uint4*>(dst + o * tstr);
+          const uint4 v = *p;
+          uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float f[4];
+            decode4<kFmt>(w[e], f);
+            w[e] = encode4<kFmt>(f[0], f[1], f[2], f[3], ratio);
+          }
+          *p = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      if (threadIdx.x == 0) *at = scale;
     }
-    if (threadIdx.x == 0) scales[sidx] = scale;
     t = end;
     __syncthreads();   // s_new and s_max are free for the next run
   }
@@ -336,9 +363,11 @@ static void write_launch(const WriteArgs& a, dim3 grid, int threads, cudaStream_
 cudaError_t launch_cache_write(const ckv_cache& c, const CacheRows& r, cudaStream_t st) {
   WriteArgs a;
   a.c = c; a.r = r; a.block_log2 = log2_of(c.block_size);
-  // a decode step has a run per token: one CTA each; a prompt's runs are whole blocks
+  // a decode step has a run per token: a CTA for each and each (head, K / V); a prompt's runs are
+  // whole blocks, and a CTA that writes 4 pairs finds its run once for all of them
   a.piece = r.tokens <= 1024 ? 1 : c.block_size;
-  const dim3 grid((r.tokens + a.piece - 1) / a.piece, c.num_kv_heads, 2);
+  a.items = r.tokens <= 1024 ? 1 : 4;
+  const dim3 grid((r.tokens + a.piece - 1) / a.piece, (2 * c.num_kv_heads + a.items - 1) / a.items);
   const int threads = c.block_size / kRowsPerWarp * 32;
   const bool e4 = c.format == CKV_CACHE_E4M3;
   switch (r.dtype) {

@@ -59,14 +59,11 @@ CKV_DEV Sum3 scan3(Sum3 v, Sum3* scratch, Sum3* total) {
   return {base.tok + x.tok - v.tok, base.back + x.back - v.back, base.need + x.need - v.need};
 }
 
-// p[i]; kL2: written by the launch before, read from L2.
-template <bool kL2> CKV_DEV int get(const int* p, int i) { return kL2 ? __ldcg(p + i) : p[i]; }
-
 // Last row in [lo, hi] whose prefix p[row] is <= x (p ascending, p[lo] <= x).
-template <bool kL2> CKV_DEV int row_of(const int* p, int lo, int hi, int x) {
+CKV_DEV int row_of(const int* p, int lo, int hi, int x) {
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (get<kL2>(p, mid) <= x) lo = mid;
+    if (p[mid] <= x) lo = mid;
     else hi = mid - 1;
   }
   return lo;
@@ -80,40 +77,39 @@ struct StepView {
   int count, have, taken;
 };
 
-// Stores of the threads gt of gn: blocks given back, table entries, slots and positions.  cu is in
-// shared memory; kL2: the rest of the view is the scan's, in global memory.
-template <bool kL2> CKV_DEV void fill_step(const ckv_table_step& s, const StepView& v, int gt, int gn) {
+// Stores of the threads gt of gn: blocks given back, table entries, slots and positions.
+CKV_DEV void fill_step(const ckv_table_step& s, const StepView& v, int gt, int gn) {
   const int R = s.requests, lane = threadIdx.x & 31;
   const uint32_t b = s.block_size;
   // the j-th block from the bottom of the stack, after the blocks given back went on top
   auto stack = [&](int j) -> int {
     if (j < v.count) return __ldcg(s.free_list + j);
-    const int e = j - v.count, r = row_of<kL2>(v.back, 0, R - 1, e);
-    return __ldcg(s.tables + r * s.table_stride + (e - get<kL2>(v.back, r)));
+    const int e = j - v.count, r = row_of(v.back, 0, R - 1, e);
+    return __ldcg(s.tables + r * s.table_stride + (e - v.back[r]));
   };
   for (int i = gt; i < v.have - v.count; i += gn) s.free_list[v.count + i] = stack(v.count + i);
   for (int i = gt; i < v.taken; i += gn) {
-    const int r = row_of<kL2>(v.fresh, 0, R - 1, i);
-    s.tables[r * s.table_stride + ((uint32_t)get<kL2>(v.len, r) + b - 1) / b + (i - get<kL2>(v.fresh, r))] = stack(v.have - 1 - i);
+    const int r = row_of(v.fresh, 0, R - 1, i);
+    s.tables[r * s.table_stride + ((uint32_t)v.len[r] + b - 1) / b + (i - v.fresh[r])] = stack(v.have - 1 - i);
   }
   // tokens: a warp takes 128 at a time, its rows bracketed by two searches
   const int asked = v.cu[R], warp = gt >> 5, warps = gn >> 5;
   for (int t0 = warp * 128; t0 < s.total; t0 += warps * 128) {
-    const int first = row_of<false>(v.cu, 0, R - 1, min(t0, max(asked - 1, 0)));
-    const int last = row_of<false>(v.cu, first, R - 1, min(t0 + 127, max(asked - 1, 0)));
+    const int first = row_of(v.cu, 0, R - 1, min(t0, max(asked - 1, 0)));
+    const int last = row_of(v.cu, first, R - 1, min(t0 + 127, max(asked - 1, 0)));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = t0 + i * 32 + lane;
       if (t >= s.total) break;
       long long slot = -1, where = 0;
       if (t < asked) {
-        const int r = row_of<false>(v.cu, first, last, t);
-        const uint32_t n = get<kL2>(v.len, r), pos = n + (uint32_t)(t - v.cu[r]);
+        const int r = row_of(v.cu, first, last, t);
+        const uint32_t n = v.len[r], pos = n + (uint32_t)(t - v.cu[r]);
         where = (long long)pos + (s.shift ? s.shift[r] : 0);
-        if (get<kL2>(v.give, r) > 0) {
+        if (v.give[r] > 0) {
           const uint32_t bi = pos / b, held = (n + b - 1) / b;
           const int block = bi < held ? __ldcg(s.tables + r * s.table_stride + bi)
-                                      : stack(v.have - 1 - (get<kL2>(v.fresh, r) + (int)(bi - held)));
+                                      : stack(v.have - 1 - (v.fresh[r] + (int)(bi - held)));
           slot = (long long)block * b + (pos - bi * b);
         }
       }
@@ -191,30 +187,27 @@ __global__ void __launch_bounds__(kTabThreads) k_block_tables(const ckv_table_st
     s.out_free_count[0] = have - taken;
   }
   if (solo) {
-    fill_step<false>(s, StepView{cu, back, fresh, len, give, count, have, taken}, tid, blockDim.x);
+    fill_step(s, StepView{cu, back, fresh, len, give, count, have, taken}, tid, blockDim.x);
     return;
   }
-  int* w = s.work;                // [3 * (R + 1)]: back, fresh, old length, then count, have, taken
-  for (int r = tid; r <= R; r += blockDim.x) {
-    w[r] = back[r];
-    w[R + 1 + r] = fresh[r];
-    if (r < R) w[2 * (R + 1) + r] = len[r];
-  }
-  if (tid == 0) { w[3 * (R + 1)] = count; w[3 * (R + 1) + 1] = have; w[3 * (R + 1) + 2] = taken; }
+  int* w = s.work;                // the shared arrays, then count, have, taken
+  for (int i = tid; i < 5 * R + 3; i += blockDim.x) w[i] = tab_smem[i];
+  if (tid < 3) w[5 * R + 3 + tid] = tid == 0 ? count : tid == 1 ? have : taken;
 }
 
-constexpr int kFillThreads = 512;
+constexpr int kFillThreads = 1024;
 
 __global__ void __launch_bounds__(kFillThreads) k_block_tables_fill(const ckv_table_step s) {
-  extern __shared__ int tab_smem[];   // [R + 1] cu: searched most
+  extern __shared__ int tab_smem[];   // the scan's arrays: they are searched over and over
   const int R = s.requests;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int r = threadIdx.x; r <= R; r += kFillThreads) tab_smem[r] = __ldcg(s.out_cu + r);
-  const int* w = s.work;
-  const int count = __ldcg(w + 3 * (R + 1)), have = __ldcg(w + 3 * (R + 1) + 1), taken = __ldcg(w + 3 * (R + 1) + 2);
+  const int* w = s.work + 5 * R + 3;
+  const int count = __ldcg(w), have = __ldcg(w + 1), taken = __ldcg(w + 2);
+  for (int i = threadIdx.x; i < 5 * R + 3; i += kFillThreads) tab_smem[i] = __ldcg(s.work + i);
   __syncthreads();
-  fill_step<true>(s, StepView{tab_smem, w, w + R + 1, w + 2 * (R + 1), s.out_granted, count, have, taken},
-            blockIdx.x * kFillThreads + threadIdx.x, gridDim.x * kFillThreads);
+  const int *cu = tab_smem, *back = cu + R + 1, *fresh = back + R + 1, *len = fresh + R + 1;
+  fill_step(s, StepView{cu, back, fresh, len, len + R, count, have, taken}, blockIdx.x * kFillThreads + threadIdx.x,
+            gridDim.x * kFillThreads);
 }
 
 constexpr int kOneCta = 4096;   // tokens and requests up to which one CTA makes the step
@@ -225,11 +218,12 @@ cudaError_t launch_block_tables(const ckv_table_step& s, cudaStream_t st) {
   const bool solo = (int64_t)s.total + s.requests <= kOneCta;
   k_block_tables<<<1, kTabThreads, smem, st>>>(s, solo ? 1 : 0);
   if (cudaError_t e = cudaGetLastError(); solo || e != cudaSuccess) return e;
+  if (cudaError_t e = ensure_dynamic_smem((const void*)k_block_tables_fill, smem); e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(2 * 148);
+  cfg.gridDim = dim3(148);
   cfg.blockDim = dim3(kFillThreads);
-  cfg.dynamicSmemBytes = (size_t)(s.requests + 1) * sizeof(int);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
