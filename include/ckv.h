@@ -431,7 +431,7 @@ typedef struct ckv_table_step {
   int64_t* out_slots;
   int64_t* out_positions;
   int32_t* out_granted;
-  int32_t* work;               /* [5 * requests + 6], scratch */
+  int32_t* work;               /* [3 * requests + 4], scratch */
 } ckv_table_step;
 int ckv_block_tables(const ckv_table_step* step, ckv_stream_t stream);
 

@@ -80,17 +80,21 @@ template <> struct Row16<float> {
     for (int i = 0; i < 4; ++i) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   CKV_DEV float4 get(int i) const { return x[i]; }
-  CKV_DEV uint32_t amax(uint32_t top) const {   // magnitudes are ordered as their bits, NaN above infinity
+  CKV_DEV uint32_t amax(uint32_t top) const {   // a NaN stays
+    float m = __uint_as_float(top);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      top = max(top, __float_as_uint(x[i].x) & 0x7fffffffu);
-      top = max(top, __float_as_uint(x[i].y) & 0x7fffffffu);
-      top = max(top, __float_as_uint(x[i].z) & 0x7fffffffu);
-      top = max(top, __float_as_uint(x[i].w) & 0x7fffffffu);
+      m = max3_abs(m, x[i].x, x[i].y);
+      m = max3_abs(m, x[i].z, x[i].w);
     }
-    return top;
+    return __float_as_uint(m);
   }
-  static CKV_DEV uint32_t fp32_bits(uint32_t top) { return top; }
+  static CKV_DEV float max3_abs(float a, float b, float c) {
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+  }
+  static CKV_DEV uint32_t fp32_bits(uint32_t top) { return top & 0x7fffffffu; }
 };
 template <typename H> struct Row16 {
   uint32_t w[8];
@@ -107,14 +111,17 @@ template <typename H> struct Row16 {
     const float2 a = f2(w[2 * i]), b = f2(w[2 * i + 1]);
     return make_float4(a.x, a.y, b.x, b.y);
   }
-  CKV_DEV uint32_t amax(uint32_t top) const {   // of both halves of the words
+  CKV_DEV uint32_t amax(uint32_t top) const {   // of both halves of the words, of any sign; a NaN stays
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (std::is_same<H, __half>::value) asm("max.NaN.xorsign.abs.f16x2 %0, %0, %1;" : "+r"(top) : "r"(w[i]));
+      else asm("max.NaN.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(w[i]));
+    }
     return top;
   }
-  static CKV_DEV uint32_t fp32_bits(uint32_t top) {
-    const uint32_t m = max(top & 0xffffu, top >> 16);
-    return __float_as_uint(f2(m).x);
+  static CKV_DEV uint32_t fp32_bits(uint32_t top) {   // ordered as the magnitudes, a NaN on top
+    const float2 m = f2(top & 0x7fff7fffu);
+    return max(__float_as_uint(m.x), __float_as_uint(m.y));
   }
   static CKV_DEV float2 f2(uint32_t v) {
     if constexpr (sizeof(H) == 2 && std::is_same<H, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
@@ -150,42 +157,61 @@ struct WriteArgs {
   int items;       // of the 2 * heads (head, K / V) pairs, how many a CTA writes
 };
 
+constexpr int kSlotWindow = 2 * kCacheMaxBlock + 2;
+
 // grid (pieces, 2 * heads / items); block_size / 16 warps.
 template <typename T, int kFmt, int D>
 __global__ void __launch_bounds__(kCacheMaxBlock / kRowsPerWarp * 32) k_cache_write(const WriteArgs a) {
   constexpr int kLanesPerRow = D / 16, kRowsPerStep = 32 / kLanesPerRow, kSteps = kRowsPerWarp / kRowsPerStep;
   __shared__ uint32_t s_max[2][kCacheMaxBlock / kRowsPerWarp];   // of this item and the next
   __shared__ uint32_t s_new[kCacheMaxBlock / 32];                // places of the block that this run writes
+  __shared__ int s_slot[2][kSlotWindow];                          // block (-1: none) and place of the tokens from T0 - 1 on
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
   const int bs = a.c.block_size, T0 = blockIdx.x * a.piece, T1 = min(a.r.tokens, T0 + a.piece);
   const int item0 = blockIdx.y * a.items, item1 = min(2 * a.c.num_kv_heads, item0 + a.items);
   const int64_t pool = (int64_t)a.c.num_blocks << a.block_log2;
   const int64_t* slots = a.r.slots;
-  auto block_of = [&](int t) -> int {
-    const int64_t s = __ldg(slots + t);
-    return s >= 0 && s < pool ? (int)(s >> a.block_log2) : -1;
+  auto decode = [&](int i, int& blk, int& place) {
+    const int64_t s = i >= 0 && i < a.r.tokens ? __ldg(slots + i) : -1;
+    blk = s >= 0 && s < pool ? (int)(s >> a.block_log2) : -1;
+    place = (int)s & (bs - 1);
+  };
+  // the piece's slots and those that a run may reach, in one reading
+  const int window = T1 - T0 + bs + 2;
+  for (int j = threadIdx.x; j < window; j += blockDim.x) decode(T0 - 1 + j, s_slot[0][j], s_slot[1][j]);
+  __syncthreads();
+  auto block_of = [&](int i) -> int {
+    if (i - T0 + 1 < window) return s_slot[0][i - T0 + 1];
+    int blk, place;
+    decode(i, blk, place);
+    return blk;
+  };
+  auto place_at = [&](int i) -> int {
+    if (i - T0 + 1 < window) return s_slot[1][i - T0 + 1];
+    int blk, place;
+    decode(i, blk, place);
+    return place;
   };
   int t = T0;
   while (t < T1) {   // every warp takes the same path
     // the next token that begins a run: its block is not the token's before it
     const int cand = t + lane;
     const int mine = cand < T1 ? block_of(cand) : -1;
-    const uint32_t begins = __ballot_sync(0xffffffffu, mine >= 0 && (cand == 0 || block_of(cand - 1) != mine));
+    const uint32_t begins = __ballot_sync(0xffffffffu, mine >= 0 && block_of(cand - 1) != mine);
     if (begins == 0) { t += 32; continue; }
     t += __ffs(begins) - 1;
     const int blk = __shfl_sync(0xffffffffu, mine, __ffs(begins) - 1);
-    // the run's end, and whether it has the block's first token and rising slots
+    // the run's end, and whether it has the block's first token and rising places
     int end = t;
     bool rising = true, anew = false;
     for (bool more = true; more;) {
       const int i = end + lane;
-      const int64_t s = i < a.r.tokens ? __ldg(slots + i) : -1;
-      const bool in = s >= 0 && s < pool && (int)(s >> a.block_log2) == blk;
-      const uint32_t m = __ballot_sync(0xffffffffu, in);
+      const uint32_t m = __ballot_sync(0xffffffffu, block_of(i) == blk);
       const int n = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
       const bool own = lane < n;
-      rising = rising && __all_sync(0xffffffffu, !own || i == t || __ldg(slots + i - 1) < s);
-      anew = anew || __any_sync(0xffffffffu, own && ((int)s & (bs - 1)) == 0);
+      const int place = own ? place_at(i) : -1;
+      rising = rising && __all_sync(0xffffffffu, !own || i == t || place_at(i - 1) < place);
+      anew = anew || __any_sync(0xffffffffu, place == 0);
       end += n;
       more = n == 32;
     }
@@ -193,7 +219,7 @@ __global__ void __launch_bounds__(kCacheMaxBlock / kRowsPerWarp * 32) k_cache_wr
       if (threadIdx.x < kCacheMaxBlock / 32) s_new[threadIdx.x] = 0;
       __syncthreads();
       for (int i = t + threadIdx.x; i < end; i += blockDim.x) {
-        const int o = (int)__ldg(slots + i) & (bs - 1);
+        const int o = place_at(i);
         atomicOr(&s_new[o >> 5], 1u << (o & 31));
       }
     }
@@ -204,11 +230,11 @@ __global__ void __launch_bounds__(kCacheMaxBlock / kRowsPerWarp * 32) k_cache_wr
     // where row i goes; -1: past the run, or its slot is named again later (its last token stays)
     auto place_of = [&](int i) -> int {
       if (i >= end) return -1;
-      const int64_t slot = __ldg(slots + i);
+      const int o = place_at(i);
       if (!rising)
         for (int j = i + 1; j < end; ++j)
-          if (__ldg(slots + j) == slot) return -1;
-      return (int)slot & (bs - 1);
+          if (place_at(j) == o) return -1;
+      return o;
     };
     int place[kSteps];
 #pragma unroll
@@ -363,11 +389,13 @@ static void write_launch(const WriteArgs& a, dim3 grid, int threads, cudaStream_
 cudaError_t launch_cache_write(const ckv_cache& c, const CacheRows& r, cudaStream_t st) {
   WriteArgs a;
   a.c = c; a.r = r; a.block_log2 = log2_of(c.block_size);
-  // a decode step has a run per token: a CTA for each and each (head, K / V); a prompt's runs are
-  // whole blocks, and a CTA that writes 4 pairs finds its run once for all of them
+  // a decode step has a run per token: a CTA for each and each (head, K / V).  A prompt's runs are
+  // whole blocks; a CTA that writes more pairs finds its run once for all of them, but fewer CTAs
+  // hide less latency (131072 tokens of 8 heads: 2 pairs 137 us, 4 pairs 132; 33,000 tokens: 37, 39)
   a.piece = r.tokens <= 1024 ? 1 : c.block_size;
-  a.items = r.tokens <= 1024 ? 1 : 4;
-  const dim3 grid((r.tokens + a.piece - 1) / a.piece, (2 * c.num_kv_heads + a.items - 1) / a.items);
+  const int pieces = (r.tokens + a.piece - 1) / a.piece, pairs = 2 * c.num_kv_heads;
+  a.items = r.tokens <= 1024 ? 1 : (int64_t)pieces * pairs / 4 >= 148 * 32 ? 4 : 2;
+  const dim3 grid(pieces, (pairs + a.items - 1) / a.items);
   const int threads = c.block_size / kRowsPerWarp * 32;
   const bool e4 = c.format == CKV_CACHE_E4M3;
   switch (r.dtype) {

@@ -11,9 +11,13 @@
 // sums, independently of all others (a block that is given back and taken in the same step is
 // looked up where it was given back, not where it is put down).
 //
-// Bound: latency.  A small step is one CTA: scan, then stores.  Above kOneCta tokens and
-// requests the stores go to a second launch over the whole GPU (one CTA's search and stores of
-// 630,000 tokens took 126 us on a cluster of 8 CTAs; in two launches the step takes 9).
+// Bound: latency.  A small step is one CTA: scan, then stores, each token's request found by
+// binary search in shared memory.  Above kOneCta tokens and requests the stores go to a second
+// launch with CTAs for each request, which need no search but for blocks that came back in the
+// same step (1024 requests, 630,000 tokens: 126 us when a cluster of 8 CTAs searched for every
+// token, 17 us in two launches that did, 14 with CTAs by request).
+#include <algorithm>
+
 #include "ckv_cache.h"
 #include "ckv_common.cuh"
 
@@ -79,7 +83,7 @@ struct StepView {
 
 // Stores of the threads gt of gn: blocks given back, table entries, slots and positions.
 CKV_DEV void fill_step(const ckv_table_step& s, const StepView& v, int gt, int gn) {
-  const int R = s.requests, lane = threadIdx.x & 31;
+  const int R = s.requests;
   const uint32_t b = s.block_size;
   // the j-th block from the bottom of the stack, after the blocks given back went on top
   auto stack = [&](int j) -> int {
@@ -92,30 +96,22 @@ CKV_DEV void fill_step(const ckv_table_step& s, const StepView& v, int gt, int g
     const int r = row_of(v.fresh, 0, R - 1, i);
     s.tables[r * s.table_stride + ((uint32_t)v.len[r] + b - 1) / b + (i - v.fresh[r])] = stack(v.have - 1 - i);
   }
-  // tokens: a warp takes 128 at a time, its rows bracketed by two searches
-  const int asked = v.cu[R], warp = gt >> 5, warps = gn >> 5;
-  for (int t0 = warp * 128; t0 < s.total; t0 += warps * 128) {
-    const int first = row_of(v.cu, 0, R - 1, min(t0, max(asked - 1, 0)));
-    const int last = row_of(v.cu, first, R - 1, min(t0 + 127, max(asked - 1, 0)));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = t0 + i * 32 + lane;
-      if (t >= s.total) break;
-      long long slot = -1, where = 0;
-      if (t < asked) {
-        const int r = row_of(v.cu, first, last, t);
-        const uint32_t n = v.len[r], pos = n + (uint32_t)(t - v.cu[r]);
-        where = (long long)pos + (s.shift ? s.shift[r] : 0);
-        if (v.give[r] > 0) {
-          const uint32_t bi = pos / b, held = (n + b - 1) / b;
-          const int block = bi < held ? __ldcg(s.tables + r * s.table_stride + bi)
-                                      : stack(v.have - 1 - (v.fresh[r] + (int)(bi - held)));
-          slot = (long long)block * b + (pos - bi * b);
-        }
+  const int asked = v.cu[R];
+  for (int t = gt; t < s.total; t += gn) {
+    long long slot = -1, where = 0;
+    if (t < asked) {
+      const int r = row_of(v.cu, 0, R - 1, t);
+      const uint32_t n = v.len[r], pos = n + (uint32_t)(t - v.cu[r]);
+      where = (long long)pos + (s.shift ? s.shift[r] : 0);
+      if (v.give[r] > 0) {
+        const uint32_t bi = pos / b, held = (n + b - 1) / b;
+        const int block = bi < held ? __ldcg(s.tables + r * s.table_stride + bi)
+                                    : stack(v.have - 1 - (v.fresh[r] + (int)(bi - held)));
+        slot = (long long)block * b + (pos - bi * b);
       }
-      s.out_slots[t] = slot;
-      s.out_positions[t] = where;
     }
+    s.out_slots[t] = slot;
+    s.out_positions[t] = where;
   }
 }
 
@@ -190,24 +186,108 @@ __global__ void __launch_bounds__(kTabThreads) k_block_tables(const ckv_table_st
     fill_step(s, StepView{cu, back, fresh, len, give, count, have, taken}, tid, blockDim.x);
     return;
   }
-  int* w = s.work;                // the shared arrays, then count, have, taken
-  for (int i = tid; i < 5 * R + 3; i += blockDim.x) w[i] = tab_smem[i];
-  if (tid < 3) w[5 * R + 3 + tid] = tid == 0 ? count : tid == 1 ? have : taken;
+  int* w = s.work;                // [3 R + 4]: back, fresh, old length, count, have
+  for (int i = tid; i <= R; i += blockDim.x) {
+    w[i] = back[i];
+    w[R + 1 + i] = fresh[i];
+    if (i < R) w[2 * (R + 1) + i] = len[i];
+  }
+  if (tid < 2) w[3 * R + 2 + tid] = tid == 0 ? count : have;
 }
 
-constexpr int kFillThreads = 1024;
+// The stores of a large step: CTA (r, part) has a part of request r's tokens, CTA (R, part) of
+// the rows past the last request's.
+constexpr int kFillThreads = 128, kFillBlocks = 512;
+
+// Last row whose prefix p[row] is <= x, by one warp, 32 probes at a time; p in L2.
+CKV_DEV int warp_row_of(const int* p, int rows, int x) {
+  int lo = 0, n = rows;
+  while (n > 1) {
+    const int step = (n + 31) / 32, i = (threadIdx.x & 31) * step;
+    const uint32_t m = __ballot_sync(0xffffffffu, i < n && __ldcg(p + lo + min(i, n - 1)) <= x);
+    const int hit = m ? 31 - __clz(m) : 0;
+    lo += hit * step;
+    n = min(step, n - hit * step);
+  }
+  return lo;
+}
 
 __global__ void __launch_bounds__(kFillThreads) k_block_tables_fill(const ckv_table_step s) {
-  extern __shared__ int tab_smem[];   // the scan's arrays: they are searched over and over
-  const int R = s.requests;
+  __shared__ int s_id[kFillBlocks];
+  const int R = s.requests, r = blockIdx.x, part = blockIdx.y, parts = gridDim.y, tid = threadIdx.x;
+  const uint32_t b = s.block_size;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int* w = s.work + 5 * R + 3;
-  const int count = __ldcg(w), have = __ldcg(w + 1), taken = __ldcg(w + 2);
-  for (int i = threadIdx.x; i < 5 * R + 3; i += kFillThreads) tab_smem[i] = __ldcg(s.work + i);
-  __syncthreads();
-  const int *cu = tab_smem, *back = cu + R + 1, *fresh = back + R + 1, *len = fresh + R + 1;
-  fill_step(s, StepView{cu, back, fresh, len, len + R, count, have, taken}, blockIdx.x * kFillThreads + threadIdx.x,
-            gridDim.x * kFillThreads);
+  const int *back = s.work, *fresh = back + R + 1, *len = fresh + R + 1, *tail = len + R;
+  if (r == R) {   // no request's tokens
+    for (int64_t t = (int64_t)__ldcg(s.out_cu + R) + part * kFillThreads + tid; t < s.total; t += parts * kFillThreads) {
+      s.out_slots[t] = -1;
+      s.out_positions[t] = 0;
+    }
+    return;
+  }
+  const int t0 = __ldcg(s.out_cu + r), ask = __ldcg(s.out_cu + r + 1) - t0, give = __ldcg(s.out_granted + r);
+  const int n = __ldcg(len + r), b0 = __ldcg(back + r), returned = __ldcg(back + r + 1) - b0, f0 = __ldcg(fresh + r);
+  const int count = __ldcg(tail), have = __ldcg(tail + 1);
+  const int shift = s.shift ? __ldg(s.shift + r) : 0;
+  int32_t* table = s.tables + r * s.table_stride;
+  for (int k = part * kFillThreads + tid; k < returned; k += parts * kFillThreads)
+    if (count + b0 + k < have) s.free_list[count + b0 + k] = table[k];
+  const int each = (ask + parts - 1) / parts, i0 = min((int64_t)part * each, (int64_t)ask), i1 = min((int64_t)i0 + each, (int64_t)ask);
+  if (i0 >= i1) return;
+  if (give == 0) {   // refused
+    for (int i = i0 + tid; i < i1; i += kFillThreads)
+      if (t0 + i < s.total) {
+        s.out_slots[t0 + i] = -1;
+        s.out_positions[t0 + i] = (long long)n + i + shift;
+      }
+    return;
+  }
+  // the blocks of these tokens, kFillBlocks at a time, then the tokens in them
+  const uint32_t held = ((uint32_t)n + b - 1) / b, first = ((uint32_t)n + i0) / b, last = ((uint32_t)n + i1 - 1) / b;
+  int row_lo = 0, row_hi = R - 1;   // the requests whose blocks came back and go to this one
+  if (last >= held) {
+    const int top = have - 1 - (f0 + (int)(max(first, held) - held)), low = have - 1 - (f0 + (int)(last - held));
+    if (top >= count) {
+      row_hi = warp_row_of(back, R, top - count);
+      row_lo = warp_row_of(back, R, max(low - count, 0));
+    }
+  }
+  for (uint32_t c = first; c <= last; c += kFillBlocks) {
+    const int blocks = (int)min(last - c + 1, (uint32_t)kFillBlocks);
+    __syncthreads();
+    for (int k = tid; k < blocks; k += kFillThreads) {
+      const uint32_t bi = c + k;
+      int id;
+      if (bi < held) {
+        id = table[bi];
+      } else {
+        const int j = have - 1 - (f0 + (int)(bi - held));   // from the bottom of the stack, what came back on top
+        if (j < count) {
+          id = __ldg(s.free_list + j);
+        } else {
+          int lo = row_lo, hi = row_hi;
+          while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (__ldcg(back + mid) <= j - count) lo = mid;
+            else hi = mid - 1;
+          }
+          id = __ldg(s.tables + lo * s.table_stride + (j - count - __ldcg(back + lo)));
+        }
+        const int64_t at = (int64_t)bi * b - n;             // the block's first token: its part writes the entry
+        if (at >= i0 && at < i1) table[bi] = id;
+      }
+      s_id[k] = id;
+    }
+    __syncthreads();
+    const int64_t from = max((int64_t)i0, (int64_t)c * b - n), to = min((int64_t)i1, (int64_t)(c + blocks) * b - n);
+    for (int i = (int)from + tid; i < to; i += kFillThreads) {
+      const uint32_t pos = (uint32_t)n + i, bi = pos / b;
+      if (t0 + i < s.total) {
+        s.out_slots[t0 + i] = (long long)s_id[bi - c] * b + (pos - bi * b);
+        s.out_positions[t0 + i] = (long long)pos + shift;
+      }
+    }
+  }
 }
 
 constexpr int kOneCta = 4096;   // tokens and requests up to which one CTA makes the step
@@ -218,12 +298,11 @@ cudaError_t launch_block_tables(const ckv_table_step& s, cudaStream_t st) {
   const bool solo = (int64_t)s.total + s.requests <= kOneCta;
   k_block_tables<<<1, kTabThreads, smem, st>>>(s, solo ? 1 : 0);
   if (cudaError_t e = cudaGetLastError(); solo || e != cudaSuccess) return e;
-  if (cudaError_t e = ensure_dynamic_smem((const void*)k_block_tables_fill, smem); e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(148);
+  const int parts = s.requests >= 592 ? 1 : std::min(592 / s.requests, 64);   // about four CTAs per SM
+  cfg.gridDim = dim3(s.requests + 1, parts);
   cfg.blockDim = dim3(kFillThreads);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -503,7 +503,7 @@ def block_tables(lens: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, fr
         _need(total >= 0, "total must not be negative")
         raise ValueError("tables must be an int32 tensor [requests, width] with contiguous rows")
     dev, width = lens.device, tables.shape[1]
-    small = torch.empty(6 * R + 7, dtype=i32, device=dev)   # cu, then scratch
+    small = torch.empty(4 * R + 5, dtype=i32, device=dev)   # cu, then scratch
     cu = small[:R + 1]
     granted = torch.empty(R, dtype=i32, device=dev)
     slots = torch.empty(total, dtype=torch.int64, device=dev)
