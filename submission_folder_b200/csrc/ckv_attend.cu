@@ -525,25 +525,35 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
           ve[u] = (float)((int)(bits >> 23 & 255u) - 127);
           if (mant) ve[u] = isnan(v) ? v : ve[u] + __log2f(__uint_as_float(mant | 0x3f800000u));   // not a power of two
         }
-        const bool masked = (s + 1) * kAttStep > see_min;
+        bool hide = false;   // a token that a row does not see stands in a block whose value scale is NaN
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const float f = qs[nt][r] * ks[u];
+              sc[nt][u][r] *= f;
+              sc[nt][u][2 + r] *= f;
+            }
+        if ((s + 1) * kAttStep > see_min) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (s * kAttStep + u * 16 + g + (e >> 1) * 8 >= see[nt][e & 1]) sc[nt][u][e] = -INFINITY;
+          hide = isnan(ve[0]) || isnan(ve[1]);
+        }
         bool past = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const float f = qs[nt][r] * ks[u];
-              sc[nt][u][r] *= f;
-              sc[nt][u][2 + r] *= f;
-              if (masked) {
-                const int tok = s * kAttStep + u * 16 + g;
-                if (tok >= see[nt][r]) sc[nt][u][r] = -INFINITY;
-                if (tok + 8 >= see[nt][r]) sc[nt][u][2 + r] = -INFINITY;
-              }
-              const float h = fmaxf(sc[nt][u][r], sc[nt][u][2 + r]);
-              past = past || h > m[nt][r] + kSlack || h + ve[u] > mw[nt][r] + kSlack;
-            }
+          for (int r = 0; r < 2; ++r) {
+            const float h0 = fmaxf(sc[nt][0][r], sc[nt][0][2 + r]), h1 = fmaxf(sc[nt][1][r], sc[nt][1][2 + r]);
+            past = past || fmaxf(h0, h1) > m[nt][r] + kSlack || fmaxf(h0 + ve[0], h1 + ve[1]) > mw[nt][r] + kSlack;
+          }
         if (__any_sync(0xffffffffu, past)) {
           // the rows that passed theirs get new references (whole numbers: the rescaling is exact),
           // the same in all lanes of a row and whatever the other rows do
@@ -579,7 +589,11 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
               const int r = e & 1;
               l[nt][r] += ex2(sc[nt][u][e] - m[nt][r]);
               w[e] = ex2(sc[nt][u][e] + (ve[u] - mw[nt][r] + kTop));
-              if (masked && sc[nt][u][e] == -INFINITY) w[e] = 0.f;   // whatever the scale
+            }
+            if (hide) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (sc[nt][u][e] == -INFINITY) w[e] = 0.f;
             }
             if constexpr (kTerms == 1) {
               pf[nt][0][u][0] = transpose8(half2_bits(w[0], w[1]));
