@@ -54,6 +54,7 @@ struct AttArgs {
   float* ws;                     // [ctas][kAttMaxWarps + 2] partial results
   int4* desc;                    // [ctas]: what k_attend_merge has to merge from this CTA on
   int block_log2, group, ctas;
+  int dense;                     // token rows are head_dim bytes apart
   float inv_group;
 };
 
@@ -336,6 +337,12 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
     return D == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
   };
   constexpr int kChunks = D / 16, kRows = 32 / kChunks;   // of one copy instruction
+  // from the place of row crow to that of row crow + i * kRows (kRows = 4 at D = 128: every second turns
+  // the chunk's third bit; 8 at D = 64: the swizzle is the same)
+  auto turn = [&](int i) -> uint32_t {
+    const uint32_t here = swz(lane / kChunks, lane % kChunks), there = swz(lane / kChunks + i * kRows, lane % kChunks);
+    return there - here;
+  };
   const int crow = lane / kChunks, cchunk = lane % kChunks;
   if (left > 0) {
     int n = seq_len(p, r), q0, nq;
@@ -359,45 +366,59 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
       int pbase = (s_begin * kAttStep) >> p.block_log2;
       auto page = [&](int i) { return i < pages ? __ldg(table + i) : 0; };
       int pcur = page(pbase + lane), pnext = page(pbase + 32 + lane);
+      // the 32 tokens of step s, as two halves of 16 that may stand in two blocks
       auto issue = [&](int s, int stage) {
-        {
-          const uint32_t st = ring_a + stage * kStageBytes;
+        const int tok0 = s * kAttStep, tok1 = tok0 + 16, last = (1 << p.block_log2) - 1;
+        if ((tok0 >> p.block_log2) - pbase >= 32) {   // pbase is even where a step has two pages
+          pbase += 32;
+          pcur = pnext;
+          pnext = page(pbase + 32 + lane);
+        }
+        const int blk0 = __shfl_sync(0xffffffffu, pcur, (tok0 >> p.block_log2) - pbase);
+        const int blk1 = __shfl_sync(0xffffffffu, pcur, (tok1 >> p.block_log2) - pbase);
+        const bool good0 = (uint32_t)blk0 < (uint32_t)p.c.num_blocks, good1 = (uint32_t)blk1 < (uint32_t)p.c.num_blocks;
+        const uint32_t st = ring_a + stage * kStageBytes + swz(crow, cchunk);
+        if (p.dense && good0 && good1 && tok0 + kAttStep <= n) {   // rows D bytes apart: constant offsets
+          const char* k0 = kh + (uint64_t)(uint32_t)blk0 * p.c.k_block_stride + (tok0 & last) * D;
+          const char* v0 = vh + (uint64_t)(uint32_t)blk0 * p.c.v_block_stride + (tok0 & last) * D;
+          const char* k1 = k0 + 16 * D;
+          const char* v1 = v0 + 16 * D;
+          if (p.block_log2 == 4) {
+            k1 = kh + (uint64_t)(uint32_t)blk1 * p.c.k_block_stride;
+            v1 = vh + (uint64_t)(uint32_t)blk1 * p.c.v_block_stride;
+          }
 #pragma unroll
+          for (int i = 0; i < 16 / kRows; ++i) {   // the swizzle repeats every 8 rows
+            const uint32_t d = st + turn(i);
+            cp16(d, k0 + i * kRows * D);
+            cp16(d + 16 * D, k1 + i * kRows * D);
+            cp16(d + kAttStep * D, v0 + i * kRows * D);
+            cp16(d + kAttStep * D + 16 * D, v1 + i * kRows * D);
+          }
+        } else {
+#pragma unroll 1
           for (int half = 0; half < 2; ++half) {
-            const int tok0 = s * kAttStep + half * 16, pi = tok0 >> p.block_log2;
-            if (pi - pbase >= 32) {
-              pbase += 32;
-              pcur = pnext;
-              pnext = page(pbase + 32 + lane);
-            }
-            const int blk = __shfl_sync(0xffffffffu, pcur, pi - pbase);
-            const bool good = (uint32_t)blk < (uint32_t)p.c.num_blocks;
-            const int64_t b = good ? blk : 0;
-            const int off = tok0 & ((1 << p.block_log2) - 1);
-            const int have = good ? n - tok0 : 0;   // rows of these 16 that hold tokens
-            const char* ks = kh + b * p.c.k_block_stride + off * p.c.k_tok_stride;
-            const char* vs = vh + b * p.c.v_block_stride + off * p.c.v_tok_stride;
-            if (have >= 16) {
+            const int tok = half ? tok1 : tok0;
+            const bool good = half ? good1 : good0;
+            const int64_t b = good ? (half ? blk1 : blk0) : 0;
+            const int have = good ? n - tok : 0;   // rows of these 16 that hold tokens
+            const char* ks = kh + b * p.c.k_block_stride + (tok & last) * p.c.k_tok_stride;
+            const char* vs = vh + b * p.c.v_block_stride + (tok & last) * p.c.v_tok_stride;
 #pragma unroll
-              for (int i = 0; i < 16 / kRows; ++i) {
-                const uint32_t d = st + swz(half * 16 + i * kRows + crow, cchunk);
-                cp16(d, ks + i * kRows * p.c.k_tok_stride);
-                cp16(d + kAttStep * D, vs + i * kRows * p.c.v_tok_stride);
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 16 / kRows; ++i) {
-                const uint32_t in = i * kRows + crow < have ? 16u : 0u;
-                const uint32_t d = st + swz(half * 16 + i * kRows + crow, cchunk);
-                cp16_or_zero(d, in ? ks + i * kRows * p.c.k_tok_stride : kh, in);
-                cp16_or_zero(d + kAttStep * D, in ? vs + i * kRows * p.c.v_tok_stride : vh, in);
-              }
-            }
-            if (lane < 2) {
-              if (have > 0) cp4(scale_a + (stage * 4 + half * 2 + lane) * 4, (lane ? p.c.v_scale : p.c.k_scale) + b * p.c.num_kv_heads + head);
-              else s_scale[wid][stage][half * 2 + lane] = tok0 < n ? __uint_as_float(0x7fffffffu) : 0.f;   // a bad page reads as NaN
+            for (int i = 0; i < 16 / kRows; ++i) {
+              const uint32_t in = i * kRows + crow < have ? 16u : 0u;
+              const uint32_t d = st + turn(i) + half * 16 * D;
+              cp16_or_zero(d, in ? ks + i * kRows * p.c.k_tok_stride : kh, in);
+              cp16_or_zero(d + kAttStep * D, in ? vs + i * kRows * p.c.v_tok_stride : vh, in);
             }
           }
+        }
+        if (lane < 4) {   // scales: K, V of each half; a bad page reads as NaN
+          const int blk = lane < 2 ? blk0 : blk1;
+          const float* from = (lane & 1 ? p.c.v_scale : p.c.k_scale) + (int64_t)blk * p.c.num_kv_heads + head;
+          if ((lane < 2 ? tok0 : tok1) >= n) s_scale[wid][stage][lane] = 0.f;
+          else if (lane < 2 ? good0 : good1) cp4(scale_a + (stage * 4 + lane) * 4, from);
+          else s_scale[wid][stage][lane] = __uint_as_float(0x7fffffffu);
         }
       };
 
@@ -825,6 +846,7 @@ cudaError_t launch_cache_attention(const ckv_cache& c, const ckv_attention_args&
   p.group = a.q_heads / c.num_kv_heads;
   p.ctas = kAttMaxCtas;
   p.inv_group = 1.f / p.group;
+  p.dense = c.k_tok_stride == c.head_dim && c.v_tok_stride == c.head_dim;
   const int rows = a.max_q * p.group;
   const bool e4 = c.format == CKV_CACHE_E4M3;
   if (c.head_dim == 64)
