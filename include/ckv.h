@@ -431,8 +431,10 @@ typedef struct ckv_table_step {
   int64_t* out_slots;
   int64_t* out_positions;
   int32_t* out_granted;
-  int32_t* work;               /* [3 * requests + 4], scratch */
+  int32_t* work;               /* [3 * requests + 4], scratch; may be NULL when requests + total is at
+                                  most CKV_TABLES_SMALL */
 } ckv_table_step;
+enum { CKV_TABLES_SMALL = 4096 };
 int ckv_block_tables(const ckv_table_step* step, ckv_stream_t stream);
 
 /* Rotary positions of queries and keys: pair i of a head turns by positions[t] * inv_freq[i]

@@ -7,8 +7,8 @@ no fallback: if the library or a CUDA device is missing, the calls raise.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
-import struct
 from typing import Optional
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -149,15 +149,6 @@ class AttentionArgs(ctypes.Structure):
     ]
 
 
-_STRUCT_CODES = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f"}
-
-
-def packer(kind):
-    """``pack(*fields)`` of a structure above to bytes, its C layout (pointers as integers, 0 for
-    NULL): the same as ``kind(*fields)``, in a fifth of the time."""
-    return struct.Struct("@" + "".join(_STRUCT_CODES[t] for _, t in kind._fields_) + "0q").pack
-
-
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -208,13 +199,12 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         "ckv_gather": (i32, [L, i32, vp, i32, i32, vp, vp, vp]),
         "ckv_device_accessible": (i32, [vp, ctypes.POINTER(i32)]),
         "ckv_copy_rows": (i32, [vp, sz, vp, sz, sz, i32, vp]),
-        # structures of the paged cache's calls: byref(...) or the bytes of packer()
-        "ckv_block_tables": (i32, [vp, vp]),
-        "ckv_rotary": (i32, [vp, vp]),
-        "ckv_cache_write": (i32, [vp, vp, i64, i64, vp, i64, i64, i32, vp, i32, vp]),
-        "ckv_cache_read": (i32, [vp, vp, vp, i32, vp, i32, vp]),
+        "ckv_block_tables": (i32, [ctypes.POINTER(TableStep), vp]),
+        "ckv_rotary": (i32, [ctypes.POINTER(RotaryArgs), vp]),
+        "ckv_cache_write": (i32, [ctypes.POINTER(Cache), vp, i64, i64, vp, i64, i64, i32, vp, i32, vp]),
+        "ckv_cache_read": (i32, [ctypes.POINTER(Cache), vp, vp, i32, vp, i32, vp]),
         "ckv_cache_attention_workspace": (i32, [i32, i32, i32, i32, ctypes.POINTER(sz)]),
-        "ckv_cache_attention": (i32, [vp, vp, vp, sz, vp]),
+        "ckv_cache_attention": (i32, [ctypes.POINTER(Cache), ctypes.POINTER(AttentionArgs), vp, sz, vp]),
         "ckv_set_stage_events": (i32, [ctypes.POINTER(vp), i32]),
         "ckv_last_error_string": (ctypes.c_char_p, []),
         "ckv_version": (ctypes.c_char_p, []),
@@ -225,6 +215,26 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_torch_calls = None
+
+
+def torch_calls():
+    """The module of ``csrc/ckv_torch.cpp`` (the paged cache's calls on torch tensors), loaded once
+    from beside the library; raises if it is missing."""
+    global _torch_calls
+    if _torch_calls is None:
+        load()
+        path = os.path.join(os.path.dirname(LIB_PATH), "_ckv_torch.so")
+        if not os.path.exists(path):
+            raise ImportError(f"_ckv_torch.so not found at {path}; build it with `python -m submission_folder_b200.build`")
+        import torch  # noqa: F401  (its libraries are what the module links to)
+        spec = importlib.util.spec_from_file_location("_ckv_torch", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _torch_calls = module
+    return _torch_calls
 
 
 def check(status: int, what: str) -> None:

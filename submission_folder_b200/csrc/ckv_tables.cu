@@ -12,7 +12,7 @@
 // looked up where it was given back, not where it is put down).
 //
 // Bound: latency.  A small step is one CTA: scan, then stores, each token's request found by
-// binary search in shared memory.  Above kOneCta tokens and requests the stores go to a second
+// binary search in shared memory.  Above CKV_TABLES_SMALL tokens and requests the stores go to a second
 // launch with CTAs for each request, which need no search but for blocks that came back in the
 // same step (1024 requests, 630,000 tokens: 126 us when a cluster of 8 CTAs searched for every
 // token, 17 us in two launches that did, 14 with CTAs by request).
@@ -290,12 +290,10 @@ __global__ void __launch_bounds__(kFillThreads) k_block_tables_fill(const ckv_ta
   }
 }
 
-constexpr int kOneCta = 4096;   // tokens and requests up to which one CTA makes the step
-
 cudaError_t launch_block_tables(const ckv_table_step& s, cudaStream_t st) {
   const size_t smem = (size_t)(5 * s.requests + 3) * sizeof(int);
   if (cudaError_t e = ensure_dynamic_smem((const void*)k_block_tables, smem); e != cudaSuccess) return e;
-  const bool solo = (int64_t)s.total + s.requests <= kOneCta;
+  const bool solo = (int64_t)s.total + s.requests <= CKV_TABLES_SMALL;
   k_block_tables<<<1, kTabThreads, smem, st>>>(s, solo ? 1 : 0);
   if (cudaError_t e = cudaGetLastError(); solo || e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};

@@ -401,32 +401,17 @@ def gather(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, idx: 
 # ---------------------------------------------------------------------------
 # paged 8-bit decode cache: block tables, rotary positions, write / read, attention
 #
-# A decode step makes several of these calls per layer and its kernels take a few
-# microseconds, so the wrappers keep to few Python operations: arguments are checked in one
-# expression (a second function says what is wrong), structures are packed bytes, and the
-# stream is read as a plain integer.
+# The calls go through csrc/ckv_torch.cpp, which checks the arguments, allocates the outputs
+# and launches: a decode step makes several per layer and its kernels take a few microseconds.
+# Where it refuses an argument, the functions here say which one and why.
 # ---------------------------------------------------------------------------
-_CACHE_FORMATS = {torch.float8_e4m3fn: _lib.CACHE_E4M3, torch.int8: _lib.CACHE_INT8}
-_CODES = {dt: _lib.DTYPE_CODES[name] for dt, name in _DT.items()}
-_pack_cache, _pack_tables = _lib.packer(_lib.Cache), _lib.packer(_lib.TableStep)
-_pack_rotary, _pack_attention = _lib.packer(_lib.RotaryArgs), _lib.packer(_lib.AttentionArgs)
-
-
-def _call(name: str, index: int, *args) -> None:
-    """One library call on the current stream of device ``index``, with that device current."""
-    fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        check(rc, name)
+_CACHE_FORMATS = (torch.float8_e4m3fn, torch.int8)
 
 
 def _one_device(*ts: Optional[torch.Tensor]) -> None:
     """Raises unless all the tensors are on one CUDA device."""
     ts = [t for t in ts if t is not None]
+    _need(all(isinstance(t, torch.Tensor) for t in ts), "expected tensors", TypeError)
     _require_cuda(*ts)
     for t in ts:
         if t.device != ts[0].device:
@@ -445,12 +430,39 @@ def _need_vector(t: torch.Tensor, dtype: torch.dtype, n: int, what: str) -> None
 
 def _need_rows(t: torch.Tensor, what: str) -> None:
     _need(t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1), f"{what} must be [tokens, heads, head_dim] with contiguous head_dim")
-    _need(t.dtype in _CODES, f"{what} must be bf16, fp16 or fp32, got {t.dtype}", TypeError)
+    _need(t.dtype in _DT, f"{what} must be bf16, fp16 or fp32, got {t.dtype}", TypeError)
+    _need(not (t.requires_grad and torch.is_grad_enabled()), f"{what} requires grad, but the paged cache's calls record no "
+          "autograd graph; call them on detached tensors", RuntimeError)
 
 
-def _need_no_grad(what: str, *ts: Optional[torch.Tensor]) -> None:
-    _need(not any(t is not None and t.requires_grad for t in ts), f"{what} records no autograd graph; call it on detached tensors",
-          RuntimeError)
+def _need_tables(t: torch.Tensor, requests: int) -> None:
+    _need(t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] == requests and t.stride(1) == 1,
+          f"tables must be an int32 tensor [{requests}, width] with contiguous rows")
+
+
+def _need_out(out: Optional[torch.Tensor], like: Optional[torch.Tensor], what: str) -> None:
+    _need((out is None) == (like is None) and (out is None or (out.shape == like.shape and out.dtype == like.dtype)),
+          f"{what} must be like its input")
+    if out is not None:
+        _need_rows(out, what)
+
+
+def _need_cache(k_cache, v_cache, k_scale, v_scale) -> Tuple[int, int]:
+    _need(k_cache.dtype in _CACHE_FORMATS and v_cache.dtype == k_cache.dtype,
+          "k_cache and v_cache must both be float8_e4m3fn or int8", TypeError)
+    _need(k_cache.dim() == 4 and v_cache.shape == k_cache.shape and k_cache.stride(3) == 1 and v_cache.stride(3) == 1,
+          "k_cache and v_cache must be [blocks, kv_heads, block_size, head_dim] with contiguous head_dim")
+    for s in (k_scale, v_scale):
+        _need(s.dtype == torch.float32 and s.shape == k_cache.shape[:2] and s.is_contiguous(),
+              f"scales must be contiguous float32 tensors of shape {tuple(k_cache.shape[:2])}")
+    return k_cache.shape[1], k_cache.shape[3]
+
+
+def _failed(name: str, rc) -> None:
+    """Raises for what ckv_torch.cpp returned in place of a result."""
+    if type(rc) is int:
+        check(rc, name)
+    raise ValueError(f"{name}: arguments out of range")
 
 
 class TableStep(NamedTuple):
@@ -478,42 +490,22 @@ def block_tables(lens: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, fr
     sum get slot -1.  ``shift`` int32 ``[R]`` is added to the positions (the number of tokens
     evicted from the request).  A request that does not fit gets slots of -1 and ``granted`` 0.
     """
-    if lens_out is None:
-        lens_out = lens
-    if free_count_out is None:
-        free_count_out = free_count
-    i32 = torch.int32
-    index, R = lens.get_device(), lens.shape[0] if lens.dim() == 1 else 0
-    ts = (lens, new, tables, free_list, free_count, lens_out, free_count_out)
-    good = index >= 0 and total >= 0 and tables.dim() == 2
-    for t in ts:
-        good = good and t.get_device() == index and t.dtype is i32 and (t is tables or (t.dim() == 1 and t.is_contiguous()))
-    if shift is not None:
-        good = good and shift.get_device() == index and shift.dtype is i32 and shift.dim() == 1 and shift.is_contiguous() \
-            and shift.shape[0] == R
-    if not (good and new.shape[0] == R and lens_out.shape[0] == R and tables.shape[0] == R and tables.stride(1) == 1
-            and free_count.shape[0] == 1 and free_count_out.shape[0] == 1):
-        _one_device(*ts, shift)
+    r = _lib.torch_calls().block_tables(lens, new, tables, free_list, free_count, block_size, total, shift, lens_out,
+                                        free_count_out)
+    if type(r) is tuple:
+        return TableStep._make(r)
+    if r is None:
+        _one_device(lens, new, tables, free_list, free_count, shift, lens_out, free_count_out)
         _need(lens.dim() == 1, "lens must be a vector")
-        for t, n, what in ((lens, R, "lens"), (new, R, "new"), (lens_out, R, "lens_out"), (free_count, 1, "free_count"),
-                           (free_count_out, 1, "free_count_out"), (free_list, free_list.numel(), "free_list")):
-            _need_vector(t, i32, n, what)
-        if shift is not None:
-            _need_vector(shift, i32, R, "shift")
+        n = lens.shape[0]
+        for t, size, what in ((lens, n, "lens"), (new, n, "new"), (lens_out, n, "lens_out"), (free_count, 1, "free_count"),
+                              (free_count_out, 1, "free_count_out"), (free_list, free_list.numel(), "free_list"),
+                              (shift, n, "shift")):
+            if t is not None:
+                _need_vector(t, torch.int32, size, what)
+        _need_tables(tables, n)
         _need(total >= 0, "total must not be negative")
-        raise ValueError("tables must be an int32 tensor [requests, width] with contiguous rows")
-    dev, width = lens.device, tables.shape[1]
-    small = torch.empty(4 * R + 5, dtype=i32, device=dev)   # cu, then scratch
-    cu = small[:R + 1]
-    granted = torch.empty(R, dtype=i32, device=dev)
-    slots = torch.empty(total, dtype=torch.int64, device=dev)
-    positions = torch.empty(total, dtype=torch.int64, device=dev)
-    _call("ckv_block_tables", index, _pack_tables(
-        lens.data_ptr(), new.data_ptr(), 0 if shift is None else shift.data_ptr(), tables.data_ptr(),
-        max(tables.stride(0), width), width, free_list.data_ptr(), free_list.shape[0], free_count.data_ptr(), block_size, R,
-        total, lens_out.data_ptr(), free_count_out.data_ptr(), cu.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-        granted.data_ptr(), small.data_ptr() + 4 * (R + 1)))
-    return TableStep(lens_out, free_count_out, cu, slots, positions, granted)
+    _failed("ckv_block_tables", r)
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -528,70 +520,23 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     ``rotary(grad_q, grad_k, ..., inverse=True)`` is the backward pass.  ``out=(q, k)`` works in
     place.  Returns ``(q_out, k_out)``.
     """
-    index, dtype = q.get_device(), q.dtype
-    good = index >= 0 and q.dim() == 3 and dtype in _CODES and positions.get_device() == index \
-        and inv_freq.get_device() == index and positions.dtype is torch.int64 and inv_freq.dtype is torch.float64 \
-        and positions.dim() == 1 and inv_freq.dim() == 1 and positions.is_contiguous() and inv_freq.is_contiguous() \
-        and not ((q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled())
-    if good:
-        T, H, D = q.shape
-        qt, qh, qd = q.stride()
-        good = positions.shape[0] == T and (qd == 1 or D == 1)
-        Hk = kp = kt = kh = ko_p = kot = koh = 0
-        if k is not None and good:
-            good = k.dim() == 3 and k.dtype is dtype and k.get_device() == index and k.shape[0] == T and k.shape[2] == D \
-                and (k.stride(2) == 1 or D == 1)
-    if not good:
-        _one_device(q, k, positions, inv_freq)
-        if torch.is_grad_enabled():
-            _need_no_grad("rotary", q, k)
+    qo, ko = (None, None) if out is None else out
+    r = _lib.torch_calls().rotary(q, k, positions, inv_freq, interleaved, factor, inverse, qo, ko)
+    if type(r) is tuple:
+        return r
+    if r is None:
+        _one_device(q, k, positions, inv_freq, qo, ko)
         _need_rows(q, "q")
         if k is not None:
             _need_rows(k, "k")
-            _need(k.dtype == dtype and k.shape[0] == q.shape[0] and k.shape[2] == q.shape[2],
+            _need(k.dtype == q.dtype and k.shape[0] == q.shape[0] and k.shape[2] == q.shape[2],
                   "q and k must agree in dtype, tokens and head_dim")
         _need_vector(positions, torch.int64, q.shape[0], "positions")
-        raise ValueError("inv_freq must be a contiguous float64 vector")
-    if out is None:
-        qo = torch.empty(T, H, D, dtype=dtype, device=q.device)
-        ko = None if k is None else torch.empty(T, k.shape[1], D, dtype=dtype, device=q.device)
-    else:
-        qo, ko = out
-        for x, o, what in ((q, qo, "out[0]"), (k, ko, "out[1]")):
-            _need((x is None) == (o is None) and (x is None or (o.shape == x.shape and o.dtype == x.dtype)),
-                  f"{what} must be like its input")
-            if o is not None:
-                _need_rows(o, what)
-        _one_device(q, qo, ko)
-    if k is not None:
-        Hk, kp, kt, kh = k.shape[1], k.data_ptr(), k.stride(0), k.stride(1)
-        ko_p, kot, koh = ko.data_ptr(), ko.stride(0), ko.stride(1)
-    _call("ckv_rotary", index, _pack_rotary(
-        q.data_ptr(), qt, qh, kp, kt, kh, qo.data_ptr(), qo.stride(0), qo.stride(1), ko_p, kot, koh, positions.data_ptr(),
-        inv_freq.data_ptr(), factor, T, H, Hk, D, 2 * inv_freq.shape[0], _CODES[dtype], interleaved, inverse, 0))
-    return qo, ko
-
-
-def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, index: int):
-    """The packed ``ckv_cache`` of a layer, and its shape."""
-    fmt = _CACHE_FORMATS.get(k_cache.dtype)
-    shape = k_cache.shape
-    if not (fmt is not None and len(shape) == 4 and v_cache.dtype is k_cache.dtype and v_cache.shape == shape
-            and k_cache.get_device() == index and v_cache.get_device() == index and k_scale.get_device() == index
-            and v_scale.get_device() == index and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32
-            and k_scale.shape == shape[:2] and v_scale.shape == shape[:2] and k_scale.is_contiguous()
-            and v_scale.is_contiguous() and k_cache.stride(3) == 1 and v_cache.stride(3) == 1):
-        _one_device(k_cache, v_cache, k_scale, v_scale)
-        _need(k_cache.get_device() == index, "the cache is on another device", RuntimeError)
-        _need(fmt is not None and v_cache.dtype == k_cache.dtype, "k_cache and v_cache must both be float8_e4m3fn or int8", TypeError)
-        _need(len(shape) == 4 and v_cache.shape == shape and k_cache.stride(3) == 1 and v_cache.stride(3) == 1,
-              "k_cache and v_cache must be [blocks, kv_heads, block_size, head_dim] with contiguous head_dim")
-        raise ValueError(f"scales must be contiguous float32 tensors of shape {tuple(shape[:2])}")
-    N, H, B, D = shape
-    kb, kh, kt, _ = k_cache.stride()
-    vb, vh, vt, _ = v_cache.stride()
-    return _pack_cache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), kb, kh, kt, vb, vh, vt,
-                       N, H, B, D, fmt), H, D
+        _need_vector(inv_freq, torch.float64, inv_freq.numel(), "inv_freq")
+        if out is not None:
+            _need_out(qo, q, "out[0]")
+            _need_out(ko, k, "out[1]")
+    _failed("ckv_rotary", r)
 
 
 def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -605,22 +550,18 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
     begins anew, otherwise its other tokens stay (rescaled where the scale grew).  Slots outside the
     pool (-1) are no tokens.  A NaN or an infinity makes its block and head read as NaN.
     """
-    index, dtype, shape = k.get_device(), k.dtype, k.shape
-    if not (index >= 0 and v.get_device() == index and slots.get_device() == index and len(shape) == 3 and v.shape == shape
-            and dtype in _CODES and v.dtype is dtype and slots.dtype is torch.int64 and slots.dim() == 1
-            and slots.shape[0] == shape[0] and slots.is_contiguous() and k.stride(2) == 1 and v.stride(2) == 1
-            and not ((k.requires_grad or v.requires_grad) and torch.is_grad_enabled())):
-        _one_device(k, v, slots)
-        if torch.is_grad_enabled():
-            _need_no_grad("cache_write", k, v)
+    r = _lib.torch_calls().cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots)
+    if r is True:
+        return
+    if r is None:
+        _one_device(k, v, k_cache, v_cache, k_scale, v_scale, slots)
         _need_rows(k, "k")
         _need_rows(v, "v")
-        _need(v.dtype == dtype and v.shape == shape, "k and v must agree in dtype and shape")
-        _need_vector(slots, torch.int64, shape[0], "slots")
-    c, H, D = _cache(k_cache, v_cache, k_scale, v_scale, index)
-    _need(shape[1] == H and shape[2] == D, f"k and v must be [tokens, {H}, {D}]")
-    _call("ckv_cache_write", index, c, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-          _CODES[dtype], slots.data_ptr(), shape[0])
+        _need(v.dtype == k.dtype and v.shape == k.shape, "k and v must agree in dtype and shape")
+        _need_vector(slots, torch.int64, k.shape[0], "slots")
+        H, D = _need_cache(k_cache, v_cache, k_scale, v_scale)
+        _need(tuple(k.shape[1:]) == (H, D), f"k and v must be [tokens, {H}, {D}]")
+    _failed("ckv_cache_write", r)
 
 
 def cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -628,26 +569,15 @@ def cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
     """The values at ``slots`` (int64 ``[T]``) of a paged 8-bit cache as ``(k, v)`` ``[T, Hkv, D]`` of
     ``dtype``; a slot outside the pool gives zeros.  A cache that is to be scored and compressed
     again goes through here back to ``score_evict``."""
-    _one_device(k_cache, slots)
-    _need(dtype in _CODES, f"dtype must be bf16, fp16 or fp32, got {dtype}", TypeError)
-    index = slots.get_device()
-    c, H, D = _cache(k_cache, v_cache, k_scale, v_scale, index)
-    T = slots.numel()
-    _need_vector(slots, torch.int64, T, "slots")
-    k = torch.empty(T, H, D, dtype=dtype, device=slots.device)
-    v = torch.empty_like(k)
-    _call("ckv_cache_read", index, c, k.data_ptr(), v.data_ptr(), _CODES[dtype], slots.data_ptr(), T)
-    return k, v
-
-
-_att_ws_bytes = {}
-
-
-def _attention_workspace_bytes(key) -> int:
-    b = ctypes.c_size_t()
-    check(_lib.load().ckv_cache_attention_workspace(*key, ctypes.byref(b)), "ckv_cache_attention_workspace")
-    _att_ws_bytes[key] = b.value
-    return b.value
+    r = _lib.torch_calls().cache_read(k_cache, v_cache, k_scale, v_scale, slots, dtype)
+    if type(r) is tuple:
+        return r
+    if r is None:
+        _one_device(k_cache, v_cache, k_scale, v_scale, slots)
+        _need(dtype in _DT, f"dtype must be bf16, fp16 or fp32, got {dtype}", TypeError)
+        _need_cache(k_cache, v_cache, k_scale, v_scale)
+        _need_vector(slots, torch.int64, slots.numel(), "slots")
+    _failed("ckv_cache_read", r)
 
 
 def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -665,45 +595,22 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``out``, if given).  Returns ``out``, or ``(out, lse)`` with ``want_lse``: natural-log
     log-sum-exp, float32 ``[T, H]``.
     """
-    index, dtype, shape = q.get_device(), q.dtype, q.shape
-    R = lens.shape[0] if lens.dim() == 1 else -1
-    if not (index >= 0 and len(shape) == 3 and dtype in _CODES and q.stride(2) == 1 and tables.get_device() == index
-            and lens.get_device() == index and tables.dtype is torch.int32 and lens.dtype is torch.int32 and tables.dim() == 2
-            and tables.shape[0] == R and tables.stride(1) == 1 and lens.is_contiguous()
-            and (shape[0] == R if cu is None else cu.get_device() == index and cu.dtype is torch.int32 and cu.dim() == 1
-                 and cu.shape[0] == R + 1 and cu.is_contiguous())
-            and not (q.requires_grad and torch.is_grad_enabled())):
-        _one_device(q, tables, lens, cu)
-        if torch.is_grad_enabled():
-            _need_no_grad("cache_attention", q)
+    r = _lib.torch_calls().cache_attention(q, k_cache, v_cache, k_scale, v_scale, tables, lens, cu, max_q, scale, causal,
+                                           want_lse, out)
+    if r is not None and type(r) is not int:
+        return r
+    if r is None:
+        _one_device(q, k_cache, v_cache, k_scale, v_scale, tables, lens, cu, out)
         _need_rows(q, "q")
-        _need(tables.dtype == torch.int32 and tables.dim() == 2 and tables.stride(1) == 1,
-              "tables must be an int32 tensor [requests, width] with contiguous rows")
-        _need_vector(lens, torch.int32, tables.shape[0], "lens")
-        _need(cu is not None or R == shape[0], "without cu, q has one row per request")
-        _need_vector(cu, torch.int32, R + 1, "cu")
-    T, H, D = shape
-    c, Hk, cd = _cache(k_cache, v_cache, k_scale, v_scale, index)
-    _need(D == cd and H % Hk == 0, f"q must be [tokens, heads, {cd}] with a multiple of {Hk} heads")
-    dev = q.device
-    if cu is None:
-        max_q = 1
-    if out is None:
-        out = torch.empty(T, H, D, dtype=dtype, device=dev)
-        ot, oh = H * D, D
-    else:
-        _need(out.shape == shape and out.dtype == dtype, "out must be like q")
-        _need_rows(out, "out")
-        _one_device(q, out)
-        ot, oh, _ = out.stride()
-    lse = torch.empty(T, H, dtype=torch.float32, device=dev) if want_lse else None
-    key = (D, max_q, H, Hk)
-    nbytes = _att_ws_bytes.get(key) or _attention_workspace_bytes(key)
-    # from the allocator for each call: two streams, or two captured graphs, never share it
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    a = _pack_attention(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), ot, oh, 0 if lse is None else lse.data_ptr(),
-                        tables.data_ptr(), max(tables.stride(0), tables.shape[1]), tables.shape[1], lens.data_ptr(),
-                        0 if cu is None else cu.data_ptr(), R, T, max_q, H, causal, D ** -0.5 if scale is None else scale,
-                        _CODES[dtype])
-    _call("ckv_cache_attention", index, c, a, ws.data_ptr(), nbytes)
-    return (out, lse) if want_lse else out
+        H, D = _need_cache(k_cache, v_cache, k_scale, v_scale)
+        _need(q.shape[2] == D and H > 0 and q.shape[1] % H == 0, f"q must be [tokens, heads, {D}] with a multiple of {H} heads")
+        R = lens.shape[0] if lens.dim() == 1 else -1
+        _need_tables(tables, R)
+        _need_vector(lens, torch.int32, R, "lens")
+        if cu is None:
+            _need(R == q.shape[0], "without cu, q has one row per request")
+        else:
+            _need_vector(cu, torch.int32, R + 1, "cu")
+        if out is not None:
+            _need_out(out, q, "out")
+    _failed("ckv_cache_attention", r)

@@ -74,7 +74,7 @@ def test_attention_workspace_is_checked():
     assert lib.ckv_cache_attention_workspace(128, 1, 8, 2, None) == -1
 
 
-@pytest.mark.parametrize("over", [dict(lens=None), dict(out_slots=None), dict(out_granted=None), dict(work=None), dict(requests=0), dict(requests=8193),
+@pytest.mark.parametrize("over", [dict(lens=None), dict(out_slots=None), dict(out_granted=None), dict(work=None, total=4096), dict(requests=0), dict(requests=8193),
                                   dict(total=-1), dict(table_width=0), dict(table_stride=1), dict(block_size=0),
                                   dict(free_capacity=-1)])
 def test_bad_table_steps_are_refused(over):
