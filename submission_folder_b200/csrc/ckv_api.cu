@@ -882,7 +882,8 @@ static int check_cache(const ckv_cache* c) {
 
 int ckv_block_tables(const ckv_table_step* s, ckv_stream_t stream) {
   if (!s || !s->lens || !s->new_tokens || !s->tables || !s->free_list || !s->free_count || !s->out_lens ||
-      !s->out_free_count || !s->out_cu || !s->out_granted || !s->work || (s->total > 0 && (!s->out_slots || !s->out_positions)))
+      !s->out_free_count || !s->out_cu || !s->out_granted || (s->total > 0 && (!s->out_slots || !s->out_positions)) ||
+      (!s->work && (int64_t)s->requests + s->total > CKV_TABLES_SMALL))
     return fail(CKV_ERR_ARG, "null argument");
   if (s->requests < 1 || s->requests > kMaxRequests) return fail(CKV_ERR_ARG, "1 to 8192 requests");
   if (s->total < 0 || s->table_width < 1 || s->table_stride < s->table_width || s->free_capacity < 0)
