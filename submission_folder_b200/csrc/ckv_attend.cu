@@ -515,26 +515,31 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
         // logits^T: lane holds tokens g, g + 8 of each 16 x rows 2t, 2t + 1
         float sc[NT][2][4];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int row = u * 16 + g;
+        for (int c = 0; c < D / 64; ++c) {
+          uint4 w[2][2];
 #pragma unroll
-          for (int c = 0; c < D / 64; ++c) {
-            const uint4 wa = lds4(kst + swz(row, D == 128 ? 2 * t + c : t)), wb = lds4(kst + swz(row + 8, D == 128 ? 2 * t + c : t));
-            const uint32_t a4[4] = {wa.x, wa.y, wa.z, wa.w}, b4[4] = {wb.x, wb.y, wb.z, wb.w};
+          for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t a[4];
-              codes4<kFmt>(a4[e], a[0], a[2]);
-              codes4<kFmt>(b4[e], a[1], a[3]);
+            for (int h = 0; h < 2; ++h) w[u][h] = lds4(kst + swz(u * 16 + h * 8 + g, D == 128 ? 2 * t + c : t));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t a[2][4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              codes4<kFmt>(e == 0 ? w[u][0].x : e == 1 ? w[u][0].y : e == 2 ? w[u][0].z : w[u][0].w, a[u][0], a[u][2]);
+              codes4<kFmt>(e == 0 ? w[u][1].x : e == 1 ? w[u][1].y : e == 2 ? w[u][1].z : w[u][1].w, a[u][1], a[u][3]);
+            }
+            // the sums of the 16-token halves and the row tiles are independent: they take turns
+#pragma unroll
+            for (int k = 0; k < kTerms; ++k)
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int k = 0; k < kTerms; ++k) {
+                for (int u = 0; u < 2; ++u) {
                   const uint32_t(&b)[2] = qf[nt][k][c * 4 + e];
-                  if (c == 0 && e == 0 && k == 0) mma16816_zero(sc[nt][u], a, b[0], b[1]);
-                  else mma16816(sc[nt][u], a, b[0], b[1]);
+                  if (c == 0 && e == 0 && k == 0) mma16816_zero(sc[nt][u], a[u], b[0], b[1]);
+                  else mma16816(sc[nt][u], a[u], b[0], b[1]);
                 }
-            }
           }
         }
         float ks[2], ve[2];
