@@ -294,8 +294,8 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
   static_assert(2 * kWarps <= 32, "one ballot");
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x, R = p.a.requests;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid < 2 * kWarps) s_entry[tid].used = 0;
+  after_previous();
 
   // ---- the line of units: its length, and where this warp stands in it (each warp for itself)
   const uint32_t first = lane < R ? seq_work<NT>(p, lane) : 0;
@@ -794,7 +794,7 @@ constexpr int kMergeThreads = 256;
 
 template <int D, int NT>
 __global__ void __launch_bounds__(kMergeThreads) k_attend_merge(const AttArgs p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  after_previous();
   constexpr int kPart = part_floats(D, 8 * NT);
   const int cta = blockIdx.x;
   const int4 d = __ldcg(p.desc + cta);
@@ -822,18 +822,8 @@ static cudaError_t att_launch(AttArgs& p, void* ws, cudaStream_t st) {
   p.desc = reinterpret_cast<int4*>(p.ws + (size_t)kAttMaxCtas * (kAttMaxWarps + 2) * part_floats(D, 8 * NT));
   auto fn = k_attend<D, kFmt, NT, kTerms>;
   if (cudaError_t e = ensure_dynamic_smem((const void*)fn, smem); e != cudaSuccess) return e;
-  fn<<<p.ctas, att_warps(NT, kTerms) * 32, smem, st>>>(p);
-  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(p.ctas);
-  cfg.blockDim = dim3(kMergeThreads);
-  cfg.stream = st;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_attend_merge<D, NT>, p);
+  if (cudaError_t e = launch_after(fn, dim3(p.ctas), att_warps(NT, kTerms) * 32, smem, st, p); e != cudaSuccess) return e;
+  return launch_after(k_attend_merge<D, NT>, dim3(p.ctas), kMergeThreads, 0, st, p);
 }
 
 template <int D, int kFmt>

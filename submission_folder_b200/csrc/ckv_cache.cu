@@ -176,6 +176,7 @@ __global__ void __launch_bounds__(kCacheMaxBlock / kRowsPerWarp * 32) k_cache_wr
     blk = s >= 0 && s < pool ? (int)(s >> a.block_log2) : -1;
     place = (int)s & (bs - 1);
   };
+  after_previous();
   // the piece's slots and those that a run may reach, in one reading
   const int window = T1 - T0 + bs + 2;
   for (int j = threadIdx.x; j < window; j += blockDim.x) decode(T0 - 1 + j, s_slot[0][j], s_slot[1][j]);
@@ -333,6 +334,7 @@ __global__ void __launch_bounds__(256) k_cache_read(const ckv_cache c, const Cac
   const uint32_t per_row = c.head_dim / 16, per_tok = per_row * c.num_kv_heads;
   const uint32_t i = blockIdx.x * 256 + threadIdx.x, half = (r.tokens + kReadTokens - 1) / kReadTokens;
   const uint32_t t = i / per_tok;
+  after_previous();
   if (t >= half) return;
   const uint32_t h = (i - t * per_tok) / per_row, v16 = i - t * per_tok - h * per_row;
   const int64_t pool = (int64_t)c.num_blocks << block_log2;
@@ -381,9 +383,8 @@ static int log2_of(int x) {
 }
 
 template <typename T, int kFmt>
-static void write_launch(const WriteArgs& a, dim3 grid, int threads, cudaStream_t st) {
-  if (a.c.head_dim == 64) k_cache_write<T, kFmt, 64><<<grid, threads, 0, st>>>(a);
-  else k_cache_write<T, kFmt, 128><<<grid, threads, 0, st>>>(a);
+static cudaError_t write_launch(const WriteArgs& a, dim3 grid, int threads, cudaStream_t st) {
+  return launch_after(a.c.head_dim == 64 ? k_cache_write<T, kFmt, 64> : k_cache_write<T, kFmt, 128>, grid, threads, 0, st, a);
 }
 
 cudaError_t launch_cache_write(const ckv_cache& c, const CacheRows& r, cudaStream_t st) {
@@ -400,17 +401,13 @@ cudaError_t launch_cache_write(const ckv_cache& c, const CacheRows& r, cudaStrea
   const bool e4 = c.format == CKV_CACHE_E4M3;
   switch (r.dtype) {
     case CKV_BF16:
-      e4 ? write_launch<__nv_bfloat16, CKV_CACHE_E4M3>(a, grid, threads, st)
-         : write_launch<__nv_bfloat16, CKV_CACHE_INT8>(a, grid, threads, st);
-      break;
+      return e4 ? write_launch<__nv_bfloat16, CKV_CACHE_E4M3>(a, grid, threads, st)
+                : write_launch<__nv_bfloat16, CKV_CACHE_INT8>(a, grid, threads, st);
     case CKV_FP16:
-      e4 ? write_launch<__half, CKV_CACHE_E4M3>(a, grid, threads, st) : write_launch<__half, CKV_CACHE_INT8>(a, grid, threads, st);
-      break;
+      return e4 ? write_launch<__half, CKV_CACHE_E4M3>(a, grid, threads, st) : write_launch<__half, CKV_CACHE_INT8>(a, grid, threads, st);
     default:
-      e4 ? write_launch<float, CKV_CACHE_E4M3>(a, grid, threads, st) : write_launch<float, CKV_CACHE_INT8>(a, grid, threads, st);
-      break;
+      return e4 ? write_launch<float, CKV_CACHE_E4M3>(a, grid, threads, st) : write_launch<float, CKV_CACHE_INT8>(a, grid, threads, st);
   }
-  return cudaGetLastError();
 }
 
 cudaError_t launch_cache_read(const ckv_cache& c, const CacheRows& r, cudaStream_t st) {
@@ -420,19 +417,13 @@ cudaError_t launch_cache_read(const ckv_cache& c, const CacheRows& r, cudaStream
   const bool e4 = c.format == CKV_CACHE_E4M3;
   switch (r.dtype) {
     case CKV_BF16:
-      e4 ? k_cache_read<__nv_bfloat16, CKV_CACHE_E4M3><<<grid, 256, 0, st>>>(c, r, bl)
-         : k_cache_read<__nv_bfloat16, CKV_CACHE_INT8><<<grid, 256, 0, st>>>(c, r, bl);
-      break;
+      return launch_after(e4 ? k_cache_read<__nv_bfloat16, CKV_CACHE_E4M3> : k_cache_read<__nv_bfloat16, CKV_CACHE_INT8>, grid, 256, 0,
+                          st, c, r, bl);
     case CKV_FP16:
-      e4 ? k_cache_read<__half, CKV_CACHE_E4M3><<<grid, 256, 0, st>>>(c, r, bl)
-         : k_cache_read<__half, CKV_CACHE_INT8><<<grid, 256, 0, st>>>(c, r, bl);
-      break;
+      return launch_after(e4 ? k_cache_read<__half, CKV_CACHE_E4M3> : k_cache_read<__half, CKV_CACHE_INT8>, grid, 256, 0, st, c, r, bl);
     default:
-      e4 ? k_cache_read<float, CKV_CACHE_E4M3><<<grid, 256, 0, st>>>(c, r, bl)
-         : k_cache_read<float, CKV_CACHE_INT8><<<grid, 256, 0, st>>>(c, r, bl);
-      break;
+      return launch_after(e4 ? k_cache_read<float, CKV_CACHE_E4M3> : k_cache_read<float, CKV_CACHE_INT8>, grid, 256, 0, st, c, r, bl);
   }
-  return cudaGetLastError();
 }
 
 }  // namespace ckv

@@ -10,6 +10,29 @@
 
 namespace ckv {
 
+// A launch that may begin while the launch before it on the stream drains (programmatic
+// dependent launch): its blocks are placed early and wait in after_previous(), which every
+// kernel launched so calls in every thread before it touches global memory.  Saves the gap
+// between the short kernels of a decode step.
+template <typename... P>
+cudaError_t launch_after(void (*fn)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, P... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fn, args...);
+}
+__device__ __forceinline__ void after_previous() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the next launch may be placed
+  asm volatile("griddepcontrol.wait;" ::: "memory");                // the previous one is complete
+}
+
 constexpr int kMaxRequests = 8192;   // rows of one block-table step (their prefix sums sit in shared memory)
 constexpr int kCacheMaxBlock = 128;  // tokens of a cache block: 16, 32, 64 or 128
 

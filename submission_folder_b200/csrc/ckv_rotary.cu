@@ -30,6 +30,7 @@ template <typename T, int N> struct alignas(sizeof(T) * N) Vec { T x[N]; };
 template <typename T, int N, bool kInter>
 __global__ void __launch_bounds__(kRotThreads) k_rotary(const ckv_rotary_args a, int tokens_per_cta) {
   extern __shared__ float2 rot_cs[];   // [tokens_per_cta][pairs]
+  after_previous();
   const int pairs = a.rotary_dim / 2;
   const int t0 = blockIdx.x * tokens_per_cta;
   const int nt = min(tokens_per_cta, a.tokens - t0);
@@ -98,10 +99,9 @@ __global__ void __launch_bounds__(kRotThreads) k_rotary(const ckv_rotary_args a,
 }
 
 template <typename T, int N>
-static void rot_launch(const ckv_rotary_args& a, int tpc, dim3 grid, cudaStream_t st) {
+static cudaError_t rot_launch(const ckv_rotary_args& a, int tpc, dim3 grid, cudaStream_t st) {
   const size_t smem = (size_t)tpc * (a.rotary_dim / 2) * sizeof(float2);
-  if (a.interleaved) k_rotary<T, N, true><<<grid, kRotThreads, smem, st>>>(a, tpc);
-  else k_rotary<T, N, false><<<grid, kRotThreads, smem, st>>>(a, tpc);
+  return launch_after(a.interleaved ? k_rotary<T, N, true> : k_rotary<T, N, false>, grid, kRotThreads, smem, st, a, tpc);
 }
 
 cudaError_t launch_rotary(const ckv_rotary_args& args, cudaStream_t st) {
@@ -122,11 +122,10 @@ cudaError_t launch_rotary(const ckv_rotary_args& args, cudaStream_t st) {
   a.heads_per_cta = (heads + splits - 1) / splits;
   const dim3 grid((a.tokens + tpc - 1) / tpc, (heads + a.heads_per_cta - 1) / a.heads_per_cta);
   switch (a.dtype) {
-    case CKV_BF16: vec ? rot_launch<__nv_bfloat16, 8>(a, tpc, grid, st) : rot_launch<__nv_bfloat16, 1>(a, tpc, grid, st); break;
-    case CKV_FP16: vec ? rot_launch<__half, 8>(a, tpc, grid, st) : rot_launch<__half, 1>(a, tpc, grid, st); break;
-    default: vec ? rot_launch<float, 4>(a, tpc, grid, st) : rot_launch<float, 1>(a, tpc, grid, st); break;
+    case CKV_BF16: return vec ? rot_launch<__nv_bfloat16, 8>(a, tpc, grid, st) : rot_launch<__nv_bfloat16, 1>(a, tpc, grid, st);
+    case CKV_FP16: return vec ? rot_launch<__half, 8>(a, tpc, grid, st) : rot_launch<__half, 1>(a, tpc, grid, st);
+    default: return vec ? rot_launch<float, 4>(a, tpc, grid, st) : rot_launch<float, 1>(a, tpc, grid, st);
   }
-  return cudaGetLastError();
 }
 
 }  // namespace ckv

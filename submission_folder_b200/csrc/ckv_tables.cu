@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kTabThreads) k_block_tables(const ckv_table_st
   int* fresh = back + R + 1;      // [R + 1] fresh blocks wanted before request r
   int* len = fresh + R + 1;       // [R] old length
   int* give = len + R;            // [R] tokens granted; before that -2: ended, -1: does not fit its row
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  after_previous();
   if (tid == 0) s_taken = 0;
   const int count = min(max(*s.free_count, 0), s.free_capacity);
   Sum3 run = {0, 0, 0};
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kFillThreads) k_block_tables_fill(const ckv_ta
   __shared__ int s_id[kFillBlocks];
   const int R = s.requests, r = blockIdx.x, part = blockIdx.y, parts = gridDim.y, tid = threadIdx.x;
   const uint32_t b = s.block_size;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  after_previous();
   const int *back = s.work, *fresh = back + R + 1, *len = fresh + R + 1, *tail = len + R;
   if (r == R) {   // no request's tokens
     for (int64_t t = (int64_t)__ldcg(s.out_cu + R) + part * kFillThreads + tid; t < s.total; t += parts * kFillThreads) {
@@ -294,19 +294,10 @@ cudaError_t launch_block_tables(const ckv_table_step& s, cudaStream_t st) {
   const size_t smem = (size_t)(5 * s.requests + 3) * sizeof(int);
   if (cudaError_t e = ensure_dynamic_smem((const void*)k_block_tables, smem); e != cudaSuccess) return e;
   const bool solo = (int64_t)s.total + s.requests <= CKV_TABLES_SMALL;
-  k_block_tables<<<1, kTabThreads, smem, st>>>(s, solo ? 1 : 0);
-  if (cudaError_t e = cudaGetLastError(); solo || e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  if (cudaError_t e = launch_after(k_block_tables, dim3(1), kTabThreads, smem, st, s, solo ? 1 : 0); solo || e != cudaSuccess)
+    return e;
   const int parts = s.requests >= 592 ? 1 : std::min(592 / s.requests, 64);   // about four CTAs per SM
-  cfg.gridDim = dim3(s.requests + 1, parts);
-  cfg.blockDim = dim3(kFillThreads);
-  cfg.stream = st;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_block_tables_fill, s);
+  return launch_after(k_block_tables_fill, dim3(s.requests + 1, parts), kFillThreads, 0, st, s);
 }
 
 }  // namespace ckv

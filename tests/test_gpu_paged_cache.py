@@ -612,6 +612,66 @@ def test_attention_streams_and_graphs(dev):
             assert all(torch.equal(a, b) for a, b in zip(outs, alone))
 
 
+def test_launches_wait_for_what_comes_before(dev):
+    """Kernels that may be placed early still wait: for a long kernel, a copy or a fill just before
+    them on the stream, for another stream through an event, and eagerly as in a captured graph."""
+    T, H, D = 4, 4, 64
+    f, _ = rotary_frequencies(D, device=dev)
+    pos = torch.arange(T, device=dev)
+    src = torch.randn(T, H, D, device=dev, generator=torch.Generator(device=dev).manual_seed(3))
+    big = torch.randn(3000, 3000, device=dev)
+    zero = torch.zeros(T, H, D, device=dev)
+    want, _ = ops.rotary(src, None, pos, f)
+    q = torch.empty_like(src)
+    pool = _pool(dev, 4, H, 16, D, E4M3)
+    slots = torch.arange(T, device=dev)
+
+    def step():
+        y = big @ big                                             # something long, then a small kernel
+        q.copy_(src + 0 * y[0, 0])
+        a, _ = ops.rotary(q, None, pos, f)
+        q.zero_()                                                 # a fill and a copy of memory between the launches
+        b, _ = ops.rotary(q, None, pos, f)
+        q.copy_(src)
+        ops.cache_write(q, q, *pool, slots)
+        k, v = ops.cache_read(*pool, slots, torch.float32)
+        return a, b, k, v
+
+    r = ref.RefCache(H, 16, E4M3)
+    r.write(src.double().cpu(), list(range(T)))
+    held = r.read(list(range(T)), D).float()
+
+    def check(got):
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want) and torch.equal(got[1], zero)
+        assert torch.equal(got[2].cpu(), held) and torch.equal(got[3].cpu(), held)
+
+    check(step())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        for t in got:
+            t.fill_(7.0)
+        graph.replay()
+        check(got)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        q.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a):
+            y = big @ big
+            q.copy_(src + 0 * y[0, 0])
+            done = torch.cuda.Event()
+            done.record()
+        with torch.cuda.stream(b):
+            b.wait_event(done)
+            got, _ = ops.rotary(q, None, pos, f)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_attention_refusals(dev):
     pool, tables, n, q, k, v = _attention_case(dev, [20, 30], 2, 2, 64, 16, E4M3, torch.bfloat16, [1] * 2)
     cu = torch.tensor([0, 1, 2], dtype=torch.int32, device=dev)
