@@ -162,13 +162,21 @@ CKV_DEV void row_split(const AttArgs& p, int rho, int& token, int& member) {
   member = rho - token * p.group;
 }
 
+// x / y for y > 0 by a reciprocal: two rounds leave the quotient within one of the truth.
+CKV_DEV uint32_t div_u32(uint32_t x, uint32_t y) {
+  const float inv = __frcp_rn((float)y);
+  uint32_t q = (uint32_t)(__uint2float_rz(x) * (inv * 0.9999998f));   // below the quotient, by x 2^-21 / y at most
+  q += (uint32_t)(__uint2float_rz(x - q * y) * (inv * 0.9999998f));
+  return x - q * y >= y ? q + 1 : q;
+}
+
 // The line of units cut in `parts`: the first `rem` parts have one step more.
 struct Cut {
   uint32_t each, rem;
   CKV_DEV uint32_t at(uint32_t part) const { return part * each + min(part, rem); }
   CKV_DEV uint32_t of(uint32_t x) const {   // the part that holds step x
     const uint32_t big = rem * (each + 1);
-    return x < big ? x / (each + 1) : rem + (x - big) / each;
+    return x < big ? div_u32(x, each + 1) : rem + div_u32(x - big, each);
   }
 };
 
@@ -304,7 +312,8 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
   for (int r = lane + 32; r < R; r += 32) total += seq_work<NT>(p, r);
   total = __reduce_add_sync(0xffffffffu, total);
   const uint32_t nctas = min((uint32_t)p.ctas, (total + kWarps - 1) / kWarps);
-  const Cut cut = {nctas ? total / nctas : 0u, nctas ? total % nctas : 0u};
+  const uint32_t per_cta = nctas ? div_u32(total, nctas) : 0u;
+  const Cut cut = {per_cta, total - per_cta * nctas};
   const uint32_t c0 = cta < nctas ? cut.at(cta) : total, c1 = cta < nctas ? cut.at(cta + 1) : total;
   const Cut warps = {(c1 - c0) / kWarps, (c1 - c0) % kWarps};
   const uint32_t here = c0 + warps.at(wid);
@@ -348,14 +357,14 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
     int n = seq_len(p, r), q0, nq;
     seq_queries(p, r, q0, nq);
     uint32_t steps = steps_of(n);
-    uint32_t unit = (here - seq_at) / steps;
+    uint32_t unit = div_u32(here - seq_at, steps);
     int step = (int)(here - seq_at - unit * steps);
     bool first_piece = true;
     while (left > 0) {
       const int todo = (int)min(left, steps - step);
       const int s_begin = step, s_end = step + todo;
       const uint32_t tiles = (uint32_t)(nq * p.group + 8 * NT - 1) / (8 * NT);
-      const int head = unit / tiles, tile = unit - head * tiles;
+      const int head = tiles == 1 ? unit : div_u32(unit, tiles), tile = unit - head * tiles;
       const int rows = nq * p.group;
       const int32_t* table = p.a.tables + r * p.a.table_stride;
       const int pages = (n + (1 << p.block_log2) - 1) >> p.block_log2;
@@ -440,27 +449,37 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
       cp_commit();
       // lane (g, t) has row g's dimensions of its chunks
       auto load_queries = [&]() {
-        float4 x[NT][kSteps16];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int k = 0; k < kSteps16; ++k) {
-            const int dim = D == 128 ? (2 * t + k / 4) * 16 + (k & 3) * 4 : t * 16 + k * 4;
-            x[nt][k] = load_q4(q_a + ((nt * 8 + g) << q_log2 << 4), g, p.a.dtype, dim);
-          }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const int rho = (tile * NT + nt) * 8 + g;
-          float top = 0.f;
+          const uint32_t row = q_a + ((nt * 8 + g) << q_log2 << 4);
+          auto dim_of = [&](int k) { return D == 128 ? (2 * t + k / 4) * 16 + (k & 3) * 4 : t * 16 + k * 4; };
+          float top;
+          float4 x[kSteps16];
+          uint2 w[kSteps16];
+          if constexpr (kTerms == 1) {   // bf16: magnitudes of both halves of a word at a time
+            uint32_t m = 0;
 #pragma unroll
-          for (int k = 0; k < kSteps16; ++k)
-            top = fmaxf(fmaxf(fmaxf(top, fabsf(x[nt][k].x)), fmaxf(fabsf(x[nt][k].y), fabsf(x[nt][k].z))), fabsf(x[nt][k].w));
+            for (int k = 0; k < kSteps16; ++k) {
+              w[k] = lds2(row + (((dim_of(k) >> 3) ^ g) << 4) + (dim_of(k) & 4) * 2);
+              asm("max.NaN.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[k].x));
+              asm("max.NaN.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[k].y));
+            }
+            top = fmaxf(fabsf(__uint_as_float(m << 16)), fabsf(__uint_as_float(m & 0xffff0000u)));
+          } else {
+            top = 0.f;
+#pragma unroll
+            for (int k = 0; k < kSteps16; ++k) {
+              x[k] = load_q4(row, g, p.a.dtype, dim_of(k));
+              top = fmaxf(fmaxf(fmaxf(top, fabsf(x[k].x)), fmaxf(fabsf(x[k].y), fabsf(x[k].z))), fabsf(x[k].w));
+            }
+          }
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           // the row times 2^(14 - exponent); exponents at the ends of the range are clamped
           const int e = min(max((int)(__float_as_uint(top) >> 23), 16), 254);   // biased
           const float up = __uint_as_float((uint32_t)(268 - e) << 23);
-          const float mine = p.a.scale * kLog2e / up;
+          const float mine = p.a.scale * kLog2e * __uint_as_float((uint32_t)(e - 14) << 23);   // over up
           int i, member;
           row_split(p, rho, i, member);
           const int sees = rho < rows && p.a.causal ? n - nq + i + 1 : n;
@@ -472,13 +491,15 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
           }
 #pragma unroll
           for (int k = 0; k < kSteps16; ++k) {
-            const float4 v = x[nt][k];
             if constexpr (kTerms == 1) {
-              qf[nt][0][k][0] = half2_bits(v.x * up, v.y * up);
-              qf[nt][0][k][1] = half2_bits(v.z * up, v.w * up);
+              auto to_half = [&](uint32_t v) {
+                return half2_bits(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xffff0000u) * up);
+              };
+              qf[nt][0][k][0] = to_half(w[k].x);
+              qf[nt][0][k][1] = to_half(w[k].y);
             } else {
-              split2(v.x * up, v.y * up, qf[nt][0][k][0], qf[nt][1][k][0]);
-              split2(v.z * up, v.w * up, qf[nt][0][k][1], qf[nt][1][k][1]);
+              split2(x[k].x * up, x[k].y * up, qf[nt][0][k][0], qf[nt][1][k][0]);
+              split2(x[k].z * up, x[k].w * up, qf[nt][0][k][1], qf[nt][1][k][1]);
             }
           }
         }
@@ -766,7 +787,7 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
         list &= list - 1;
         return part;
       }, count, tid, kWarps * 32, dst, e.q0, e.rows, e.head, e.tile);
-      if (begins && !ends) todo = make_int4((int)(cut.of(e.end - 1) - cta + 1) | e.head << 8, e.q0, e.rows, e.tile);
+      if (tid == 0 && begins && !ends) todo = make_int4((int)(cut.of(e.end - 1) - cta + 1) | e.head << 8, e.q0, e.rows, e.tile);
       firsts = later;
     }
     if (tid == 0) p.desc[cta] = todo;
