@@ -224,59 +224,52 @@ CKV_DEV void row_home(const AttArgs& p, int q0, int head, int rho, int64_t& out,
 CKV_DEV float row_factor(float m, float mw, float l) { return l > 0.f || isnan(l) ? exp2f(mw - m - kTop) / l : 0.f; }
 CKV_DEV float row_lse(float m, float l) { return l > 0.f || isnan(l) ? (m + log2f(l)) * kLn2 : -INFINITY; }
 
-// Merge of `count` partial results of one unit, next() their places in turn: to the output, or to
-// `dst`.  A thread has four dimensions of a row; kBatch parts are read at a time.  kL2: other
-// CTAs' results, read from L2.
+// Merge of `count` partial results of one unit, next() their places in turn: four dimensions, from d
+// on, of row `row` of the unit, to the output or to `dst`.  kBatch parts are read at a time.  kL2:
+// other CTAs' results, read from L2.
 template <int D, int NT, bool kL2, int kBatch, typename F>
-CKV_DEV void merge_parts(const AttArgs& p, F parts, int count, int tid, int threads, float* dst, int q0, int rows, int head,
-                         int tile) {
+CKV_DEV void merge_row(const AttArgs& p, F next, int count, int row, int d, float* dst, int q0, int head, int tile) {
   auto get4 = [](const float* x) {
     return kL2 ? __ldcg(reinterpret_cast<const float4*>(x)) : *reinterpret_cast<const float4*>(x);
   };
-  for (int i = tid; i < 8 * NT * (D / 4); i += threads) {
-    const int row = i / (D / 4), d = i % (D / 4) * 4;
-    const int rho = tile * 8 * NT + row;
-    if (rho >= rows) break;
-    auto next = parts;
-    float m = kNone, mw = kNone, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < count; k += kBatch) {
-      float4 s[kBatch], x[kBatch];
+  float m = kNone, mw = kNone, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < count; k += kBatch) {
+    float4 s[kBatch], x[kBatch];
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        s[j] = make_float4(kNone, kNone, 0.f, 0.f);
-        x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (k + j < count) {
-          const float* q = next();
-          s[j] = get4(q + row * 4);
-          x[j] = get4(q + 8 * NT * 4 + row * D + d);
-        }
+    for (int j = 0; j < kBatch; ++j) {
+      s[j] = make_float4(kNone, kNone, 0.f, 0.f);
+      x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k + j < count) {
+        const float* q = next();
+        s[j] = get4(q + row * 4);
+        x[j] = get4(q + 8 * NT * 4 + row * D + d);
       }
-      float nm = m, nw = mw;
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) { nm = fmaxf(nm, s[j].x); nw = fmaxf(nw, s[j].y); }
-      l *= ex2(m - nm);
-      const float f0 = ex2(mw - nw);
-      o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        l += s[j].z * ex2(s[j].x - nm);
-        const float f = ex2(s[j].y - nw);
-        o.x += x[j].x * f; o.y += x[j].y * f; o.z += x[j].z * f; o.w += x[j].w * f;
-      }
-      m = nm;
-      mw = nw;
     }
-    if (dst) {
-      if (d == 0) *reinterpret_cast<float4*>(dst + row * 4) = make_float4(m, mw, l, 0.f);
-      *reinterpret_cast<float4*>(dst + 8 * NT * 4 + row * D + d) = o;
-    } else {
-      int64_t at, lat;
-      row_home(p, q0, head, rho, at, lat);
-      const float f = row_factor(m, mw, l);
-      store_out4(p.a.out, p.a.dtype, at + d, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
-      if (p.a.lse && d == 0) p.a.lse[lat] = row_lse(m, l);
+    float nm = m, nw = mw;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) { nm = fmaxf(nm, s[j].x); nw = fmaxf(nw, s[j].y); }
+    l *= ex2(m - nm);
+    const float f0 = ex2(mw - nw);
+    o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      l += s[j].z * ex2(s[j].x - nm);
+      const float f = ex2(s[j].y - nw);
+      o.x += x[j].x * f; o.y += x[j].y * f; o.z += x[j].z * f; o.w += x[j].w * f;
     }
+    m = nm;
+    mw = nw;
+  }
+  if (dst) {
+    if (d == 0) *reinterpret_cast<float4*>(dst + row * 4) = make_float4(m, mw, l, 0.f);
+    *reinterpret_cast<float4*>(dst + 8 * NT * 4 + row * D + d) = o;
+  } else {
+    int64_t at, lat;
+    row_home(p, q0, head, tile * 8 * NT + row, at, lat);
+    const float f = row_factor(m, mw, l);
+    store_out4(p.a.out, p.a.dtype, at + d, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+    if (p.a.lse && d == 0) p.a.lse[lat] = row_lse(m, l);
   }
 }
 
@@ -299,6 +292,8 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
   extern __shared__ __align__(128) char att_smem[];
   __shared__ float s_scale[kWarps][kStages][4];  // K, V of the step's first and second 16 tokens
   __shared__ Entry s_entry[2 * kWarps];
+  __shared__ int2 s_group[2 * kWarps];           // of each unit in pieces: its first entry, and all of them as a mask
+  __shared__ int s_groups;
   static_assert(2 * kWarps <= 32, "one ballot");
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x, R = p.a.requests;
@@ -768,29 +763,43 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
   // ---- merge the pieces of each unit within the CTA; a unit that reaches past the CTA leaves its
   // part in slot 0 (begun in a CTA before) or 1 (begun here)
   if (c1 > c0) {
-    int4 todo = make_int4(0, 0, 0, 0);
-    // the used entries in order, and the first of each unit (each warp for itself)
-    const bool used = lane < 2 * kWarps && s_entry[lane].used;
-    const uint32_t mask = __ballot_sync(0xffffffffu, used), below = mask & ((1u << lane) - 1);
-    const uint32_t mine = used ? s_entry[lane].begin : 0;
-    const uint32_t prev = __shfl_sync(0xffffffffu, mine, below ? 31 - __clz(below) : 0);
-    uint32_t firsts = __ballot_sync(0xffffffffu, used && (!below || prev != mine));
-    while (firsts) {
-      const Entry& e = s_entry[__ffs(firsts) - 1];
-      const uint32_t later = firsts & (firsts - 1);
-      uint32_t list = mask & (0u - (firsts & -firsts)) & (later ? (later & -later) - 1 : 0xffffffffu);
-      const int count = __popc(list);
+    if (wid == 0) {
+      const bool used = lane < 2 * kWarps && s_entry[lane].used;
+      const uint32_t mask = __ballot_sync(0xffffffffu, used), below = mask & ((1u << lane) - 1);
+      const uint32_t mine = used ? s_entry[lane].begin : 0;
+      const uint32_t prev = __shfl_sync(0xffffffffu, mine, below ? 31 - __clz(below) : 0);
+      const bool first_of = used && (!below || prev != mine);
+      const uint32_t firsts = __ballot_sync(0xffffffffu, first_of);
+      const uint32_t later = lane < 31 ? firsts >> (lane + 1) << (lane + 1) : 0;
+      if (first_of)
+        s_group[__popc(firsts & ((1u << lane) - 1))] =
+            make_int2(lane, mask & (0xffffffffu << lane) & (later ? (later & -later) - 1 : 0xffffffffu));
+      if (lane == 0) s_groups = __popc(firsts);
+    }
+    __syncthreads();
+    const int groups = s_groups;
+    // a thread has four dimensions of a row of a unit; the units of a CTA side by side, row by row
+    for (int i = tid; i < groups * 8 * NT * (D / 4); i += kWarps * 32) {
+      const int d = i % (D / 4) * 4, row = i / (D / 4) / groups, grp = i / (D / 4) - row * groups;
+      const Entry& e = s_entry[s_group[grp].x];
+      if (e.tile * 8 * NT + row >= e.rows) continue;
+      uint32_t list = s_group[grp].y;
       const bool begins = e.begin >= c0, ends = e.end <= c1;
       float* dst = begins && ends ? nullptr : p.ws + ((size_t)cta * (kAttMaxWarps + 2) + kAttMaxWarps + (begins ? 1 : 0)) * kPart;
-      merge_parts<D, NT, false, 4>(p, [list]() mutable {
+      merge_row<D, NT, false, 4>(p, [&]() {
         const float* part = s_entry[__ffs(list) - 1].part;
         list &= list - 1;
         return part;
-      }, count, tid, kWarps * 32, dst, e.q0, e.rows, e.head, e.tile);
-      if (tid == 0 && begins && !ends) todo = make_int4((int)(cut.of(e.end - 1) - cta + 1) | e.head << 8, e.q0, e.rows, e.tile);
-      firsts = later;
+      }, __popc(list), row, d, dst, e.q0, e.head, e.tile);
     }
-    if (tid == 0) p.desc[cta] = todo;
+    if (tid == kWarps * 32 - 1) {   // the last unit may reach past the CTA
+      int4 todo = make_int4(0, 0, 0, 0);
+      if (groups) {
+        const Entry& e = s_entry[s_group[groups - 1].x];
+        if (e.begin >= c0 && e.end > c1) todo = make_int4((int)(cut.of(e.end - 1) - cta + 1) | e.head << 8, e.q0, e.rows, e.tile);
+      }
+      p.desc[cta] = todo;
+    }
   } else if (tid == 0) {
     p.desc[cta] = make_int4(0, 0, 0, 0);
   }
@@ -820,13 +829,17 @@ __global__ void __launch_bounds__(kMergeThreads) k_attend_merge(const AttArgs p)
   const int cta = blockIdx.x;
   const int4 d = __ldcg(p.desc + cta);
   if (!d.x) return;
-  const float* part = p.ws + ((size_t)cta * (kAttMaxWarps + 2) + kAttMaxWarps + 1) * kPart;
-  merge_parts<D, NT, true, 8>(p, [part, first = true]() mutable {
-    const float* now = part;
-    part += ((size_t)(kAttMaxWarps + 2) - (first ? 1 : 0)) * kPart;
-    first = false;
-    return now;
-  }, d.x & 255, threadIdx.x, kMergeThreads, nullptr, d.y, d.z, d.x >> 8, d.w);
+  const float* slot = p.ws + ((size_t)cta * (kAttMaxWarps + 2) + kAttMaxWarps + 1) * kPart;
+  for (int i = threadIdx.x; i < 8 * NT * (D / 4); i += kMergeThreads) {
+    const int row = i / (D / 4);
+    if (d.w * 8 * NT + row >= d.z) break;
+    const float* part = slot;
+    merge_row<D, NT, true, 8>(p, [&]() {
+      const float* now = part;
+      part += ((size_t)(kAttMaxWarps + 2) - (now == slot ? 1 : 0)) * kPart;
+      return now;
+    }, d.x & 255, row, i % (D / 4) * 4, nullptr, d.y, d.x >> 8, d.w);
+  }
 }
 
 size_t attention_workspace_bytes(int head_dim, int rows) {
