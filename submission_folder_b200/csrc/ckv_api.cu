@@ -7,6 +7,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -863,6 +864,11 @@ int ckv_device_accessible(const void* ptr, int32_t* accessible) {
 static bool aligned16(const void* p, int64_t s0, int64_t s1, int es) {
   return (uintptr_t)p % 16 == 0 && (s0 * es) % 16 == 0 && (s1 * es) % 16 == 0;
 }
+static bool aligned_to(size_t n, std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if ((uintptr_t)p % n) return false;
+  return true;
+}
 static bool known_dtype(int dtype) { return dtype == CKV_BF16 || dtype == CKV_FP16 || dtype == CKV_FP32; }
 
 static int check_cache(const ckv_cache* c) {
@@ -877,6 +883,7 @@ static int check_cache(const ckv_cache* c) {
   if (!aligned16(c->k, c->k_block_stride, c->k_head_stride, 1) || c->k_tok_stride % 16 ||
       !aligned16(c->v, c->v_block_stride, c->v_head_stride, 1) || c->v_tok_stride % 16)
     return fail(CKV_ERR_ARG, "cache pointers and strides must be multiples of 16 bytes");
+  if (!aligned_to(4, {c->k_scale, c->v_scale})) return fail(CKV_ERR_ARG, "scales must be aligned to 4 bytes");
   return CKV_OK;
 }
 
@@ -885,6 +892,10 @@ int ckv_block_tables(const ckv_table_step* s, ckv_stream_t stream) {
       !s->out_free_count || !s->out_cu || !s->out_granted || (s->total > 0 && (!s->out_slots || !s->out_positions)) ||
       (!s->work && (int64_t)s->requests + s->total > CKV_TABLES_SMALL))
     return fail(CKV_ERR_ARG, "null argument");
+  if (!aligned_to(4, {s->lens, s->new_tokens, s->shift, s->tables, s->free_list, s->free_count, s->out_lens, s->out_free_count,
+                      s->out_cu, s->out_granted, s->work}) ||
+      !aligned_to(8, {s->out_slots, s->out_positions}))
+    return fail(CKV_ERR_ARG, "pointers must be aligned to their elements");
   if (s->requests < 1 || s->requests > kMaxRequests) return fail(CKV_ERR_ARG, "1 to 8192 requests");
   if (s->total < 0 || s->table_width < 1 || s->table_stride < s->table_width || s->free_capacity < 0)
     return fail(CKV_ERR_ARG, "bad table geometry");
@@ -903,6 +914,8 @@ int ckv_rotary(const ckv_rotary_args* a, ckv_stream_t stream) {
   if (a->tokens == 0) return CKV_OK;
   if (!a->q || !a->out_q || !a->positions || !a->inv_freq || (a->k_heads > 0 && (!a->k || !a->out_k)))
     return fail(CKV_ERR_ARG, "null argument");
+  if (!aligned_to(8, {a->positions, a->inv_freq}) || !aligned_to(a->dtype == CKV_FP32 ? 4 : 2, {a->q, a->k, a->out_q, a->out_k}))
+    return fail(CKV_ERR_ARG, "pointers must be aligned to their elements");
   const cudaError_t e = launch_rotary(*a, (cudaStream_t)stream);
   return e == cudaSuccess ? CKV_OK : cuda_fail(e, "rotary");
 }
@@ -916,6 +929,7 @@ static int cache_rows(const ckv_cache* c, void* k, int64_t kts, int64_t khs, voi
   const int es = dtype == CKV_FP32 ? 4 : 2;
   if (!aligned16(k, kts, khs, es) || !aligned16(v, vts, vhs, es))
     return fail(CKV_ERR_ARG, "row pointers and strides must be 16-byte aligned (contiguous head_dim rows)");
+  if (!aligned_to(8, {slots})) return fail(CKV_ERR_ARG, "slots must be aligned to 8 bytes");
   r->k = k; r->kts = kts; r->khs = khs; r->v = v; r->vts = vts; r->vhs = vhs;
   r->dtype = dtype; r->slots = slots; r->tokens = tokens;
   return CKV_OK;
@@ -978,6 +992,7 @@ int ckv_cache_attention(const ckv_cache* cache, const ckv_attention_args* a, voi
   if (workspace_bytes < need) return fail(CKV_ERR_WORKSPACE, "workspace too small (see ckv_cache_attention_workspace)");
   if (a->requests == 0 || a->tokens == 0) return CKV_OK;
   if (!a->q || !a->out || !a->tables || !a->lens) return fail(CKV_ERR_ARG, "null argument");
+  if (!aligned_to(4, {a->tables, a->lens, a->cu, a->lse})) return fail(CKV_ERR_ARG, "pointers must be aligned to their elements");
   const cudaError_t e = launch_cache_attention(*cache, *a, workspace, (cudaStream_t)stream);
   return e == cudaSuccess ? CKV_OK : cuda_fail(e, "cache attention");
 }

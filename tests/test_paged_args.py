@@ -23,7 +23,7 @@ def _cache(**over):
 
 @pytest.mark.parametrize("over,code", [
     (dict(k=None), -1), (dict(v_scale=None), -1), (dict(format=2), -2), (dict(head_dim=96), -3), (dict(block_size=24), -3),
-    (dict(num_blocks=0), -1), (dict(num_kv_heads=0), -1), (dict(num_kv_heads=70000), -1), (dict(k=P + 8), -1),
+    (dict(num_blocks=0), -1), (dict(num_kv_heads=0), -1), (dict(num_kv_heads=40000), -1), (dict(k=P + 8), -1), (dict(k_scale=P + 2), -1),
     (dict(v_tok_stride=120), -1), (dict(k_head_stride=2056), -1)])
 def test_bad_caches_are_refused(over, code):
     lib, c = _lib.load(), _cache(**over)
@@ -44,6 +44,7 @@ def test_bad_rows_are_refused():
     assert lib.ckv_cache_write(ref, P + 2, 256, 128, P, 256, 128, 0, P, 3, None) == -1   # alignment
     assert lib.ckv_cache_write(ref, P, 250, 128, P, 256, 128, 0, P, 3, None) == -1
     assert lib.ckv_cache_read(ref, P, None, 0, P, 3, None) == -1
+    assert lib.ckv_cache_read(ref, P, P, 0, P + 4, 3, None) == -1                          # slots' alignment
     assert lib.ckv_cache_write(ref, None, 0, 0, None, 0, 0, 0, None, 0, None) == 0       # nothing to write
     assert lib.ckv_cache_read(None, P, P, 0, P, 3, None) == -1
 
@@ -51,7 +52,8 @@ def test_bad_rows_are_refused():
 @pytest.mark.parametrize("over,code", [
     (dict(q=None), -1), (dict(tables=None), -1), (dict(lens=None), -1), (dict(dtype=5), -2), (dict(q=P + 4), -1),
     (dict(out_tok_stride=1020), -1), (dict(q_heads=7), -1), (dict(max_q=0), -1), (dict(table_width=0), -1),
-    (dict(table_stride=3), -1), (dict(tokens=2), -1), (dict(requests=-1), -1), (dict(cu=P, max_q=1 << 20), -3)])
+    (dict(table_stride=3), -1), (dict(lens=P + 2), -1), (dict(requests=1 << 30, tokens=1 << 30, table_width=4096, table_stride=4096), -3),
+    (dict(tokens=2), -1), (dict(requests=-1), -1), (dict(cu=P, max_q=1 << 20), -3)])
 def test_bad_attention_is_refused(over, code):
     lib, c = _lib.load(), _cache()
     a = dict(q=P, q_tok_stride=1024, q_head_stride=128, out=P, out_tok_stride=1024, out_head_stride=128, tables=P, table_stride=4,
@@ -76,7 +78,7 @@ def test_attention_workspace_is_checked():
 
 @pytest.mark.parametrize("over", [dict(lens=None), dict(out_slots=None), dict(out_granted=None), dict(work=None, total=4096), dict(requests=0), dict(requests=8193),
                                   dict(total=-1), dict(table_width=0), dict(table_stride=1), dict(block_size=0),
-                                  dict(free_capacity=-1)])
+                                  dict(free_capacity=-1), dict(lens=P + 2), dict(out_slots=P + 4)])
 def test_bad_table_steps_are_refused(over):
     a = dict(lens=P, new_tokens=P, tables=P, table_stride=4, table_width=4, free_list=P, free_capacity=8, free_count=P,
              block_size=16, requests=2, total=2, out_lens=P, out_free_count=P, out_cu=P, out_slots=P, out_positions=P,
@@ -88,7 +90,8 @@ def test_bad_table_steps_are_refused(over):
 
 @pytest.mark.parametrize("over,code", [(dict(q=None), -1), (dict(k_heads=1), -1), (dict(dtype=3), -2), (dict(rotary_dim=0), -1),
                                        (dict(rotary_dim=7), -1), (dict(rotary_dim=66), -1), (dict(tokens=-1), -1),
-                                       (dict(q_heads=0), -1), (dict(head_dim=2048, rotary_dim=64), -1), (dict(tokens=0), 0)])
+                                       (dict(q_heads=0), -1), (dict(head_dim=2048, rotary_dim=64), -1), (dict(positions=P + 4), -1),
+                                       (dict(q=P + 1), -1), (dict(tokens=0), 0)])
 def test_bad_rotary_is_refused(over, code):
     a = dict(q=P, q_tok_stride=64, q_head_stride=64, out_q=P, out_q_tok_stride=64, out_q_head_stride=64, positions=P, inv_freq=P,
              factor=1.0, tokens=2, q_heads=1, k_heads=0, head_dim=64, rotary_dim=64, dtype=0)
