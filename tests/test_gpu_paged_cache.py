@@ -371,6 +371,27 @@ def test_cache_write_same_slot_twice_and_strided_rows(dev):
     _check_pool(pool, refs, dim)
 
 
+@pytest.mark.parametrize("before,times", [(0, 40), (0, 300), (1200, 300)])
+def test_cache_write_slots_named_again_and_again(dev, before, times):
+    """A run far longer than its block (each slot's last token stays), in a short list and in a long
+    one whose pieces it crosses; with the block's first place and without."""
+    block, dim, heads = 16, 64, 2
+    g = torch.Generator().manual_seed(times + before)
+    ids = torch.randperm(100, generator=g).tolist()
+    slots = [ids[2 + i // block] * block + i % block for i in range(before)]
+    for low in (1, 0):
+        slots += (ids[low] * block + torch.randint(low, block, (times,), generator=g)).tolist()
+    pool, refs = _pool(dev, 100, heads, block, dim, E4M3), [ref.RefCache(heads, block, E4M3) for _ in range(2)]
+    one = torch.ones(1, heads, dim)
+    ops.cache_write(one.to(dev), one.to(dev), *pool, torch.tensor([ids[1] * block], device=dev))
+    x = [torch.randn(len(slots), heads, dim, generator=g).bfloat16() for _ in range(2)]
+    ops.cache_write(x[0].to(dev), x[1].to(dev), *pool, torch.tensor(slots, device=dev))
+    for r, xx in zip(refs, x):
+        r.write(one.double(), [ids[1] * block])
+        r.write(xx.double(), slots)
+    _check_pool(pool, refs, dim)
+
+
 def test_cache_write_read_refusals(dev):
     pool = _pool(dev, 4, 2, 16, 64, E4M3)
     x, slots = torch.zeros(3, 2, 64, device=dev), torch.arange(3, device=dev)
