@@ -25,15 +25,10 @@ template <> CKV_DEV __half from_f32<__half>(float x) { return __float2half_rn(x)
 
 template <typename T, int N> struct alignas(sizeof(T) * N) Vec { T x[N]; };
 
-// A unit is 2N elements: N of the first half and their N partners (half layout), or 2N adjacent
-// ones (interleaved), or 2N past the rotated part (N at its end, where that is odd).
-template <typename T, int N, bool kInter>
-__global__ void __launch_bounds__(kRotThreads) k_rotary(const ckv_rotary_args a, int tokens_per_cta) {
-  extern __shared__ float2 rot_cs[];   // [tokens_per_cta][pairs]
+// Cosine and sine (times factor) of tokens t0 .. t0 + nt, [nt][pairs] in shared memory.
+CKV_DEV void turns_of(const ckv_rotary_args& a, int t0, int nt, float2* cs) {
   after_previous();
   const int pairs = a.rotary_dim / 2;
-  const int t0 = blockIdx.x * tokens_per_cta;
-  const int nt = min(tokens_per_cta, a.tokens - t0);
   for (int i = threadIdx.x; i < nt * pairs; i += kRotThreads) {
     const int t = i / pairs, p = i - t * pairs;
     const double turns = (double)a.positions[t0 + t] * (a.inv_freq[p] * 0.15915494309189533577);
@@ -42,9 +37,19 @@ __global__ void __launch_bounds__(kRotThreads) k_rotary(const ckv_rotary_args a,
     float s, c;
     sincospif(2.f * hi, &s, &c);
     const float c1 = fmaf(-lo, s, c), s1 = fmaf(lo, c, s);
-    rot_cs[i] = make_float2(c1 * a.factor, (a.inverse ? -s1 : s1) * a.factor);
+    cs[i] = make_float2(c1 * a.factor, (a.inverse ? -s1 : s1) * a.factor);
   }
   __syncthreads();
+}
+
+// A unit is 2N elements: N of the first half and their N partners (half layout), or 2N adjacent
+// ones (interleaved), or 2N past the rotated part (N at its end, where that is odd).
+template <typename T, int N, bool kInter>
+__global__ void __launch_bounds__(kRotThreads) k_rotary(const ckv_rotary_args a, int tokens_per_cta) {
+  extern __shared__ float2 rot_cs[];   // [tokens_per_cta][pairs]
+  const int t0 = blockIdx.x * tokens_per_cta;
+  const int pairs = a.rotary_dim / 2, nt = min(tokens_per_cta, a.tokens - t0);
+  turns_of(a, t0, nt, rot_cs);
   const int turn_units = pairs / N;                                   // per head
   const int rest_units = (a.head_dim - a.rotary_dim + 2 * N - 1) / (2 * N);
   const int units = turn_units + rest_units;
@@ -73,10 +78,6 @@ __global__ void __launch_bounds__(kRotThreads) k_rotary(const ckv_rotary_args a,
           const float c = cs[e].x, s = cs[e].y, p = to_f32(x.x[e]), q = to_f32(y.x[e]);
           ox.x[e] = from_f32<T>(p * c - q * s);
           oy.x[e] = from_f32<T>(q * c + p * s);
-        } else if constexpr (N == 1) {
-          const float c = cs[0].x, s = cs[0].y, p = to_f32(x.x[0]), q = to_f32(y.x[0]);
-          ox.x[0] = from_f32<T>(p * c - q * s);
-          oy.x[0] = from_f32<T>(q * c + p * s);
         } else if (e % 2 == 0) {
           const float c = cs[e / 2].x, s = cs[e / 2].y, p = to_f32(x.x[e]), q = to_f32(x.x[e + 1]);
           ox.x[e] = from_f32<T>(p * c - q * s);
@@ -98,10 +99,45 @@ __global__ void __launch_bounds__(kRotThreads) k_rotary(const ckv_rotary_args a,
   }
 }
 
+// Any dimensions, strides and alignment, element by element: a warp has a row (token, head) and its
+// lanes the pairs.  (8192 tokens of 40 heads, 122 of 128 dimensions: 112 us as units of the
+// kernel above with N = 1, whose every pair divides for its place.)
+template <typename T, bool kInter>
+__global__ void __launch_bounds__(kRotThreads) k_rotary_rows(const ckv_rotary_args a, int tokens_per_cta) {
+  extern __shared__ float2 rot_cs[];
+  const int t0 = blockIdx.x * tokens_per_cta;
+  const int pairs = a.rotary_dim / 2, nt = min(tokens_per_cta, a.tokens - t0);
+  turns_of(a, t0, nt, rot_cs);
+  const int h0 = blockIdx.y * a.heads_per_cta, nh = min(a.q_heads + a.k_heads - h0, a.heads_per_cta);
+  const int lane = threadIdx.x & 31;
+  for (int row = threadIdx.x >> 5; row < nt * nh; row += kRotThreads / 32) {
+    const int t = row / nh, h = h0 + row - t * nh;
+    const bool isk = h >= a.q_heads;
+    const int64_t tok = t0 + t;
+    const T* src = isk ? static_cast<const T*>(a.k) + tok * a.k_tok_stride + (h - a.q_heads) * a.k_head_stride
+                       : static_cast<const T*>(a.q) + tok * a.q_tok_stride + h * a.q_head_stride;
+    T* dst = isk ? static_cast<T*>(a.out_k) + tok * a.out_k_tok_stride + (h - a.q_heads) * a.out_k_head_stride
+                 : static_cast<T*>(a.out_q) + tok * a.out_q_tok_stride + h * a.out_q_head_stride;
+    const float2* cs = rot_cs + t * pairs;
+#pragma unroll 2
+    for (int p = lane; p < pairs; p += 32) {
+      const int i0 = kInter ? 2 * p : p, i1 = kInter ? i0 + 1 : p + pairs;
+      const float x = to_f32(src[i0]), y = to_f32(src[i1]);
+      dst[i0] = from_f32<T>(x * cs[p].x - y * cs[p].y);
+      dst[i1] = from_f32<T>(y * cs[p].x + x * cs[p].y);
+    }
+    if (src != dst)
+      for (int d = a.rotary_dim + lane; d < a.head_dim; d += 32) dst[d] = src[d];
+  }
+}
+
 template <typename T, int N>
 static cudaError_t rot_launch(const ckv_rotary_args& a, int tpc, dim3 grid, cudaStream_t st) {
   const size_t smem = (size_t)tpc * (a.rotary_dim / 2) * sizeof(float2);
-  return launch_after(a.interleaved ? k_rotary<T, N, true> : k_rotary<T, N, false>, grid, kRotThreads, smem, st, a, tpc);
+  if constexpr (N == 1)
+    return launch_after(a.interleaved ? k_rotary_rows<T, true> : k_rotary_rows<T, false>, grid, kRotThreads, smem, st, a, tpc);
+  else
+    return launch_after(a.interleaved ? k_rotary<T, N, true> : k_rotary<T, N, false>, grid, kRotThreads, smem, st, a, tpc);
 }
 
 cudaError_t launch_rotary(const ckv_rotary_args& args, cudaStream_t st) {
