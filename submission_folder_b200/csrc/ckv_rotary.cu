@@ -11,6 +11,8 @@
 // computed once per token and shared by all heads through shared memory.
 //
 // Bound: HBM (each element read once and written once).
+#include <algorithm>
+
 #include "ckv_cache.h"
 #include "ckv_common.cuh"
 
@@ -99,26 +101,31 @@ __global__ void __launch_bounds__(kRotThreads) k_rotary(const ckv_rotary_args a,
   }
 }
 
-// Any dimensions, strides and alignment, element by element: a warp has a row (token, head) and its
-// lanes the pairs.  (8192 tokens of 40 heads, 122 of 128 dimensions: 112 us as units of the
-// kernel above with N = 1, whose every pair divides for its place.)
-template <typename T, bool kInter>
-__global__ void __launch_bounds__(kRotThreads) k_rotary_rows(const ckv_rotary_args a, int tokens_per_cta) {
+// Any rotary dimension, element by element: a warp has a row (token, head) and its lanes the pairs.
+// kStaged: 16-bit rows that start on 16 bytes go through shared memory, read and written in 16-byte
+// pieces, a few rows at a time; otherwise any alignment.  (8192 tokens of 40 heads, 122 of 128
+// dimensions in bf16: 112 us as units of the kernel above with N = 1, 90 by rows, 82 staged; fp32, 58 of
+// 64: 60, 55, 65.)
+template <typename T, bool kInter, bool kStaged>
+__global__ void __launch_bounds__(kRotThreads) k_rotary_rows(const ckv_rotary_args a, int tokens_per_cta, int batch) {
   extern __shared__ float2 rot_cs[];
   const int t0 = blockIdx.x * tokens_per_cta;
   const int pairs = a.rotary_dim / 2, nt = min(tokens_per_cta, a.tokens - t0);
   turns_of(a, t0, nt, rot_cs);
   const int h0 = blockIdx.y * a.heads_per_cta, nh = min(a.q_heads + a.k_heads - h0, a.heads_per_cta);
-  const int lane = threadIdx.x & 31;
-  for (int row = threadIdx.x >> 5; row < nt * nh; row += kRotThreads / 32) {
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  auto home = [&](int row, const T*& src, T*& dst) {
     const int t = row / nh, h = h0 + row - t * nh;
-    const bool isk = h >= a.q_heads;
     const int64_t tok = t0 + t;
-    const T* src = isk ? static_cast<const T*>(a.k) + tok * a.k_tok_stride + (h - a.q_heads) * a.k_head_stride
-                       : static_cast<const T*>(a.q) + tok * a.q_tok_stride + h * a.q_head_stride;
-    T* dst = isk ? static_cast<T*>(a.out_k) + tok * a.out_k_tok_stride + (h - a.q_heads) * a.out_k_head_stride
-                 : static_cast<T*>(a.out_q) + tok * a.out_q_tok_stride + h * a.out_q_head_stride;
-    const float2* cs = rot_cs + t * pairs;
+    if (h >= a.q_heads) {
+      src = static_cast<const T*>(a.k) + tok * a.k_tok_stride + (h - a.q_heads) * a.k_head_stride;
+      dst = static_cast<T*>(a.out_k) + tok * a.out_k_tok_stride + (h - a.q_heads) * a.out_k_head_stride;
+    } else {
+      src = static_cast<const T*>(a.q) + tok * a.q_tok_stride + h * a.q_head_stride;
+      dst = static_cast<T*>(a.out_q) + tok * a.out_q_tok_stride + h * a.out_q_head_stride;
+    }
+  };
+  auto turn = [&](const T* src, T* dst, const float2* cs) {
 #pragma unroll 2
     for (int p = lane; p < pairs; p += 32) {
       const int i0 = kInter ? 2 * p : p, i1 = kInter ? i0 + 1 : p + pairs;
@@ -126,18 +133,57 @@ __global__ void __launch_bounds__(kRotThreads) k_rotary_rows(const ckv_rotary_ar
       dst[i0] = from_f32<T>(x * cs[p].x - y * cs[p].y);
       dst[i1] = from_f32<T>(y * cs[p].x + x * cs[p].y);
     }
-    if (src != dst)
-      for (int d = a.rotary_dim + lane; d < a.head_dim; d += 32) dst[d] = src[d];
+  };
+  const T* src;
+  T* dst;
+  if constexpr (kStaged) {
+    const int vecs = a.head_dim * (int)sizeof(T) / 16;   // of a row
+    uint4* stage = reinterpret_cast<uint4*>(rot_cs + ((tokens_per_cta * pairs + 1) & ~1)) + wid * batch * vecs;
+    for (int row0 = wid * batch; row0 < nt * nh; row0 += kRotThreads / 32 * batch) {
+      const int rows = min(batch, nt * nh - row0);
+      for (int v = lane; v < rows * vecs; v += 32) {
+        const int r = v / vecs;
+        home(row0 + r, src, dst);
+        stage[v] = reinterpret_cast<const uint4*>(src)[v - r * vecs];
+      }
+      __syncwarp();
+      for (int r = 0; r < rows; ++r) {
+        T* x = reinterpret_cast<T*>(stage + r * vecs);
+        turn(x, x, rot_cs + (row0 + r) / nh * pairs);
+      }
+      __syncwarp();
+      for (int v = lane; v < rows * vecs; v += 32) {
+        const int r = v / vecs;
+        home(row0 + r, src, dst);
+        reinterpret_cast<uint4*>(dst)[v - r * vecs] = stage[v];
+      }
+      __syncwarp();
+    }
+  } else {
+    for (int row = wid; row < nt * nh; row += kRotThreads / 32) {
+      home(row, src, dst);
+      turn(src, dst, rot_cs + row / nh * pairs);
+      if (src != dst)
+        for (int d = a.rotary_dim + lane; d < a.head_dim; d += 32) dst[d] = src[d];
+    }
   }
 }
 
 template <typename T, int N>
-static cudaError_t rot_launch(const ckv_rotary_args& a, int tpc, dim3 grid, cudaStream_t st) {
-  const size_t smem = (size_t)tpc * (a.rotary_dim / 2) * sizeof(float2);
-  if constexpr (N == 1)
-    return launch_after(a.interleaved ? k_rotary_rows<T, true> : k_rotary_rows<T, false>, grid, kRotThreads, smem, st, a, tpc);
-  else
-    return launch_after(a.interleaved ? k_rotary<T, N, true> : k_rotary<T, N, false>, grid, kRotThreads, smem, st, a, tpc);
+static cudaError_t rot_launch(const ckv_rotary_args& a, int tpc, dim3 grid, bool rows16, cudaStream_t st) {
+  const size_t table = ((size_t)tpc * (a.rotary_dim / 2) + 1) / 2 * 2 * sizeof(float2);
+  if constexpr (N > 1) {
+    return launch_after(a.interleaved ? k_rotary<T, N, true> : k_rotary<T, N, false>, grid, kRotThreads, table, st, a, tpc);
+  } else if (rows16 && sizeof(T) == 2) {
+    const int row = a.head_dim * (int)sizeof(T), batch = std::max(1, 1024 / row);   // 1 KB per warp in flight
+    const size_t smem = table + (size_t)(kRotThreads / 32) * batch * row;
+    auto fn = a.interleaved ? k_rotary_rows<T, true, true> : k_rotary_rows<T, false, true>;
+    if (cudaError_t e = ensure_dynamic_smem((const void*)fn, smem); e != cudaSuccess) return e;
+    return launch_after(fn, grid, kRotThreads, smem, st, a, tpc, batch);
+  } else {
+    return launch_after(a.interleaved ? k_rotary_rows<T, true, false> : k_rotary_rows<T, false, false>, grid, kRotThreads, table, st,
+                        a, tpc, 1);
+  }
 }
 
 cudaError_t launch_rotary(const ckv_rotary_args& args, cudaStream_t st) {
@@ -148,19 +194,20 @@ cudaError_t launch_rotary(const ckv_rotary_args& args, cudaStream_t st) {
   auto al = [&](const void* p, int64_t ts, int64_t hs) {
     return (uintptr_t)p % 16 == 0 && (ts * es) % 16 == 0 && (hs * es) % 16 == 0;
   };
-  const bool vec = al(a.q, a.q_tok_stride, a.q_head_stride) && al(a.out_q, a.out_q_tok_stride, a.out_q_head_stride) &&
+  const bool rows16 = al(a.q, a.q_tok_stride, a.q_head_stride) && al(a.out_q, a.out_q_tok_stride, a.out_q_head_stride) &&
                    (a.k_heads == 0 || (al(a.k, a.k_tok_stride, a.k_head_stride) &&
                                        al(a.out_k, a.out_k_tok_stride, a.out_k_head_stride))) &&
-                   (a.rotary_dim / 2) % n == 0 && a.head_dim % n == 0;
+                      a.head_dim % n == 0;
+  const bool vec = rows16 && (a.rotary_dim / 2) % n == 0;
   // few tokens: one per CTA and the heads spread over CTAs (latency); many: four per CTA
   const int tpc = a.tokens >= 1024 ? 4 : 1;
   const int splits = a.tokens >= 1024 ? 1 : (a.tokens >= 148 ? 2 : 8);
   a.heads_per_cta = (heads + splits - 1) / splits;
   const dim3 grid((a.tokens + tpc - 1) / tpc, (heads + a.heads_per_cta - 1) / a.heads_per_cta);
   switch (a.dtype) {
-    case CKV_BF16: return vec ? rot_launch<__nv_bfloat16, 8>(a, tpc, grid, st) : rot_launch<__nv_bfloat16, 1>(a, tpc, grid, st);
-    case CKV_FP16: return vec ? rot_launch<__half, 8>(a, tpc, grid, st) : rot_launch<__half, 1>(a, tpc, grid, st);
-    default: return vec ? rot_launch<float, 4>(a, tpc, grid, st) : rot_launch<float, 1>(a, tpc, grid, st);
+    case CKV_BF16: return vec ? rot_launch<__nv_bfloat16, 8>(a, tpc, grid, rows16, st) : rot_launch<__nv_bfloat16, 1>(a, tpc, grid, rows16, st);
+    case CKV_FP16: return vec ? rot_launch<__half, 8>(a, tpc, grid, rows16, st) : rot_launch<__half, 1>(a, tpc, grid, rows16, st);
+    default: return vec ? rot_launch<float, 4>(a, tpc, grid, rows16, st) : rot_launch<float, 1>(a, tpc, grid, rows16, st);
   }
 }
 
