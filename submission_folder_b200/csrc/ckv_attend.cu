@@ -46,7 +46,12 @@ constexpr float kTop = 9.f;       // and stand at 2^kTop there: at most 2^15 in 
 // Warps and ring stages of a CTA: 12 x 2 steps of 8 KB where the registers allow 12 warps
 // (8 query rows in one term), else 8 x 3.
 __host__ __device__ constexpr int att_warps(int nt, int terms) { return nt * terms == 1 ? 12 : 8; }
-__host__ __device__ constexpr int att_stages(int nt, int terms) { return nt * terms == 1 ? 2 : 3; }
+__host__ __device__ constexpr int att_stages(int nt, int terms) { return nt * terms == 1 || nt * terms == 4 ? 2 : 3; }
+// Two row tiles in two terms: the query rows (64 registers) stand in shared memory instead.
+__host__ __device__ constexpr bool att_queries_shared(int nt, int terms) { return nt * terms == 4; }
+__host__ __device__ constexpr int att_query_bytes(int nt, int terms, int D) {
+  return att_queries_shared(nt, terms) ? nt * terms * (D / 16) * 32 * 8 : 0;   // per warp
+}
 
 struct AttArgs {
   ckv_cache c;
@@ -426,7 +431,9 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
         }
       };
 
-      uint32_t qf[NT][kTerms][kSteps16][2];
+      constexpr bool kShared = att_queries_shared(NT, kTerms);
+      uint32_t qf[kShared ? 1 : NT][kShared ? 1 : kTerms][kShared ? 1 : kSteps16][2];
+      const uint32_t qf_a = smem_u32(att_smem) + kWarps * kRing + wid * att_query_bytes(NT, kTerms, D) + lane * 16;
       float qs[NT][2];        // rows 2t, 2t + 1: scale * log2 e * the row's power of two
       int see[NT][2];         // tokens that they see
       int see_min = n;
@@ -493,8 +500,19 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
               qf[nt][0][k][0] = to_half(w[k].x);
               qf[nt][0][k][1] = to_half(w[k].y);
             } else {
-              split2(x[k].x * up, x[k].y * up, qf[nt][0][k][0], qf[nt][1][k][0]);
-              split2(x[k].z * up, x[k].w * up, qf[nt][0][k][1], qf[nt][1][k][1]);
+              uint32_t f[2][2];   // [term][pair]
+              split2(x[k].x * up, x[k].y * up, f[0][0], f[1][0]);
+              split2(x[k].z * up, x[k].w * up, f[0][1], f[1][1]);
+              if constexpr (kShared) {
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(qf_a + (k * NT + nt) * 512), "r"(f[0][0]),
+                             "r"(f[0][1]), "r"(f[1][0]), "r"(f[1][1]) : "memory");
+              } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  qf[nt][0][k][i] = f[0][i];
+                  qf[nt][1][k][i] = f[1][i];
+                }
+              }
             }
           }
         }
@@ -545,6 +563,17 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
               codes4<kFmt>(e == 0 ? w[u][0].x : e == 1 ? w[u][0].y : e == 2 ? w[u][0].z : w[u][0].w, a[u][0], a[u][2]);
               codes4<kFmt>(e == 0 ? w[u][1].x : e == 1 ? w[u][1].y : e == 2 ? w[u][1].z : w[u][1].w, a[u][1], a[u][3]);
             }
+            uint32_t b[NT][kTerms][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if constexpr (kShared) {
+                const uint4 v = lds4(qf_a + ((c * 4 + e) * NT + nt) * 512);
+                b[nt][0][0] = v.x; b[nt][0][1] = v.y; b[nt][1][0] = v.z; b[nt][1][1] = v.w;
+              } else {
+#pragma unroll
+                for (int k = 0; k < kTerms; ++k) { b[nt][k][0] = qf[nt][k][c * 4 + e][0]; b[nt][k][1] = qf[nt][k][c * 4 + e][1]; }
+              }
+            }
             // the sums of the 16-token halves and the row tiles are independent: they take turns
 #pragma unroll
             for (int k = 0; k < kTerms; ++k)
@@ -552,9 +581,8 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                  const uint32_t(&b)[2] = qf[nt][k][c * 4 + e];
-                  if (c == 0 && e == 0 && k == 0) mma16816_zero(sc[nt][u], a[u], b[0], b[1]);
-                  else mma16816(sc[nt][u], a[u], b[0], b[1]);
+                  if (c == 0 && e == 0 && k == 0) mma16816_zero(sc[nt][u], a[u], b[nt][k][0], b[nt][k][1]);
+                  else mma16816(sc[nt][u], a[u], b[nt][k][0], b[nt][k][1]);
                 }
           }
         }
@@ -849,7 +877,7 @@ size_t attention_workspace_bytes(int head_dim, int rows) {
 
 template <int D, int kFmt, int NT, int kTerms>
 static cudaError_t att_launch(AttArgs& p, void* ws, cudaStream_t st) {
-  constexpr size_t smem = (size_t)att_warps(NT, kTerms) * att_stages(NT, kTerms) * 2 * kAttStep * D;
+  constexpr size_t smem = (size_t)att_warps(NT, kTerms) * (att_stages(NT, kTerms) * 2 * kAttStep * D + att_query_bytes(NT, kTerms, D));
   static_assert(att_stages(NT, kTerms) * 2 * kAttStep * D >= part_floats(D, 8 * NT) * 4, "a warp's ring holds one partial result");
   static_assert(att_warps(NT, kTerms) <= kAttMaxWarps, "workspace slots");
   p.ws = static_cast<float*>(ws);
