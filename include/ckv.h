@@ -383,7 +383,9 @@ int ckv_gather(const ckv_layer* layer, int32_t window, const int32_t* idx, int32
  * torch cache).  A layer's keys and values live in blocks of block_size tokens of a pool,
  * as 8-bit codes with one fp32 scale per (block, KV head); value = code * scale.  Scales are
  * powers of two: the smallest (2^-126 at least) with max |x| / scale <= 448 (e4m3) or 127
- * (int8), or NaN when the block holds a NaN or an infinity.
+ * (int8), or NaN when the block holds a NaN or an infinity.  Reading and attention take any
+ * positive normal scales, as another program may leave them.  A NaN among e4m3 codes
+ * (ckv_cache_write writes none) reads as one, and reaches all new tokens of its sequence.
  * Slot of a token: block * block_size + its place in the block.
  */
 enum ckv_cache_format { CKV_CACHE_E4M3 = 0, CKV_CACHE_INT8 = 1 };
@@ -423,7 +425,7 @@ typedef struct ckv_table_step {
   int32_t free_capacity;
   const int32_t* free_count;
   int32_t block_size;
-  int32_t requests;            /* at most 8192 */
+  int32_t requests;            /* at most 8192, and requests * table_width less than 2^31 */
   int32_t total;               /* length of out_slots and out_positions */
   int32_t* out_lens;
   int32_t* out_free_count;

@@ -158,6 +158,7 @@ class PagedKVCache:
         total = self.lens.shape[0] * max_q if total is None else int(total)
         t = ops.block_tables(self.lens, new, self.tables, self.free_list, self.free_count, self.block_size, total,
                              shift=self.shift)
+        self.shift.mul_(new >= 0)       # the row's next request begins at position 0
         return CacheStep(t, int(max_q))
 
     def write(self, layer_idx: int, key_states: torch.Tensor, value_states: torch.Tensor, step: CacheStep) -> None:
@@ -201,13 +202,15 @@ class PagedKVCache:
         new = torch.zeros_like(self.lens)
         new[request] = kept
         step = self.step(new, total=kept, max_q=kept)
-        self.shift[request] = seen - kept
+        self.shift[request] = torch.where(step.tables.granted[request] == kept, seen - kept, self.shift[request])
         for i, (k, v) in enumerate(rows):
             self.write(i, k, v, step)
         return step
 
     def slots(self, request: int, tokens: int) -> torch.Tensor:
         """Slots of the first ``tokens`` tokens of a request (int64 ``[tokens]``)."""
+        if not 0 <= tokens <= self.tables.shape[1] * self.block_size:
+            raise ValueError(f"a request holds at most {self.tables.shape[1] * self.block_size} tokens, got {tokens}")
         at = torch.arange(tokens, device=self.lens.device)
         return self.tables[request].long()[at // self.block_size] * self.block_size + at % self.block_size
 

@@ -899,6 +899,8 @@ int ckv_block_tables(const ckv_table_step* s, ckv_stream_t stream) {
   if (s->requests < 1 || s->requests > kMaxRequests) return fail(CKV_ERR_ARG, "1 to 8192 requests");
   if (s->total < 0 || s->table_width < 1 || s->table_stride < s->table_width || s->free_capacity < 0)
     return fail(CKV_ERR_ARG, "bad table geometry");
+  if ((int64_t)s->requests * s->table_width > INT32_MAX)   // blocks are counted in 32 bits
+    return fail(CKV_ERR_UNSUPPORTED, "requests * table_width too large");
   if (s->block_size < 1) return fail(CKV_ERR_ARG, "block_size must be at least 1");
   const cudaError_t e = launch_block_tables(*s, (cudaStream_t)stream);
   return e == cudaSuccess ? CKV_OK : cuda_fail(e, "block tables");

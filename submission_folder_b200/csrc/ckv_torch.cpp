@@ -37,6 +37,8 @@ bool grad(const Tensor* t) { return t && t->requires_grad() && at::GradMode::is_
 bool table(const Tensor* t, int device) {
   return on(t, device) && t->scalar_type() == at::kInt && t->dim() == 2 && t->stride(1) == 1;
 }
+// Of the rows of a table; of a single row, whatever it is, at least the row.
+int64_t table_stride(const Tensor* t) { return t->size(0) > 1 ? t->stride(0) : std::max(t->stride(0), t->size(1)); }
 bool fits(int64_t x) { return x >= 0 && x <= INT32_MAX; }
 template <typename T> T* ptr(const Tensor* t) { return t ? static_cast<T*>(t->data_ptr()) : nullptr; }
 
@@ -95,7 +97,7 @@ CKV_FN(block_tables) {
   if (R + total > CKV_TABLES_SMALL) work = at::empty({3 * R + 4}, i32);
   const int64_t width = tables->size(1);
   const ckv_table_step s = {ptr<int32_t>(lens), ptr<int32_t>(fresh), ptr<int32_t>(shift), ptr<int32_t>(tables),
-                            std::max(tables->stride(0), width), (int32_t)width, ptr<int32_t>(list), (int32_t)list->numel(),
+                            table_stride(tables), (int32_t)width, ptr<int32_t>(list), (int32_t)list->numel(),
                             ptr<int32_t>(count), (int32_t)block, (int32_t)R, (int32_t)total, ptr<int32_t>(lens_out),
                             ptr<int32_t>(count_out), ptr<int32_t>(&cu), ptr<int64_t>(&slots), ptr<int64_t>(&positions),
                             ptr<int32_t>(&granted), work.defined() ? ptr<int32_t>(&work) : nullptr};
@@ -241,7 +243,7 @@ CKV_FN(cache_attention) {
   r.q = q->data_ptr(); r.q_tok_stride = q->stride(0); r.q_head_stride = q->stride(1);
   r.out = out.data_ptr(); r.out_tok_stride = out.stride(0); r.out_head_stride = out.stride(1);
   r.lse = want_lse ? ptr<float>(&lse) : nullptr;
-  r.tables = ptr<int32_t>(tables); r.table_stride = std::max(tables->stride(0), tables->size(1));
+  r.tables = ptr<int32_t>(tables); r.table_stride = table_stride(tables);
   r.table_width = (int32_t)tables->size(1);
   r.lens = ptr<int32_t>(lens); r.cu = ptr<int32_t>(cu);
   r.requests = (int32_t)R; r.tokens = (int32_t)T; r.max_q = (int32_t)max_q; r.q_heads = (int32_t)H;

@@ -126,6 +126,10 @@ def test_block_tables_refusals(dev):
                            ("shift", torch.zeros(3, dtype=torch.int64, device=dev), ValueError)]:
         with pytest.raises(err):
             ops.block_tables(**{**a, name: bad})
+    with pytest.raises(RuntimeError, match="geometry"):
+        ops.block_tables(**{**a, "tables": torch.zeros(1, 2, **i32).expand(3, 2)})
+    one = {x: a[x][:1] for x in ("lens", "new", "tables")}
+    assert ops.block_tables(**{**a, **one, "total": 1}).granted.tolist() == [1]     # a single row has any stride
     big = torch.zeros(8193, **i32)
     with pytest.raises(RuntimeError, match="8192"):
         ops.block_tables(big, big, torch.zeros(8193, 1, **i32), a["free_list"], a["free_count"], 16, 0)
@@ -525,6 +529,20 @@ def test_attention_value_scales_far_apart(dev):
     _attention_check(out, lse, q, k, v, lens, [1] * 2, 64 ** -0.5, True)
 
 
+@pytest.mark.parametrize("times_k,times_v", [(1.0, 2.0 ** -115), (1.0, 2.0 ** 118), (1.3, 1.7), (0.7, 1.1 * 2.0 ** -100)])
+def test_attention_scales_of_other_programs(dev, times_k, times_v):
+    """Value scales at both ends of the normal range, and scales that are no powers of two: their
+    logarithm is off by 2^-22 at most, their products with the codes by 2^-24, of the 2^-19 allowed."""
+    lens = [300, 64]
+    pool, tables, n, q, k, v = _attention_case(dev, lens, 2, 4, 128, 32, INT8, torch.float32, [1] * 2)
+    pool[2].mul_(times_k)
+    pool[3].mul_(times_v)
+    used = pool[3][torch.isfinite(pool[3])]
+    assert used.min() >= 2.0 ** -126 and torch.isfinite(used * 127).all()
+    out, lse = ops.cache_attention(q, *pool, tables, n, want_lse=True)
+    _attention_check(out, lse, q, k * times_k, v * times_v, lens, [1] * 2, 128 ** -0.5, True)
+
+
 def test_attention_nan_and_bad_pages(dev):
     """A NaN block reaches the rows that see it and no others; a table entry outside the pool reads as
     NaN; queries with a NaN or an infinity stay in their row."""
@@ -705,6 +723,8 @@ def test_attention_refusals(dev):
                         (dict(cu=cu, max_q=1 << 20), RuntimeError)]:
         with pytest.raises(err):
             ops.cache_attention(**{**ok, **change})
+    with pytest.raises(RuntimeError, match="geometry"):      # one row for all requests
+        ops.cache_attention(**{**ok, "tables": tables[:1].expand(2, -1)})
     e = torch.empty(0, dtype=torch.int32, device=dev)
     assert ops.cache_attention(q[:0], *pool, tables[:0], e).shape == (0, 4, 64)
 
@@ -824,6 +844,27 @@ def test_captured_decode_step(dev):
                     (caches[1].k, caches[1].lens, caches[1].tables, caches[1].free_count)):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
     del graph
+
+
+def test_positions_of_a_row_that_is_used_again(dev):
+    """A request ends after evictions; the next one of its row begins at position 0, and one that
+    is refused leaves nothing behind."""
+    c = PagedKVCache(1, 8, 2, 64, 2, 64, 16, device=dev)
+    z = torch.zeros(1, 2, 20, 64, dtype=torch.bfloat16, device=dev)
+    new = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)   # noqa: E731
+    c.admit(0, [(z, z)], 500)
+    c.admit(1, [(z, z)], 300)
+    assert c.step(new(1, 1)).tables.positions.tolist() == [500, 300]
+    c.step(new(-1, 0))
+    assert c.step(new(1, 1)).tables.positions.tolist() == [0, 301]
+    c.step(new(-1, 1))
+    big = z.repeat(1, 1, 4, 1)
+    step = c.admit(0, [(big, big)], 900)                        # 80 tokens, 64 fit the row
+    assert int(step.tables.granted[0]) == 0
+    assert c.step(new(2, 1), total=3).tables.positions.tolist() == [0, 1, 303]
+    with pytest.raises(ValueError):
+        c.read(0, 0, 65)
+    assert c.read(0, 0, 64)[0].shape == (1, 2, 64, 64) and c.read(0, 1, 0)[0].shape == (1, 2, 0, 64)
 
 
 def test_paged_cache_class_refusals(dev):

@@ -88,6 +88,21 @@ def test_bad_table_steps_are_refused(over):
     assert _lib.load().ckv_block_tables(ctypes.byref(s), None) == -1
 
 
+def test_tables_of_more_blocks_than_32_bits_count_are_refused():
+    s = _lib.TableStep(lens=P, new_tokens=P, tables=P, table_stride=1 << 20, table_width=1 << 20, free_list=P, free_capacity=8,
+                       free_count=P, block_size=16, requests=2048, total=2, out_lens=P, out_free_count=P, out_cu=P, out_slots=P,
+                       out_positions=P, out_granted=P, work=P)
+    assert _lib.load().ckv_block_tables(ctypes.byref(s), None) == -3
+
+
+def test_slots_past_a_row_are_refused():
+    c = PagedKVCache(1, 8, 2, 60, 2, 64, 16, device="cpu")
+    assert c.slots(1, 64).tolist() == [i % 16 for i in range(64)]       # a table of zeros
+    for tokens in (65, -1):
+        with pytest.raises(ValueError, match="at most 64"):
+            c.slots(1, tokens)
+
+
 @pytest.mark.parametrize("over,code", [(dict(q=None), -1), (dict(k_heads=1), -1), (dict(dtype=3), -2), (dict(rotary_dim=0), -1),
                                        (dict(rotary_dim=7), -1), (dict(rotary_dim=66), -1), (dict(tokens=-1), -1),
                                        (dict(q_heads=0), -1), (dict(head_dim=2048, rotary_dim=64), -1), (dict(positions=P + 4), -1),
