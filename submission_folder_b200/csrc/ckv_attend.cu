@@ -31,9 +31,9 @@
 // ascending order: no atomics, and the same bits every time.
 //
 // Bound: HBM (each code is read once) for large batches: 32 sequences of up to 32768 tokens, 8 of
-// 32 heads of 128 in bf16: 187 us, 6.1 TB/s.  One sequence of 131072 tokens: 52 us with one bf16 query
-// (5.1 TB/s), 60 us with four (two row tiles); 84 us with four fp32 queries, where the two terms'
-// products and their sums bound it.  One sequence of 512: 9.4 us, launches and the merges.
+// 32 heads of 128 in bf16: 187 us, 6.1 TB/s.  One sequence of 131072 tokens: 50 us with one bf16 query
+// (5.4 TB/s), 57 us with four (two row tiles); 80 us with four fp32 queries, where the two terms'
+// products and their sums bound it.  One sequence of 512: 9.2 us, launches and the merges.
 #include "ckv_cache.h"
 #include "ckv_common.cuh"
 
@@ -52,7 +52,7 @@ constexpr float kTop = 9.f;       // and stand at 2^kTop there: at most 2^15 in 
 __host__ __device__ constexpr int att_warps(int nt, int terms) { return nt * terms == 1 ? 12 : 8; }
 __host__ __device__ constexpr int att_stages(int nt, int terms) { return nt * terms == 1 || nt * terms == 4 ? 2 : 3; }
 // Two row tiles in two terms: the query rows (64 registers) stand in shared memory instead, so
-// that nothing spills (131072 tokens x 4 fp32 queries: 91 -> 87 us).
+// that little spills (131072 tokens x 4 fp32 queries: 91 -> 87 us).
 __host__ __device__ constexpr bool att_queries_shared(int nt, int terms) { return nt * terms == 4; }
 __host__ __device__ constexpr int att_query_bytes(int nt, int terms, int D) {
   return att_queries_shared(nt, terms) ? nt * terms * (D / 16) * 32 * 8 : 0;   // per warp
@@ -238,53 +238,36 @@ CKV_DEV float4 row_out(float m, float mw, float l, float4 o) {
 }
 CKV_DEV float row_lse(float m, float l) { return l > 0.f || isnan(l) ? (m + log2f(l)) * kLn2 : -INFINITY; }
 
-// Merge of `count` partial results of one unit, next() their places in turn: four dimensions, from d
-// on, of row `row` of the unit, to the output or to `dst`.  kBatch parts are read at a time.  kL2:
-// other CTAs' results, read from L2.
-template <int D, int NT, bool kL2, int kBatch, typename F>
-CKV_DEV void merge_row(const AttArgs& p, F next, int count, int row, int d, float* dst, int q0, int head, int tile) {
-  auto get4 = [](const float* x) {
-    return kL2 ? __ldcg(reinterpret_cast<const float4*>(x)) : *reinterpret_cast<const float4*>(x);
-  };
+// A row's running references and sum, and four of its dimensions.
+struct RowSum {
   float m = kNone, mw = kNone, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k = 0; k < count; k += kBatch) {
-    float4 s[kBatch], x[kBatch];
+};
+// Joined by partial results: s their (m, m', l, -), x their sums.
+template <int N> CKV_DEV void join(RowSum& a, const float4 (&s)[N], const float4 (&x)[N]) {
+  float nm = a.m, nw = a.mw;
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      s[j] = make_float4(kNone, kNone, 0.f, 0.f);
-      x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (k + j < count) {
-        const float* q = next();
-        s[j] = get4(q + row * 4);
-        x[j] = get4(q + 8 * NT * 4 + row * D + d);
-      }
-    }
-    float nm = m, nw = mw;
+  for (int j = 0; j < N; ++j) { nm = fmaxf(nm, s[j].x); nw = fmaxf(nw, s[j].y); }
+  a.l *= ex2(a.m - nm);
+  const float f0 = ex2(a.mw - nw);
+  a.o.x *= f0; a.o.y *= f0; a.o.z *= f0; a.o.w *= f0;
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) { nm = fmaxf(nm, s[j].x); nw = fmaxf(nw, s[j].y); }
-    l *= ex2(m - nm);
-    const float f0 = ex2(mw - nw);
-    o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      l += s[j].z * ex2(s[j].x - nm);
-      const float f = ex2(s[j].y - nw);
-      o.x += x[j].x * f; o.y += x[j].y * f; o.z += x[j].z * f; o.w += x[j].w * f;
-    }
-    m = nm;
-    mw = nw;
+  for (int j = 0; j < N; ++j) {
+    a.l += s[j].z * ex2(s[j].x - nm);
+    const float f = ex2(s[j].y - nw);
+    a.o.x += x[j].x * f; a.o.y += x[j].y * f; a.o.z += x[j].z * f; a.o.w += x[j].w * f;
   }
-  if (dst) {
-    if (d == 0) *reinterpret_cast<float4*>(dst + row * 4) = make_float4(m, mw, l, 0.f);
-    *reinterpret_cast<float4*>(dst + 8 * NT * 4 + row * D + d) = o;
-  } else {
-    int64_t at, lat;
-    row_home(p, q0, head, tile * 8 * NT + row, at, lat);
-    store_out4(p.a.out, p.a.dtype, at + d, row_out(m, mw, l, o));
-    if (p.a.lse && d == 0) p.a.lse[lat] = row_lse(m, l);
-  }
+  a.m = nm;
+  a.mw = nw;
 }
+// Four dimensions, from d on, of row rho of a sequence and head, to the output.
+CKV_DEV void store_row(const AttArgs& p, const RowSum& a, int q0, int head, int rho, int d) {
+  int64_t at, lat;
+  row_home(p, q0, head, rho, at, lat);
+  store_out4(p.a.out, p.a.dtype, at + d, row_out(a.m, a.mw, a.l, a.o));
+  if (p.a.lse && d == 0) p.a.lse[lat] = row_lse(a.m, a.l);
+}
+constexpr float4 kNoStats = {kNone, kNone, 0.f, 0.f}, kNoSums = {0.f, 0.f, 0.f, 0.f};
 
 struct Entry {     // a piece of a unit that ended in this CTA without being the whole unit
   int used, q0, rows, head, tile;
@@ -827,11 +810,28 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
       uint32_t list = s_group[grp].y;
       const bool begins = e.begin >= c0, ends = e.end <= c1;
       float* dst = begins && ends ? nullptr : p.ws + ((size_t)cta * (kAttMaxWarps + 2) + kAttMaxWarps + (begins ? 1 : 0)) * kPart;
-      merge_row<D, NT, false, 4>(p, [&]() {
-        const float* part = s_entry[__ffs(list) - 1].part;
-        list &= list - 1;
-        return part;
-      }, __popc(list), row, d, dst, e.q0, e.head, e.tile);
+      RowSum sum;
+      while (list) {   // four pieces at a time
+        float4 st[4], x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          st[j] = kNoStats;
+          x[j] = kNoSums;
+          if (list) {
+            const float* part = s_entry[__ffs(list) - 1].part;
+            list &= list - 1;
+            st[j] = *reinterpret_cast<const float4*>(part + row * 4);
+            x[j] = *reinterpret_cast<const float4*>(part + 8 * NT * 4 + row * D + d);
+          }
+        }
+        join(sum, st, x);
+      }
+      if (dst) {
+        if (d == 0) *reinterpret_cast<float4*>(dst + row * 4) = make_float4(sum.m, sum.mw, sum.l, 0.f);
+        *reinterpret_cast<float4*>(dst + 8 * NT * 4 + row * D + d) = sum.o;
+      } else {
+        store_row(p, sum, e.q0, e.head, e.tile * 8 * NT + row, d);
+      }
     }
     if (tid == kWarps * 32 - 1) {   // the last unit may reach past the CTA
       int4 todo = make_int4(0, 0, 0, 0);
@@ -860,27 +860,56 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
 }
 
 // CTA c merges the unit that begins in CTA c of k_attend and reaches past it: its slot 1 and
-// slot 0 of the CTAs that follow, up to the one where it ends.
-constexpr int kMergeThreads = 256;
+// slot 0 of the CTAs that follow, up to the one where it ends.  A thread has four dimensions of
+// a row; the parts go round kGroups groups of threads, whose sums meet in shared memory (one
+// group: 131072 tokens x 4 fp32 queries 84 us in all, 80 so).
+constexpr int kMergeThreads = 1024;
 
 template <int D, int NT>
 __global__ void __launch_bounds__(kMergeThreads) k_attend_merge(const AttArgs p) {
+  constexpr int kPart = part_floats(D, 8 * NT), kItems = 8 * NT * (D / 4), kGroups = kMergeThreads / kItems, kBatch = 4;
+  __shared__ float4 s_stats[kMergeThreads], s_sums[kMergeThreads];
   after_previous();
-  constexpr int kPart = part_floats(D, 8 * NT);
-  const int cta = blockIdx.x;
-  const int4 d = __ldcg(p.desc + cta);
-  if (!d.x) return;
-  const float* slot = p.ws + ((size_t)cta * (kAttMaxWarps + 2) + kAttMaxWarps + 1) * kPart;
-  for (int i = threadIdx.x; i < 8 * NT * (D / 4); i += kMergeThreads) {
-    const int row = i / (D / 4);
-    if (d.w * 8 * NT + row >= d.z) break;
-    const float* part = slot;
-    merge_row<D, NT, true, 8>(p, [&]() {
-      const float* now = part;
-      part += ((size_t)(kAttMaxWarps + 2) - (now == slot ? 1 : 0)) * kPart;
-      return now;
-    }, d.x & 255, row, i % (D / 4) * 4, nullptr, d.y, d.x >> 8, d.w);
+  const int cta = blockIdx.x, item = threadIdx.x % kItems, grp = threadIdx.x / kItems;
+  const int row = item / (D / 4), d = item % (D / 4) * 4;
+  auto load = [&](int k, float4& s, float4& x) {
+    const float* part = p.ws + ((size_t)(cta + k) * (kAttMaxWarps + 2) + kAttMaxWarps + (k == 0 ? 1 : 0)) * kPart;
+    s = __ldcg(reinterpret_cast<const float4*>(part + row * 4));
+    x = __ldcg(reinterpret_cast<const float4*>(part + 8 * NT * 4 + row * D + d));
+  };
+  // a group's first part is read before it is known whether there is one
+  float4 s0[1] = {kNoStats}, x0[1] = {kNoSums};
+  if (cta + grp < p.ctas) load(grp, s0[0], x0[0]);
+  const int4 unit = __ldcg(p.desc + cta);   // parts | head << 8, first query token, rows, tile
+  if (!unit.x) return;
+  const int parts = unit.x & 255, rho = unit.w * 8 * NT + row;
+  RowSum sum;
+  if (grp < parts) join(sum, s0, x0);
+  for (int k = grp + kGroups; k < parts; k += kGroups * kBatch) {
+    float4 s[kBatch], x[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      s[j] = kNoStats;
+      x[j] = kNoSums;
+      if (k + j * kGroups < parts) load(k + j * kGroups, s[j], x[j]);
+    }
+    join(sum, s, x);
   }
+  if constexpr (kGroups > 1) {
+    if (grp > 0) {
+      s_stats[threadIdx.x] = make_float4(sum.m, sum.mw, sum.l, 0.f);
+      s_sums[threadIdx.x] = sum.o;
+    }
+    __syncthreads();
+    if (grp > 0) return;
+#pragma unroll
+    for (int g = 1; g < kGroups; ++g) {
+      s0[0] = s_stats[g * kItems + item];
+      x0[0] = s_sums[g * kItems + item];
+      join(sum, s0, x0);
+    }
+  }
+  if (rho < unit.z) store_row(p, sum, unit.y, unit.x >> 8, rho, d);
 }
 
 size_t attention_workspace_bytes(int head_dim, int rows) {
