@@ -802,35 +802,51 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
     }
     __syncthreads();
     const int groups = s_groups;
-    // a thread has four dimensions of a row of a unit; the units of a CTA side by side, row by row
-    for (int i = tid; i < groups * 8 * NT * (D / 4); i += kWarps * 32) {
-      const int d = i % (D / 4) * 4, row = i / (D / 4) / groups, grp = i / (D / 4) - row * groups;
+    // a warp has a row of a unit: lane i the references and sum of piece i, then four dimensions
+    for (int i = wid; i < groups * 8 * NT; i += kWarps) {
+      const int row = i / groups, grp = i - row * groups, d = lane * 4;
       const Entry& e = s_entry[s_group[grp].x];
       if (e.tile * 8 * NT + row >= e.rows) continue;
       uint32_t list = s_group[grp].y;
-      const bool begins = e.begin >= c0, ends = e.end <= c1;
-      float* dst = begins && ends ? nullptr : p.ws + ((size_t)cta * (kAttMaxWarps + 2) + kAttMaxWarps + (begins ? 1 : 0)) * kPart;
+      const bool begins = e.begin >= c0, ends = e.end <= c1, mine = list >> lane & 1u;
+      const unsigned long long my_part = mine ? reinterpret_cast<unsigned long long>(s_entry[lane].part) : 0;
+      const float4 st = mine ? *(reinterpret_cast<const float4*>(my_part) + row) : kNoStats;
       RowSum sum;
-      while (list) {   // four pieces at a time
-        float4 st[4], x[4];
+      sum.m = st.x;
+      sum.mw = st.y;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        sum.m = fmaxf(sum.m, __shfl_xor_sync(0xffffffffu, sum.m, o));
+        sum.mw = fmaxf(sum.mw, __shfl_xor_sync(0xffffffffu, sum.mw, o));
+      }
+      sum.l = st.z * ex2(st.x - sum.m);
+      const float f = ex2(st.y - sum.mw);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) sum.l += __shfl_xor_sync(0xffffffffu, sum.l, o);
+      while (list) {   // four pieces at a time, ascending
+        float4 x[4];
+        float w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          st[j] = kNoStats;
+          const int piece = list ? __ffs(list) - 1 : 0;
+          const float* part = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, my_part, piece));
+          w[j] = __shfl_sync(0xffffffffu, f, piece);
           x[j] = kNoSums;
-          if (list) {
-            const float* part = s_entry[__ffs(list) - 1].part;
-            list &= list - 1;
-            st[j] = *reinterpret_cast<const float4*>(part + row * 4);
-            x[j] = *reinterpret_cast<const float4*>(part + 8 * NT * 4 + row * D + d);
-          }
+          if (list && d < D) x[j] = *reinterpret_cast<const float4*>(part + 8 * NT * 4 + row * D + d);
+          list &= list - 1;
         }
-        join(sum, st, x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sum.o.x += x[j].x * w[j]; sum.o.y += x[j].y * w[j]; sum.o.z += x[j].z * w[j]; sum.o.w += x[j].w * w[j];
+        }
       }
-      if (dst) {
+      if (d >= D) continue;
+      if (begins && ends) {
+        store_row(p, sum, e.q0, e.head, e.tile * 8 * NT + row, d);
+      } else {
+        float* dst = p.ws + ((size_t)cta * (kAttMaxWarps + 2) + kAttMaxWarps + (begins ? 1 : 0)) * kPart;
         if (d == 0) *reinterpret_cast<float4*>(dst + row * 4) = make_float4(sum.m, sum.mw, sum.l, 0.f);
         *reinterpret_cast<float4*>(dst + 8 * NT * 4 + row * D + d) = sum.o;
-      } else {
-        store_row(p, sum, e.q0, e.head, e.tile * 8 * NT + row, d);
       }
     }
     if (tid == kWarps * 32 - 1) {   // the last unit may reach past the CTA
