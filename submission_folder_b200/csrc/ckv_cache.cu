@@ -39,17 +39,17 @@ template <int kFmt> CKV_DEV float scale_for(uint32_t amax_bits) {
 // 1 / scale of a power of two in [2^-126, 2^121].
 CKV_DEV float inv_pow2(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
-// Four codes from four values times the inverse scale (a power of two: the product is exact).
+// Four codes from four values over the scale.
 // int8: adding 1.5 2^23 leaves the nearest whole number, ties to even, in the low byte.
-template <int kFmt> CKV_DEV uint32_t encode4(float a, float b, float c, float d, float inv) {
+template <int kFmt> CKV_DEV uint32_t encode4(float a, float b, float c, float d) {
   uint32_t r;
   if constexpr (kFmt == CKV_CACHE_E4M3) {
     asm("{\n.reg .b16 lo, hi;\ncvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\ncvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n"
-        "mov.b32 %0, {lo, hi};\n}\n" : "=r"(r) : "f"(a * inv), "f"(b * inv), "f"(c * inv), "f"(d * inv));
+        "mov.b32 %0, {lo, hi};\n}\n" : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
   } else {
     constexpr float kMagic = 12582912.f;
-    const uint32_t x = __float_as_uint(fmaf(a, inv, kMagic)), y = __float_as_uint(fmaf(b, inv, kMagic));
-    const uint32_t z = __float_as_uint(fmaf(c, inv, kMagic)), w = __float_as_uint(fmaf(d, inv, kMagic));
+    const uint32_t x = __float_as_uint(a + kMagic), y = __float_as_uint(b + kMagic);
+    const uint32_t z = __float_as_uint(c + kMagic), w = __float_as_uint(d + kMagic);
     r = __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
   }
   return r;
@@ -67,7 +67,8 @@ template <int kFmt> CKV_DEV void decode4(uint32_t w, float (&o)[4]) {
   }
 }
 
-// 16 elements of a row as they are, their largest magnitude, and four of them as fp32.
+// 16 elements of a row as they are, their largest magnitude, and four of them as fp32 times a
+// power of two.
 template <typename T> struct Row16;
 template <> struct Row16<float> {
   float4 x[4];
@@ -79,7 +80,7 @@ template <> struct Row16<float> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  CKV_DEV float4 get(int i) const { return x[i]; }
+  CKV_DEV float4 get(int i, float by) const { return make_float4(x[i].x * by, x[i].y * by, x[i].z * by, x[i].w * by); }
   CKV_DEV uint32_t amax(uint32_t top) const {   // a NaN stays
     float m = __uint_as_float(top);
 #pragma unroll
@@ -107,9 +108,18 @@ template <typename H> struct Row16 {
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = 0;
   }
-  CKV_DEV float4 get(int i) const {
-    const float2 a = f2(w[2 * i]), b = f2(w[2 * i + 1]);
-    return make_float4(a.x, a.y, b.x, b.y);
+  CKV_DEV float4 get(int i, float by) const {
+    if constexpr (std::is_same<H, __half>::value) {   // `by` may be out of its range
+      const float2 a = f2(w[2 * i]), b = f2(w[2 * i + 1]);
+      return make_float4(a.x * by, a.y * by, b.x * by, b.y * by);
+    } else {   // exact in bf16 too, above 2^-126 (every format's zero)
+      const uint32_t by2 = __byte_perm(__float_as_uint(by), 0, 0x3232);
+      uint32_t x, y;
+      asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(x) : "r"(w[2 * i]), "r"(by2));
+      asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(w[2 * i + 1]), "r"(by2));
+      const float2 a = f2(x), b = f2(y);
+      return make_float4(a.x, a.y, b.x, b.y);
+    }
   }
   CKV_DEV uint32_t amax(uint32_t top) const {   // of both halves of the words, of any sign; a NaN stays
 #pragma unroll
@@ -280,8 +290,8 @@ __global__ void __launch_bounds__(kCacheMaxBlock / kRowsPerWarp * 32) k_cache_wr
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float4 f = row.get(e);
-          w[e] = encode4<kFmt>(f.x, f.y, f.z, f.w, inv);
+          const float4 f = row.get(e, inv);
+          w[e] = encode4<kFmt>(f.x, f.y, f.z, f.w);
         }
         if (bad) w[0] = w[1] = w[2] = w[3] = 0;
         *reinterpret_cast<uint4*>(dst + o * tstr) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -313,7 +323,7 @@ __global__ void __launch_bounds__(kCacheMaxBlock / kRowsPerWarp * 32) k_cache_wr
           for (int e = 0; e < 4; ++e) {
             float f[4];
             decode4<kFmt>(w[e], f);
-            w[e] = encode4<kFmt>(f[0], f[1], f[2], f[3], ratio);
+            w[e] = encode4<kFmt>(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
           }
           *p = make_uint4(w[0], w[1], w[2], w[3]);
         }
