@@ -296,7 +296,11 @@ cudaError_t launch_block_tables(const ckv_table_step& s, cudaStream_t st) {
   const bool solo = (int64_t)s.total + s.requests <= CKV_TABLES_SMALL;
   if (cudaError_t e = launch_after(k_block_tables, dim3(1), kTabThreads, smem, st, s, solo ? 1 : 0); solo || e != cudaSuccess)
     return e;
-  const int parts = s.requests >= 592 ? 1 : std::min(592 / s.requests, 64);   // about four CTAs per SM
+  // up to about four CTAs per SM, with work for each of their threads: a CTA costs more than it
+  // saves without (16 requests, 23,000 tokens: 37 CTAs each 9.1 us, 12 each 7.2; 200 requests, 127,000
+  // tokens: 2 each 8.8 us, 1 each 12, 11 each 13)
+  const int most = s.requests >= 592 ? 1 : std::min(592 / s.requests, 64);
+  const int parts = (int)std::min((int64_t)most, s.total / ((int64_t)kFillThreads * s.requests) + 1);
   return launch_after(k_block_tables_fill, dim3(s.requests + 1, parts), kFillThreads, 0, st, s);
 }
 
