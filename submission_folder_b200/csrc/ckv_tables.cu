@@ -20,6 +20,7 @@
 
 #include "ckv_cache.h"
 #include "ckv_common.cuh"
+#include "ckv_share.h"
 
 namespace ckv {
 
@@ -232,14 +233,14 @@ __global__ void __launch_bounds__(kFillThreads) k_block_tables_fill(const ckv_ta
   int32_t* table = s.tables + r * s.table_stride;
   for (int k = part * kFillThreads + tid; k < returned; k += parts * kFillThreads)
     if (count + b0 + k < have) s.free_list[count + b0 + k] = table[k];
-  const int each = (ask + parts - 1) / parts, i0 = min((int64_t)part * each, (int64_t)ask), i1 = min((int64_t)i0 + each, (int64_t)ask);
+  const Share mine = share_of(ask, give, t0, s.total, part, parts);
+  const uint32_t i0 = mine.from, i1 = mine.to, rows = max(s.total - t0, 0);   // tokens i < rows have a row
   if (i0 >= i1) return;
   if (give == 0) {   // refused
-    for (int i = i0 + tid; i < i1; i += kFillThreads)
-      if (t0 + i < s.total) {
-        s.out_slots[t0 + i] = -1;
-        s.out_positions[t0 + i] = (long long)n + i + shift;
-      }
+    for (uint32_t i = i0 + tid; i < i1; i += kFillThreads) {
+      s.out_slots[t0 + i] = -1;
+      s.out_positions[t0 + i] = (long long)n + i + shift;
+    }
     return;
   }
   // the blocks of these tokens, kFillBlocks at a time, then the tokens in them
@@ -280,9 +281,9 @@ __global__ void __launch_bounds__(kFillThreads) k_block_tables_fill(const ckv_ta
     }
     __syncthreads();
     const int64_t from = max((int64_t)i0, (int64_t)c * b - n), to = min((int64_t)i1, (int64_t)(c + blocks) * b - n);
-    for (int i = (int)from + tid; i < to; i += kFillThreads) {
+    for (uint32_t i = (uint32_t)from + tid; i < to; i += kFillThreads) {
       const uint32_t pos = (uint32_t)n + i, bi = pos / b;
-      if (t0 + i < s.total) {
+      if (i < rows) {
         s.out_slots[t0 + i] = (long long)s_id[bi - c] * b + (pos - bi * b);
         s.out_positions[t0 + i] = (long long)pos + shift;
       }

@@ -116,6 +116,33 @@ def test_block_tables_release_feeds_admission(dev):
     assert s.granted.tolist() == [0, 33]
 
 
+@pytest.mark.parametrize("R,total", [(3, 8000), (600, 4000), (20, 100)])
+@pytest.mark.parametrize("ask", [2 ** 31 - 1, 2 ** 31 - 100, 1 << 28])
+def test_block_tables_refused_request_of_nearly_2_31_tokens(dev, R, total, ask):
+    """Its rows say -1 and their positions; the requests before it and after it (for which the step has no
+    rows) get what they get without it.  Several CTAs for each request, one, and one for all."""
+    i32 = dict(dtype=torch.int32, device=dev)
+    block, width, rng = 16, 6, random.Random(R)
+    lens, tables, free = _tables_state(rng, R, block, width, 40, 4 * R)
+    new = [rng.choice([1, 0, 33, -1]) for _ in range(R)]
+    big = R // 3
+    lens[big], new[big] = 5, total + (width + 1) * block
+    cap = sum(-(-n // block) for n in lens) + len(free)
+    t = ref.RefTables(lens, tables, free, block)
+    shift = [rng.randint(0, 200000) for _ in range(R)]
+    d = [torch.tensor(x, **i32) for x in (lens, tables, free + [-1] * (cap - len(free)), [len(free)])]
+    want = t.step(new, total, shift)
+    new[big] = ask
+    got = ops.block_tables(d[0], torch.tensor(new, **i32), d[1], d[2], d[3], block, total, shift=torch.tensor(shift, **i32))
+    for name in ("lens", "slots", "positions", "granted"):
+        assert getattr(got, name).tolist() == want[name], name
+    cu = [0]
+    for n in new:
+        cu.append(min(cu[-1] + max(n, 0), 2 ** 31 - 1))
+    assert got.cu.tolist() == cu and d[1].tolist() == t.tables
+    assert int(d[3]) == len(t.free) and d[2][:len(t.free)].tolist() == t.free
+
+
 def test_block_tables_refusals(dev):
     i32 = dict(dtype=torch.int32, device=dev)
     a = dict(lens=torch.zeros(3, **i32), new=torch.ones(3, **i32), tables=torch.zeros(3, 2, **i32),
