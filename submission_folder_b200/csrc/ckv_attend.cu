@@ -293,7 +293,9 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
   static_assert(2 * kWarps <= 32, "one ballot");
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x, R = p.a.requests;
-  if (tid < 2 * kWarps) s_entry[tid].used = 0;
+  // each warp clears the entries that it may set itself: no other warp's clearing can come after them
+  if (lane < 2) s_entry[2 * wid + lane].used = 0;
+  __syncwarp();
   after_previous();
 
   // ---- the line of units: its length, and where this warp stands in it (each warp for itself)
