@@ -738,6 +738,18 @@ def test_launches_wait_for_what_comes_before(dev):
         assert torch.equal(got, want)
 
 
+def test_attention_on_two_devices(dev):
+    """The same call on each device of one process, whichever is current."""
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two devices")
+    lens = [300, 64]
+    pool, tables, n, q, k, v = _attention_case(dev, lens, 2, 4, 128, 16, E4M3, torch.bfloat16, [1] * 2)
+    want = ops.cache_attention(q, *pool, tables, n)
+    other = torch.device("cuda", 1)
+    got = ops.cache_attention(q.to(other), *(t.to(other) for t in pool), tables.to(other), n.to(other))
+    assert got.device == other and torch.equal(got.to(dev), want)
+
+
 def test_attention_refusals(dev):
     pool, tables, n, q, k, v = _attention_case(dev, [20, 30], 2, 2, 64, 16, E4M3, torch.bfloat16, [1] * 2)
     cu = torch.tensor([0, 1, 2], dtype=torch.int32, device=dev)

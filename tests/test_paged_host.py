@@ -4,8 +4,6 @@ ends of its range and the launch helpers, against fakes of the CUDA calls."""
 import os
 import subprocess
 
-import pytest
-
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "submission_folder_b200", "csrc")
 
@@ -43,6 +41,40 @@ int main() {
             }
             if (at != want) return printf("%d %d %d %d: %u\n", ask, t0, total, parts, at), 1;
           }
+  return 0;
+}
+''')
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_shared_memory_is_opted_in_on_each_device(tmp_path):
+    """The limit belongs to a (kernel, device) pair: one device's opt-in says nothing of another's."""
+    r = _run(tmp_path, r'''
+#include "ckv_smem.h"
+#include <stdio.h>
+#include <map>
+static int now = 0, calls = 0, broken = 0;
+static std::map<std::pair<int, const void*>, int> limit;
+extern "C" cudaError_t cudaGetDevice(int* d) { *d = now; return cudaSuccess; }
+extern "C" cudaError_t cudaFuncSetAttribute(const void* f, cudaFuncAttribute a, int bytes) {
+  if (broken || a != cudaFuncAttributeMaxDynamicSharedMemorySize) return cudaErrorInvalidValue;
+  ++calls;
+  limit[{now, f}] = bytes;
+  return cudaSuccess;
+}
+int main() {
+  static int f, g;
+  for (int round = 0; round < 2; ++round)
+    for (now = 0; now < 9; ++now) {
+      if (ckv::ensure_dynamic_smem(&f, 196608) != cudaSuccess || (limit[{now, &f}] != 196608)) return printf("device %d\n", now), 1;
+      if (ckv::ensure_dynamic_smem(&f, 1000) != cudaSuccess || (limit[{now, &f}] != 196608)) return printf("lowered\n"), 1;
+    }
+  if (calls != 9) return printf("%d calls\n", calls), 1;
+  broken = 1;
+  now = 3;
+  if (ckv::ensure_dynamic_smem(&g, 1000) != cudaErrorInvalidValue) return printf("hidden error\n"), 1;
+  broken = 0;
+  if (ckv::ensure_dynamic_smem(&g, 1000) != cudaSuccess || calls != 10) return printf("kept error\n"), 1;
   return 0;
 }
 ''')
