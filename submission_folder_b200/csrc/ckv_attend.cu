@@ -145,12 +145,12 @@ CKV_DEV void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
 
 CKV_DEV int seq_len(const AttArgs& p, int r) {
   const long long cap = (long long)p.a.table_width << p.block_log2;
-  return (int)min(min((long long)max(__ldg(p.a.lens + r), 0), cap), (long long)INT32_MAX - 2 * kAttStep);
+  return (int)min(min((long long)max(p.a.lens[r], 0), cap), (long long)INT32_MAX - 2 * kAttStep);
 }
 CKV_DEV void seq_queries(const AttArgs& p, int r, int& q0, int& nq) {
   if (p.a.cu) {
-    q0 = min(max(__ldg(p.a.cu + r), 0), p.a.tokens);
-    nq = min(max(min(__ldg(p.a.cu + r + 1), p.a.tokens) - q0, 0), p.a.max_q);
+    q0 = min(max(p.a.cu[r], 0), p.a.tokens);
+    nq = min(max(min(p.a.cu[r + 1], p.a.tokens) - q0, 0), p.a.max_q);
   } else {
     q0 = r;
     nq = 1;
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
 
       // block ids: lane l holds page pbase + l, and the next 32 pages stand by
       int pbase = (s_begin * kAttStep) >> p.block_log2;
-      auto page = [&](int i) { return i < pages ? __ldg(table + i) : 0; };
+      auto page = [&](int i) { return i < pages ? table[i] : 0; };
       int pcur = page(pbase + lane), pnext = page(pbase + 32 + lane);
       // the 32 tokens of step s, as two halves of 16 that may stand in two blocks
       auto issue = [&](int s, int stage) {
@@ -892,13 +892,13 @@ __global__ void __launch_bounds__(kMergeThreads) k_attend_merge(const AttArgs p)
   const int row = item / (D / 4), d = item % (D / 4) * 4;
   auto load = [&](int k, float4& s, float4& x) {
     const float* part = p.ws + ((size_t)(cta + k) * (kAttMaxWarps + 2) + kAttMaxWarps + (k == 0 ? 1 : 0)) * kPart;
-    s = __ldcg(reinterpret_cast<const float4*>(part + row * 4));
-    x = __ldcg(reinterpret_cast<const float4*>(part + 8 * NT * 4 + row * D + d));
+    s = *reinterpret_cast<const float4*>(part + row * 4);
+    x = *reinterpret_cast<const float4*>(part + 8 * NT * 4 + row * D + d);
   };
   // a group's first part is read before it is known whether there is one
   float4 s0[1] = {kNoStats}, x0[1] = {kNoSums};
   if (cta + grp < p.ctas) load(grp, s0[0], x0[0]);
-  const int4 unit = __ldcg(p.desc + cta);   // parts | head << 8, first query token, rows, tile
+  const int4 unit = p.desc[cta];   // parts | head << 8, first query token, rows, tile
   if (!unit.x) return;
   const int parts = unit.x & 255, rho = unit.w * 8 * NT + row;
   RowSum sum;

@@ -76,7 +76,7 @@ template <> struct Row16<float> {
   float4 x[4];
   CKV_DEV void load(const float* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __ldg(reinterpret_cast<const float4*>(p) + i);
+    for (int i = 0; i < 4; ++i) x[i] = reinterpret_cast<const float4*>(p)[i];
   }
   CKV_DEV void clear() {
 #pragma unroll
@@ -102,7 +102,7 @@ template <> struct Row16<float> {
 template <typename H> struct Row16 {
   uint32_t w[8];
   CKV_DEV void load(const H* p) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+    const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
     w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
     w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
   }
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kCacheMaxBlock / kRowsPerWarp * 32) k_cache_wr
   const int64_t pool = (int64_t)a.c.num_blocks << a.block_log2;
   const int64_t* slots = a.r.slots;
   auto decode = [&](int i, int& blk, int& place) {
-    const int64_t s = i >= 0 && i < a.r.tokens ? __ldg(slots + i) : -1;
+    const int64_t s = i >= 0 && i < a.r.tokens ? slots[i] : -1;
     blk = s >= 0 && s < pool ? (int)(s >> a.block_log2) : -1;
     place = (int)s & (bs - 1);
   };
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(256) k_cache_read(const ckv_cache c, const Cac
   const int64_t pool = (int64_t)c.num_blocks << block_log2;
   int64_t slot[kReadTokens];
 #pragma unroll
-  for (int j = 0; j < kReadTokens; ++j) slot[j] = t + j * half < (uint32_t)r.tokens ? __ldg(r.slots + t + j * half) : -1;
+  for (int j = 0; j < kReadTokens; ++j) slot[j] = t + j * half < (uint32_t)r.tokens ? r.slots[t + j * half] : -1;
   uint4 q[kReadTokens][2];
   float sc[kReadTokens][2];
 #pragma unroll

@@ -13,7 +13,9 @@ namespace ckv {
 // A launch that may begin while the launch before it on the stream drains (programmatic
 // dependent launch): its blocks are placed early and wait in after_previous(), which every
 // kernel launched so calls in every thread before it touches global memory.  Saves the gap
-// between the short kernels of a decode step.
+// between the short kernels of a decode step.  What the launch before may have written is read
+// with plain loads only: read-only (non-coherent) ones are defined for data that is constant while
+// the kernel is resident, and neither those nor cache-hinted ones are bound to stay behind the wait.
 template <typename... P>
 cudaError_t launch_after(void (*fn)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, P... args) {
   cudaLaunchConfig_t cfg = {};

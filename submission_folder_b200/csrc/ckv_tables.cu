@@ -88,9 +88,9 @@ CKV_DEV void fill_step(const ckv_table_step& s, const StepView& v, int gt, int g
   const uint32_t b = s.block_size;
   // the j-th block from the bottom of the stack, after the blocks given back went on top
   auto stack = [&](int j) -> int {
-    if (j < v.count) return __ldcg(s.free_list + j);
+    if (j < v.count) return s.free_list[j];
     const int e = j - v.count, r = row_of(v.back, 0, R - 1, e);
-    return __ldcg(s.tables + r * s.table_stride + (e - v.back[r]));
+    return s.tables[r * s.table_stride + (e - v.back[r])];
   };
   for (int i = gt; i < v.have - v.count; i += gn) s.free_list[v.count + i] = stack(v.count + i);
   for (int i = gt; i < v.taken; i += gn) {
@@ -106,7 +106,7 @@ CKV_DEV void fill_step(const ckv_table_step& s, const StepView& v, int gt, int g
       where = (long long)pos + (s.shift ? s.shift[r] : 0);
       if (v.give[r] > 0) {
         const uint32_t bi = pos / b, held = (n + b - 1) / b;
-        const int block = bi < held ? __ldcg(s.tables + r * s.table_stride + bi)
+        const int block = bi < held ? s.tables[r * s.table_stride + bi]
                                     : stack(v.have - 1 - (v.fresh[r] + (int)(bi - held)));
         slot = (long long)block * b + (pos - bi * b);
       }
@@ -200,12 +200,12 @@ __global__ void __launch_bounds__(kTabThreads) k_block_tables(const ckv_table_st
 // the rows past the last request's.
 constexpr int kFillThreads = 128, kFillBlocks = 512;
 
-// Last row whose prefix p[row] is <= x, by one warp, 32 probes at a time; p in L2.
+// Last row whose prefix p[row] is <= x, by one warp, 32 probes at a time; p in global memory.
 CKV_DEV int warp_row_of(const int* p, int rows, int x) {
   int lo = 0, n = rows;
   while (n > 1) {
     const int step = (n + 31) / 32, i = (threadIdx.x & 31) * step;
-    const uint32_t m = __ballot_sync(0xffffffffu, i < n && __ldcg(p + lo + min(i, n - 1)) <= x);
+    const uint32_t m = __ballot_sync(0xffffffffu, i < n && p[lo + min(i, n - 1)] <= x);
     const int hit = m ? 31 - __clz(m) : 0;
     lo += hit * step;
     n = min(step, n - hit * step);
@@ -220,16 +220,16 @@ __global__ void __launch_bounds__(kFillThreads) k_block_tables_fill(const ckv_ta
   after_previous();
   const int *back = s.work, *fresh = back + R + 1, *len = fresh + R + 1, *tail = len + R;
   if (r == R) {   // no request's tokens
-    for (int64_t t = (int64_t)__ldcg(s.out_cu + R) + part * kFillThreads + tid; t < s.total; t += parts * kFillThreads) {
+    for (int64_t t = (int64_t)s.out_cu[R] + part * kFillThreads + tid; t < s.total; t += parts * kFillThreads) {
       s.out_slots[t] = -1;
       s.out_positions[t] = 0;
     }
     return;
   }
-  const int t0 = __ldcg(s.out_cu + r), ask = __ldcg(s.out_cu + r + 1) - t0, give = __ldcg(s.out_granted + r);
-  const int n = __ldcg(len + r), b0 = __ldcg(back + r), returned = __ldcg(back + r + 1) - b0, f0 = __ldcg(fresh + r);
-  const int count = __ldcg(tail), have = __ldcg(tail + 1);
-  const int shift = s.shift ? __ldg(s.shift + r) : 0;
+  const int t0 = s.out_cu[r], ask = s.out_cu[r + 1] - t0, give = s.out_granted[r];
+  const int n = len[r], b0 = back[r], returned = back[r + 1] - b0, f0 = fresh[r];
+  const int count = tail[0], have = tail[1];
+  const int shift = s.shift ? s.shift[r] : 0;
   int32_t* table = s.tables + r * s.table_stride;
   for (int k = part * kFillThreads + tid; k < returned; k += parts * kFillThreads)
     if (count + b0 + k < have) s.free_list[count + b0 + k] = table[k];
@@ -264,15 +264,15 @@ __global__ void __launch_bounds__(kFillThreads) k_block_tables_fill(const ckv_ta
       } else {
         const int j = have - 1 - (f0 + (int)(bi - held));   // from the bottom of the stack, what came back on top
         if (j < count) {
-          id = __ldg(s.free_list + j);
+          id = s.free_list[j];
         } else {
           int lo = row_lo, hi = row_hi;
           while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (__ldcg(back + mid) <= j - count) lo = mid;
+            if (back[mid] <= j - count) lo = mid;
             else hi = mid - 1;
           }
-          id = __ldg(s.tables + lo * s.table_stride + (j - count - __ldcg(back + lo)));
+          id = s.tables[lo * s.table_stride + (j - count - back[lo])];
         }
         const int64_t at = (int64_t)bi * b - n;             // the block's first token: its part writes the entry
         if (at >= i0 && at < i1) table[bi] = id;

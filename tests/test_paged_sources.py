@@ -20,3 +20,12 @@ def test_a_warp_clears_only_its_own_entries():
     written = re.findall(r"s_entry\[((?!2 \* kWarps\])[^\]]*)\]", body)
     assert len(written) == 2 and all(w.startswith("2 * wid +") for w in written)
     assert body.index("__syncwarp()") > body.index("s_entry[2 * wid + lane].used = 0")
+
+
+def test_kernels_placed_early_use_plain_loads():
+    """A kernel that is resident while its predecessor runs reads through loads that the wait orders."""
+    for name in ("ckv_tables.cu", "ckv_rotary.cu", "ckv_cache.cu", "ckv_attend.cu"):
+        text = _source(name)
+        for other in ("__ldg", "__ldcg", "__ldca", "__ldcs", "ld.global.nc", "__restrict__"):
+            assert other not in text, (name, other)
+        assert text.count("__global__") <= text.count("after_previous();") + text.count("turns_of(a, t0, nt, rot_cs);"), name
