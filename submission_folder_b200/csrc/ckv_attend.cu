@@ -3,9 +3,10 @@
 // out = sum_j softmax_j(scale q.k_j) v_j with k_j = ks[b] * ck_j, v_j = vs[b] * cv_j: codes
 // c in 8 bits, scales by (block b, KV head).  One pass, with a running maximum.  The scales
 // never touch the codes: ks multiplies the logit after its dot product, and vs joins the
-// weight as an exponent, w_j = 2^(s_j + log2 vs - m'), which has its own reference m' beside
-// the softmax's m; the two meet once, at the end.  So the matrix products run on the codes,
-// which fp16 holds exactly.
+// weight as an exponent, w_j = 2^((s_j - m) + log2 vs - m'), which has a reference m' of its own
+// on top of the softmax's m; out = 2^m' sum_j w_j c_j / sum_j 2^(s_j - m).  So the matrix products
+// run on the codes, which fp16 holds exactly.  s_j - m comes first: m' and log2 vs are small numbers
+// and would be lost beside a logit beyond 2^24.
 //
 // Products: m16n8k16 in fp16 with fp32 sums, tokens (or value dimensions) as the 16 rows of the
 // left operand and 8 query rows (a KV head's query heads times the new tokens) as the
@@ -42,7 +43,7 @@ namespace ckv {
 constexpr int kAttStep = 32;      // tokens per step
 constexpr int kAttMaxCtas = 148;
 constexpr int kAttMaxWarps = 12;
-constexpr float kNone = -3e38f;   // a running maximum that has seen nothing
+constexpr float kNone = -3.402823466e38f;   // the reference of a row that has seen nothing: no logit lies below it
 constexpr float kSlack = 6.f;     // weights may pass their reference by 2^kSlack
 constexpr float kTop = 9.f;       // and stand at 2^kTop there: at most 2^15 in fp16
 
@@ -230,31 +231,35 @@ CKV_DEV void row_home(const AttArgs& p, int q0, int head, int rho, int64_t& out,
   out = (q0 + i) * p.a.out_tok_stride + hq * p.a.out_head_stride;
   lse = (int64_t)(q0 + i) * (p.c.num_kv_heads * p.group) + hq;
 }
-// A row's output from its sums, references (base 2) and weight, and its log-sum-exp.  The power of
-// two comes last: it may lie below fp32's range when the values do.
-CKV_DEV float4 row_out(float m, float mw, float l, float4 o) {
-  const float inv = l > 0.f || isnan(l) ? 1.f / l : 0.f, f = exp2f(mw - m - kTop);
+// A row's output from its sums, weights' reference (base 2) and weight, and its log-sum-exp.  The
+// power of two comes last: it may lie below fp32's range when the values do.
+CKV_DEV float4 row_out(float mw, float l, float4 o) {
+  const float inv = l > 0.f || isnan(l) ? 1.f / l : 0.f, f = exp2f(mw - kTop);
   return make_float4(o.x * inv * f, o.y * inv * f, o.z * inv * f, o.w * inv * f);
 }
 CKV_DEV float row_lse(float m, float l) { return l > 0.f || isnan(l) ? (m + log2f(l)) * kLn2 : -INFINITY; }
 
 // A row's running references and sum, and four of its dimensions.
 struct RowSum {
-  float m = kNone, mw = kNone, l = 0.f;
+  float m = kNone, mw = 0.f, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 };
 // Joined by partial results: s their (m, m', l, -), x their sums.
 template <int N> CKV_DEV void join(RowSum& a, const float4 (&s)[N], const float4 (&x)[N]) {
-  float nm = a.m, nw = a.mw;
+  float nm = a.m;
 #pragma unroll
-  for (int j = 0; j < N; ++j) { nm = fmaxf(nm, s[j].x); nw = fmaxf(nw, s[j].y); }
+  for (int j = 0; j < N; ++j) nm = fmaxf(nm, s[j].x);
+  const float kept = a.mw + (a.m - nm);   // references beside the common m
+  float nw = kept;
+#pragma unroll
+  for (int j = 0; j < N; ++j) nw = fmaxf(nw, s[j].y + (s[j].x - nm));
   a.l *= ex2(a.m - nm);
-  const float f0 = ex2(a.mw - nw);
+  const float f0 = ex2(kept - nw);
   a.o.x *= f0; a.o.y *= f0; a.o.z *= f0; a.o.w *= f0;
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     a.l += s[j].z * ex2(s[j].x - nm);
-    const float f = ex2(s[j].y - nw);
+    const float f = ex2(s[j].y + (s[j].x - nm) - nw);
     a.o.x += x[j].x * f; a.o.y += x[j].y * f; a.o.z += x[j].z * f; a.o.w += x[j].w * f;
   }
   a.m = nm;
@@ -264,10 +269,10 @@ template <int N> CKV_DEV void join(RowSum& a, const float4 (&s)[N], const float4
 CKV_DEV void store_row(const AttArgs& p, const RowSum& a, int q0, int head, int rho, int d) {
   int64_t at, lat;
   row_home(p, q0, head, rho, at, lat);
-  store_out4(p.a.out, p.a.dtype, at + d, row_out(a.m, a.mw, a.l, a.o));
+  store_out4(p.a.out, p.a.dtype, at + d, row_out(a.mw, a.l, a.o));
   if (p.a.lse && d == 0) p.a.lse[lat] = row_lse(a.m, a.l);
 }
-constexpr float4 kNoStats = {kNone, kNone, 0.f, 0.f}, kNoSums = {0.f, 0.f, 0.f, 0.f};
+constexpr float4 kNoStats = {kNone, 0.f, 0.f, 0.f}, kNoSums = {0.f, 0.f, 0.f, 0.f};
 
 struct Entry {     // a piece of a unit that ended in this CTA without being the whole unit
   int used, q0, rows, head, tile;
@@ -524,7 +529,7 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) { m[nt][r] = mw[nt][r] = kNone; l[nt][r] = 0.f; }
+        for (int r = 0; r < 2; ++r) { m[nt][r] = l[nt][r] = 0.f; mw[nt][r] = kNone; }   // kNone: m is not set yet
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
       }
@@ -594,6 +599,13 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
           ve[u] = (float)((int)(bits >> 23 & 255u) - 127);
           if (mant) ve[u] = isnan(v) ? v : ve[u] + __log2f(__uint_as_float(mant | 0x3f800000u));   // not a power of two
         }
+        float over[NT][2][2];   // log2 vs over the weights' reference, ready before the vote (x 4 fp32 queries 83.5 -> 82.6 us)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) over[nt][r][u] = ve[u] - mw[nt][r];
         bool hide = false;   // a token that a row does not see stands in a block whose value scale is NaN
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -601,9 +613,9 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
           for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              const float f = qs[nt][r] * ks[u];
-              sc[nt][u][r] *= f;
-              sc[nt][u][2 + r] *= f;
+              const float f = qs[nt][r] * ks[u];   // logits relative to m, rounded once
+              sc[nt][u][r] = fmaf(sc[nt][u][r], f, -m[nt][r]);
+              sc[nt][u][2 + r] = fmaf(sc[nt][u][2 + r], f, -m[nt][r]);
             }
         if ((s + 1) * kAttStep > see_min) {
 #pragma unroll
@@ -621,31 +633,44 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const float h0 = fmaxf(sc[nt][0][r], sc[nt][0][2 + r]), h1 = fmaxf(sc[nt][1][r], sc[nt][1][2 + r]);
-            past = past || fmaxf(h0, h1) > m[nt][r] + kSlack || fmaxf(h0 + ve[0], h1 + ve[1]) > mw[nt][r] + kSlack;
+            past = past || fmaxf(h0, h1) > kSlack || fmaxf(h0 + over[nt][r][0], h1 + over[nt][r][1]) > kSlack;
           }
         if (__any_sync(0xffffffffu, past)) {
+          float shift[NT][2];
           // the rows that passed theirs get new references (whole numbers: the rescaling is exact),
           // the same in all lanes of a row and whatever the other rows do
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const float h0 = fmaxf(sc[nt][0][r], sc[nt][0][2 + r]), h1 = fmaxf(sc[nt][1][r], sc[nt][1][2 + r]);
-              float nm = fmaxf(m[nt][r], fmaxf(h0, h1)), nw = fmaxf(mw[nt][r], fmaxf(h0 + ve[0], h1 + ve[1]));
+              float h0 = fmaxf(sc[nt][0][r], sc[nt][0][2 + r]), h1 = fmaxf(sc[nt][1][r], sc[nt][1][2 + r]);
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1) {
-                nm = fmaxf(nm, __shfl_xor_sync(0xffffffffu, nm, d));
-                nw = fmaxf(nw, __shfl_xor_sync(0xffffffffu, nw, d));
+                h0 = fmaxf(h0, __shfl_xor_sync(0xffffffffu, h0, d));
+                h1 = fmaxf(h1, __shfl_xor_sync(0xffffffffu, h1, d));
               }
-              nm = nm > m[nt][r] + kSlack ? ceilf(nm) : m[nt][r];
-              nw = nw > mw[nt][r] + kSlack ? ceilf(nw) : mw[nt][r];
-              l[nt][r] *= ex2(m[nt][r] - nm);
-              const float f = ex2(mw[nt][r] - nw);
+              // the first logit that a row sees sets m; rounded up, so that none stays above it
+              const bool unset = mw[nt][r] == kNone, move = unset ? fmaxf(h0, h1) > -INFINITY : fmaxf(h0, h1) > kSlack;
+              const float nm = move ? ceilf(__fadd_ru(m[nt][r], fmaxf(h0, h1))) : m[nt][r], d = nm - m[nt][r];
+              const float kept = mw[nt][r] - d;   // the old reference of the weights beside the new m
+              float nw = fmaxf(h0 - d + ve[0], h1 - d + ve[1]);
+              nw = nw > kept + kSlack ? ceilf(nw) : unset && !move ? kNone : fmaxf(kept, -3e38f);
+              l[nt][r] *= unset ? 1.f : ex2(-d);   // not set: nothing but zeros or a NaN
+              const float f = ex2(kept - nw);
               m[nt][r] = nm;
               mw[nt][r] = nw;
+              over[nt][r][0] = ve[0] - nw;
+              over[nt][r][1] = ve[1] - nw;
 #pragma unroll
               for (int j = 0; j < kTiles; ++j) { o[nt][j][r] *= f; o[nt][j][2 + r] *= f; }
+              shift[nt][r] = d;
             }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int u = 0; u < 2; ++u) { sc[nt][u][r] -= shift[nt][r]; sc[nt][u][2 + r] -= shift[nt][r]; }
         }
         uint32_t pf[NT][kTerms][2][2];
 #pragma unroll
@@ -656,8 +681,8 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int r = e & 1;
-              l[nt][r] += ex2(sc[nt][u][e] - m[nt][r]);
-              w[e] = ex2(sc[nt][u][e] + (ve[u] - mw[nt][r] + kTop));
+              l[nt][r] += ex2(sc[nt][u][e]);
+              w[e] = ex2(sc[nt][u][e] + (over[nt][r][u] + kTop));
             }
             if (hide) {
 #pragma unroll
@@ -750,7 +775,8 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
           for (int d = 4; d < 32; d <<= 1) lt += __shfl_xor_sync(0xffffffffu, lt, d);
           const int row = nt * 8 + 2 * t + r;
           if (part) {
-            if (g == 0) *reinterpret_cast<float4*>(part + row * 4) = make_float4(m[nt][r], mw[nt][r], lt, 0.f);
+            const bool unset = mw[nt][r] == kNone;
+            if (g == 0) *reinterpret_cast<float4*>(part + row * 4) = make_float4(unset ? kNone : m[nt][r], unset ? 0.f : mw[nt][r], lt, 0.f);
             float4* d = reinterpret_cast<float4*>(part + 8 * NT * 4 + row * D + g * 2 * kTiles);
 #pragma unroll
             for (int j = 0; j < kTiles; j += 2)
@@ -763,7 +789,7 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
 #pragma unroll
               for (int j = 0; j < kTiles; j += 2)
                 store_out4(p.a.out, p.a.dtype, at + g * 2 * kTiles + 2 * j,
-                           row_out(m[nt][r], mw[nt][r], lt, make_float4(o[nt][j][r], o[nt][j][2 + r], o[nt][j + 1][r], o[nt][j + 1][2 + r])));
+                           row_out(mw[nt][r], lt, make_float4(o[nt][j][r], o[nt][j][2 + r], o[nt][j + 1][r], o[nt][j + 1][2 + r])));
               if (p.a.lse && g == 0) p.a.lse[lat] = row_lse(m[nt][r], lt);
             }
           }
@@ -815,14 +841,14 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
       const float4 st = mine ? *(reinterpret_cast<const float4*>(my_part) + row) : kNoStats;
       RowSum sum;
       sum.m = st.x;
-      sum.mw = st.y;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        sum.m = fmaxf(sum.m, __shfl_xor_sync(0xffffffffu, sum.m, o));
-        sum.mw = fmaxf(sum.mw, __shfl_xor_sync(0xffffffffu, sum.mw, o));
-      }
+      for (int o = 1; o < 32; o <<= 1) sum.m = fmaxf(sum.m, __shfl_xor_sync(0xffffffffu, sum.m, o));
+      const float kept = st.y + (st.x - sum.m);
+      sum.mw = kept;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) sum.mw = fmaxf(sum.mw, __shfl_xor_sync(0xffffffffu, sum.mw, o));
       sum.l = st.z * ex2(st.x - sum.m);
-      const float f = ex2(st.y - sum.mw);
+      const float f = ex2(kept - sum.mw);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) sum.l += __shfl_xor_sync(0xffffffffu, sum.l, o);
       while (list) {   // four pieces at a time, ascending

@@ -570,6 +570,40 @@ def test_attention_scales_of_other_programs(dev, times_k, times_v):
     _attention_check(out, lse, q, k * times_k, v * times_v, lens, [1] * 2, 128 ** -0.5, True)
 
 
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("power", [10, 23, 24, 25, 26, 27, 28, 40, 100])
+def test_attention_logits_of_any_size(dev, power, dtype, sign):
+    """Logits of 1.37 * 2^power and 0 (sign 1: two tokens of 3000 carry everything), or all alike and below
+    zero (sign -1: all tokens carry the same), under value scales of 2^-12 to 2^12.  Equal logits are equal in any
+    arithmetic, so the output is the plain mean of their values: off by the weights' rounding (2^-11 relative for
+    bf16 queries, 2^-22 otherwise), what is subnormal in fp16 and the truncated sums, as in the header above."""
+    heads, dim, block, n = 2, 64, 32, 3000
+    g = torch.Generator().manual_seed(power)
+    pool = _pool(dev, 95, heads, block, dim, E4M3)
+    order = torch.randperm(94, generator=g)
+    at = torch.arange(n)
+    slots = (order[at // block] * block + at % block).to(dev)
+    big = torch.tensor([700, 2222]) if sign > 0 else at
+    k = torch.zeros(n, heads, dim)
+    k[big, :, 5] = 2.0 ** power
+    v = torch.randn(n, heads, dim, generator=g) * torch.exp2(torch.randint(-12, 13, (n // block + 1, 1, 1), generator=g).float())[at // block]
+    ops.cache_write(k.to(dev), v.to(dev), *pool, slots)
+    kk, vv = (x.double() for x in ops.cache_read(*pool, slots, torch.float32))
+    assert torch.equal(kk.cpu(), k.double())
+    q = torch.zeros(1, heads * 3, dim)
+    q[:, :, 5] = 1.37
+    q = q.to(dtype).to(dev)
+    lens, table = torch.tensor([n], dtype=torch.int32, device=dev), order[None].int().to(dev)
+    out, lse = ops.cache_attention(q, *pool, table, lens, scale=sign, want_lse=True)
+    vv = vv[big.to(dev)].repeat_interleave(3, 1)
+    want, mean = vv.mean(0), vv.abs().mean(0)
+    tol = half_ulp(dtype) * want.abs() + (2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -18) * mean + n * 2.0 ** -34 * vv.abs().amax()
+    assert torch.all((out[0].double() - want).abs() <= tol)
+    logit = sign * float(q[0, 0, 5]) * 2.0 ** power
+    assert torch.all((lse.double() - (logit + math.log(len(big)))).abs() <= 2.0 ** -21 * abs(logit) + 2.0 ** -20)
+
+
 def test_attention_nan_and_bad_pages(dev):
     """A NaN block reaches the rows that see it and no others; a table entry outside the pool reads as
     NaN; queries with a NaN or an infinity stay in their row."""
