@@ -14,11 +14,13 @@
 // of the first product with tokens by rows and go into the second with tokens by pairs: one
 // 8 x 8 transposition (movmatrix) per 8 tokens.
 //
-// Precision: a query row is brought to [2^14, 2^15) by a power of two, the weights to at most
-// 2^15, and both are rounded to fp16 once for bf16 queries (2^-12, against 2^-9 of the
-// output's own rounding; a bf16 query is exact in fp16).  fp16 and fp32 queries take two fp16
-// terms each, hi + lo (22 bits), at twice the products; there the products of one step are also
-// summed apart and added in fp32 with rounding, because the tensor core's own sums truncate.
+// Precision: a query row is brought to [2^14, 2^15) by a power of two; a bf16 row is exact in fp16,
+// fp16 and fp32 rows take two fp16 terms, hi + lo (22 bits).  The weights, at most 2^15, take two terms
+// for every type: in one (11 bits) they put a bf16 output off by about 1.4e-4 before its own rounding, which flipped
+// the last bit of one output in forty.  The products of one step are summed apart and added in fp32
+// with rounding, because the tensor core's own sums truncate and a warp may take thousands of
+// steps.  (Second term and additions for bf16: 1 x 512 tokens 8.7 -> 8.0 us, on fewer warps; 16 ragged
+// sequences 20.5 -> 21.7; 32 of up to 32768 tokens 187 -> 192; 131072 tokens x 4 queries 57 -> 71.)
 //
 // The references m, m' only move when a logit passes them by more than 2^kSlack, so a step
 // usually costs one vote instead of the reductions and the rescaling.
@@ -47,11 +49,12 @@ constexpr float kNone = -3.402823466e38f;   // the reference of a row that has s
 constexpr float kSlack = 6.f;     // weights may pass their reference by 2^kSlack
 constexpr float kTop = 9.f;       // and stand at 2^kTop there: at most 2^15 in fp16
 
-// Warps and ring stages of a CTA, by what registers and shared memory allow: 12 x 2 steps of
-// 8 KB for 8 query rows in one term, 8 x 3 with twice the registers, and 8 x 2 where the ring
-// shares shared memory with the query rows of two tiles in two terms.
-__host__ __device__ constexpr int att_warps(int nt, int terms) { return nt * terms == 1 ? 12 : 8; }
-__host__ __device__ constexpr int att_stages(int nt, int terms) { return nt * terms == 1 || nt * terms == 4 ? 2 : 3; }
+// Warps and ring stages of a CTA, by what registers and shared memory allow: 8 x 3 steps of
+// 8 KB, 8 x 2 where the ring shares shared memory with the query rows of two tiles in two terms.
+// 64 dimensions and 8 query rows in one term fit 168 registers: 12 warps (16 sequences of 8192
+// tokens: 35 us with 8 warps, 31 with 12; 128 dimensions spill so: 1 x 512 tokens 9.3 us, with 8 warps 7.9).
+__host__ __device__ constexpr int att_warps(int D, int nt, int terms) { return D == 64 && nt * terms == 1 ? 12 : 8; }
+__host__ __device__ constexpr int att_stages(int nt, int terms) { return nt * terms == 4 ? 2 : 3; }
 // Two row tiles in two terms: the query rows (64 registers) stand in shared memory instead, so
 // that little spills (131072 tokens x 4 fp32 queries: 91 -> 87 us).
 __host__ __device__ constexpr bool att_queries_shared(int nt, int terms) { return nt * terms == 4; }
@@ -280,10 +283,10 @@ struct Entry {     // a piece of a unit that ended in this CTA without being the
   const float* part;
 };
 
-// NT tiles of 8 query rows share the codes that a warp has converted; kTerms fp16 terms.
+// NT tiles of 8 query rows share the codes that a warp has converted; kTerms fp16 terms of a query.
 template <int D, int kFmt, int NT, int kTerms>
-__global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const AttArgs p) {
-  constexpr int kWarps = att_warps(NT, kTerms), kStages = att_stages(NT, kTerms);
+__global__ void __launch_bounds__(att_warps(D, NT, kTerms) * 32, 1) k_attend(const AttArgs p) {
+  constexpr int kWarps = att_warps(D, NT, kTerms), kStages = att_stages(NT, kTerms);
   constexpr int kSteps16 = D / 16;               // k16 steps of the logit product
   constexpr int kTiles = D / 16;                 // m16 tiles of the output
   constexpr int kStageBytes = 2 * kAttStep * D;  // K then V
@@ -672,7 +675,7 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
 #pragma unroll
               for (int u = 0; u < 2; ++u) { sc[nt][u][r] -= shift[nt][r]; sc[nt][u][2 + r] -= shift[nt][r]; }
         }
-        uint32_t pf[NT][kTerms][2][2];
+        uint32_t pf[NT][2][2][2];   // [term]
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -689,18 +692,13 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
               for (int e = 0; e < 4; ++e)
                 if (sc[nt][u][e] == -INFINITY) w[e] = 0.f;
             }
-            if constexpr (kTerms == 1) {
-              pf[nt][0][u][0] = transpose8(half2_bits(w[0], w[1]));
-              pf[nt][0][u][1] = transpose8(half2_bits(w[2], w[3]));
-            } else {
-              uint32_t h0, l0, h1, l1;
-              split2(w[0], w[1], h0, l0);
-              split2(w[2], w[3], h1, l1);
-              pf[nt][0][u][0] = transpose8(h0);
-              pf[nt][0][u][1] = transpose8(h1);
-              pf[nt][1][u][0] = transpose8(l0);
-              pf[nt][1][u][1] = transpose8(l1);
-            }
+            uint32_t h0, l0, h1, l1;
+            split2(w[0], w[1], h0, l0);
+            split2(w[2], w[3], h1, l1);
+            pf[nt][0][u][0] = transpose8(h0);
+            pf[nt][0][u][1] = transpose8(h1);
+            pf[nt][1][u][0] = transpose8(l0);
+            pf[nt][1][u][1] = transpose8(l1);
           }
         // values: lane (g, t) takes dims g * 2 kTiles .. of tokens 2t, 2t + 1, 2t + 8, 2t + 9 of each 16
         uint32_t v[2][4][D / 32];
@@ -733,18 +731,13 @@ __global__ void __launch_bounds__(att_warps(NT, kTerms) * 32, 1) k_attend(const 
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float(&acc)[4] = o[nt][2 * e + h];
-              if constexpr (kTerms == 1) {
-                mma16816(acc, a[0][h], pf[nt][0][0][0], pf[nt][0][0][1]);
-                mma16816(acc, a[1][h], pf[nt][0][1][0], pf[nt][0][1][1]);
-              } else {
-                float d[4];
-                mma16816_zero(d, a[0][h], pf[nt][1][0][0], pf[nt][1][0][1]);
-                mma16816(d, a[1][h], pf[nt][1][1][0], pf[nt][1][1][1]);
-                mma16816(d, a[0][h], pf[nt][0][0][0], pf[nt][0][0][1]);
-                mma16816(d, a[1][h], pf[nt][0][1][0], pf[nt][0][1][1]);
+              float d[4];
+              mma16816_zero(d, a[0][h], pf[nt][1][0][0], pf[nt][1][0][1]);
+              mma16816(d, a[1][h], pf[nt][1][1][0], pf[nt][1][1][1]);
+              mma16816(d, a[0][h], pf[nt][0][0][0], pf[nt][0][0][1]);
+              mma16816(d, a[1][h], pf[nt][0][1][0], pf[nt][0][1][1]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) acc[k] += d[k];
-              }
+              for (int k = 0; k < 4; ++k) acc[k] += d[k];
             }
         }
         __syncwarp();   // the stage may be filled again
@@ -963,14 +956,14 @@ size_t attention_workspace_bytes(int head_dim, int rows) {
 
 template <int D, int kFmt, int NT, int kTerms>
 static cudaError_t att_launch(AttArgs& p, void* ws, cudaStream_t st) {
-  constexpr size_t smem = (size_t)att_warps(NT, kTerms) * (att_stages(NT, kTerms) * 2 * kAttStep * D + att_query_bytes(NT, kTerms, D));
+  constexpr size_t smem = (size_t)att_warps(D, NT, kTerms) * (att_stages(NT, kTerms) * 2 * kAttStep * D + att_query_bytes(NT, kTerms, D));
   static_assert(att_stages(NT, kTerms) * 2 * kAttStep * D >= part_floats(D, 8 * NT) * 4, "a warp's ring holds one partial result");
-  static_assert(att_warps(NT, kTerms) <= kAttMaxWarps, "workspace slots");
+  static_assert(att_warps(D, NT, kTerms) <= kAttMaxWarps, "workspace slots");
   p.ws = static_cast<float*>(ws);
   p.desc = reinterpret_cast<int4*>(p.ws + (size_t)kAttMaxCtas * (kAttMaxWarps + 2) * part_floats(D, 8 * NT));
   auto fn = k_attend<D, kFmt, NT, kTerms>;
   if (cudaError_t e = ensure_dynamic_smem((const void*)fn, smem); e != cudaSuccess) return e;
-  if (cudaError_t e = launch_after(fn, dim3(p.ctas), att_warps(NT, kTerms) * 32, smem, st, p); e != cudaSuccess) return e;
+  if (cudaError_t e = launch_after(fn, dim3(p.ctas), att_warps(D, NT, kTerms) * 32, smem, st, p); e != cudaSuccess) return e;
   return launch_after(k_attend_merge<D, NT>, dim3(p.ctas), kMergeThreads, 0, st, p);
 }
 

@@ -604,6 +604,66 @@ def test_attention_logits_of_any_size(dev, power, dtype, sign):
     assert torch.all((lse.double() - (logit + math.log(len(big)))).abs() <= 2.0 ** -21 * abs(logit) + 2.0 ** -20)
 
 
+def _half_step(x, t):
+    """Half the distance of the numbers of type t around x (float64), exactly."""
+    _, e = torch.frexp(x)                                # |x| in [2^(e - 1), 2^e)
+    return torch.finfo(t).eps / 2 * torch.exp2((e - 1).double())
+
+
+@pytest.mark.parametrize("fmt", [E4M3, INT8])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,group,queries", [(128, 4, 1), (64, 4, 1), (128, 4, 3), (64, 2, 5)])
+def test_attention_is_rounded_once(dev, dim, group, queries, dtype, fmt):
+    """An output is its 64-bit value to half a step of its type, and little more: the weights carry 22 bits for
+    every type of query.  With small logits delta of the header is 2^-20 (1 + scale * mass), which moves an output by
+    2 delta sum_j p_j |v_j|; two fp16 terms put a weight off by 2^-22 of itself, or by 2^-25 where the second is subnormal,
+    that is 2^-33 of the largest (at 2^8 or more), and a sum over at most 17 steps by 17 * 2^-24."""
+    lens = [64, 200, 33, 512, 7, 100] * 8
+    pool, tables, n, q, k, v = _attention_case(dev, lens, 4, group, dim, 16, fmt, dtype, [queries] * len(lens))
+    q = (q.double() * 0.02).to(dtype)
+    cu = torch.arange(0, queries * len(lens) + 1, queries, dtype=torch.int32, device=dev)
+    out, lse = ops.cache_attention(q, *pool, tables, n, cu=cu, max_q=queries, want_lse=True)
+    b, scale = 0, dim ** -0.5
+    for r, m in enumerate(lens):
+        qq, kk, vv = q[r * queries:(r + 1) * queries].double(), k[b:b + m], v[b:b + m]
+        want, wl = ref.attention(qq, kk, vv, scale, True)
+        mean, _ = ref.attention(qq, kk, vv.abs(), scale, True)
+        mass = torch.einsum("mhd,nhd->mhn", qq.abs(), kk.abs().repeat_interleave(group, 1)).amax(-1)
+        delta = 2.0 ** -20 * (1 + scale * mass)
+        tol = (2 * delta + 2.0 ** -21 + 17 * 2.0 ** -24)[..., None] * mean + m * 2.0 ** -33 * vv.abs().amax()
+        got, gl = out[r * queries:(r + 1) * queries].double(), lse[r * queries:(r + 1) * queries].double()
+        off = (got - want).abs() - _half_step(want, dtype) - tol
+        assert float(off.max()) <= 0, (r, m, float(off.max()))
+        assert torch.all((gl - wl).abs() <= delta + 2.0 ** -23 * wl.abs())
+        b += m
+
+
+@pytest.mark.parametrize("fmt,dtype", [(E4M3, torch.bfloat16), (INT8, torch.float32)])
+@pytest.mark.parametrize("heads,group,dim,block,lens,queries", [
+    (8, 2, 64, 16, [150000, 900], [1, 1]), (8, 2, 64, 32, [300000], [1]), (4, 4, 128, 16, [70, 240000], [1, 3])])
+def test_attention_long_pieces(dev, heads, group, dim, block, lens, queries, fmt, dtype):
+    """Warps with more than 32 blocks of one unit, whose list of block ids is read on (16 steps of two blocks each, or
+    32 steps of one).  On top of the header's bounds up to 80 steps' sums in fp32, each rounded by 2^-24."""
+    warps = 148 * (12 if dim == 64 and dtype == torch.bfloat16 and max(queries) == 1 else 8)
+    steps = sum(-(-n // 32) for n in lens) * heads // warps
+    assert (32 * block) // 32 < steps <= 80
+    pool, tables, n, q, k, v = _attention_case(dev, lens, heads, group, dim, block, fmt, dtype, queries)
+    cu = torch.tensor([0] + queries, device=dev).cumsum(0).int()
+    out, lse = ops.cache_attention(q, *pool, tables, n, cu=cu, max_q=max(queries), want_lse=True)
+    a = b = 0
+    for m, nq in zip(lens, queries):
+        qq, kk, vv = q[a:a + nq].double(), k[b:b + m], v[b:b + m]
+        want, wl = ref.attention(qq, kk, vv, dim ** -0.5, True)
+        mean, _ = ref.attention(qq, kk, vv.abs(), dim ** -0.5, True)
+        mass = torch.einsum("mhd,nhd->mhn", qq.abs(), kk.abs().repeat_interleave(group, 1)).amax(-1)
+        delta = 2.0 ** -20 * (1 + dim ** -0.5 * mass) + 80 * 2.0 ** -24
+        tol = (2 * delta)[..., None] * mean + m * 2.0 ** -33 * vv.abs().amax()
+        assert torch.all((out[a:a + nq].double() - want).abs() <= _half_step(want, dtype) + tol)
+        assert torch.all((lse[a:a + nq].double() - wl).abs() <= delta + 2.0 ** -23 * wl.abs())
+        a, b = a + nq, b + m
+    assert torch.equal(ops.cache_attention(q, *pool, tables, n, cu=cu, max_q=max(queries)), out)
+
+
 def test_attention_nan_and_bad_pages(dev):
     """A NaN block reaches the rows that see it and no others; a table entry outside the pool reads as
     NaN; queries with a NaN or an infinity stay in their row."""
@@ -634,6 +694,20 @@ def test_attention_nan_and_bad_pages(dev):
     assert torch.isnan(out[5, 0]).all() and torch.equal(out[5, 1], clean[5, 1]) and torch.isnan(out[9, 1]).all()
     keep = [i for i in range(12) if i not in (5, 9)]
     assert torch.equal(out[keep], clean[keep])
+
+
+def test_attention_nan_values_that_nobody_sees(dev):
+    """As the 17-token case above with NaN value scales: a block that holds only the last new token's values
+    does not reach the rows that do not see it."""
+    for fmt, dtype in ((INT8, torch.bfloat16), (E4M3, torch.float32)):
+        lens = [17, 64, 64]
+        pool, tables, n, q, k, v = _attention_case(dev, lens, 1, 2, 128, 16, fmt, dtype, [4] * 3)
+        cu = torch.tensor([0, 4, 8, 12], dtype=torch.int32, device=dev)
+        clean = ops.cache_attention(q, *pool, tables, n, cu=cu, max_q=4)
+        pool[3][tables[0, 1]] = math.nan
+        out, lse = ops.cache_attention(q, *pool, tables, n, cu=cu, max_q=4, want_lse=True)
+        assert torch.equal(out[:3], clean[:3]) and torch.isnan(out[3]).all() and torch.equal(out[4:], clean[4:])
+        assert torch.isfinite(lse).all()            # the keys are sound
 
 
 def test_attention_lengths_that_do_not_fit(dev):
