@@ -165,3 +165,43 @@ def test_rotary_frequencies():
     for dim in (0, 3):
         with pytest.raises(ValueError):
             rotary_frequencies(dim)
+
+
+def _yarn(dim, base, s):
+    """YaRN's frequencies pair by pair, in Python floats."""
+    by, n = s["factor"], s["original_max_position_embeddings"]
+    where = [dim * math.log(n / (2 * math.pi * t)) / (2 * math.log(base)) for t in (s.get("beta_fast", 32), s.get("beta_slow", 1))]
+    if s.get("truncate", True):
+        where = [math.floor(where[0]), math.ceil(where[1])]
+    lo, hi = max(where[0], 0), min(where[1], dim - 1)
+    out = []
+    for i in range(dim // 2):
+        f = base ** (-2 * i / dim)
+        stretch = min(max((i - lo) / (hi - lo), 0.0), 1.0)
+        out.append(f * (1 - stretch) + f / by * stretch)
+    return torch.tensor(out, dtype=torch.float64)
+
+
+@pytest.mark.parametrize("dim,base,extra", [
+    (64, 150000.0, dict(factor=32.0, beta_fast=32.0, beta_slow=1.0, truncate=False)), (64, 150000.0, dict(factor=32.0, truncate=True)),
+    (128, 10000.0, dict(factor=40.0)), (64, 10000.0, dict(factor=40.0, beta_fast=32, beta_slow=1, mscale=1.0, mscale_all_dim=1.0)),
+    (64, 10000.0, dict(factor=40.0, mscale=0.707, mscale_all_dim=1.0)), (64, 10000.0, dict(factor=4.0, mscale=None, mscale_all_dim=0))])
+def test_yarn_dictionaries(dim, base, extra):
+    """Each key of a config's dictionary has its effect: the ramp between fractional or whole pairs, and
+    the factor on cosine and sine."""
+    s = dict(rope_type="yarn", original_max_position_embeddings=4096, **extra)
+    got, factor = rotary_frequencies(dim, base, s)
+    assert torch.allclose(got, _yarn(dim, base, s), rtol=1e-12, atol=0)
+    m = lambda x: 0.1 * x * math.log(extra["factor"]) + 1.0   # noqa: E731
+    want = m(extra["mscale"]) / m(extra["mscale_all_dim"]) if extra.get("mscale") else m(1.0)
+    assert math.isclose(factor, want, rel_tol=1e-14)
+
+
+def test_rope_scaling_keys_that_would_be_lost_are_refused():
+    yarn = dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=4096)
+    for bad in (dict(mscale=0.7), dict(mscale_all_dim=1.0), dict(short_factor=[1.0]), dict(beta=32.0),
+                dict(rope_theta=500000.0)):
+        with pytest.raises(ValueError):
+            rotary_frequencies(64, scaling={**yarn, **bad})
+    same = rotary_frequencies(64, scaling={**yarn, "rope_theta": 10000, "finetuned": True, "mrope_section": [16, 24, 24], "partial_rotary_factor": 0.5, "beta_fast": None})
+    assert torch.equal(same[0], rotary_frequencies(64, scaling=yarn)[0])
