@@ -153,8 +153,8 @@ class PagedKVCache:
         """Blocks, slots and positions for ``new`` int32 ``[max_requests]`` tokens per request (0: none,
         negative: the request ends and frees its blocks).  ``total``: token rows of this step's
         tensors (default ``max_requests * max_q``, rows past the sum of ``new`` are padding);
-        ``max_q``: the most tokens of one request.  A request that does not fit gets none
-        (``step.tables.granted``)."""
+        ``max_q``: the most tokens of one request (the attention of a request with more is NaN).  A request
+        that does not fit gets none (``step.tables.granted``)."""
         total = self.lens.shape[0] * max_q if total is None else int(total)
         t = ops.block_tables(self.lens, new, self.tables, self.free_list, self.free_count, self.block_size, total,
                              shift=self.shift)

@@ -151,14 +151,20 @@ CKV_DEV int seq_len(const AttArgs& p, int r) {
   const long long cap = (long long)p.a.table_width << p.block_log2;
   return (int)min(min((long long)max(p.a.lens[r], 0), cap), (long long)INT32_MAX - 2 * kAttStep);
 }
-CKV_DEV void seq_queries(const AttArgs& p, int r, int& q0, int& nq) {
+// A sequence's query rows, as many as there are; and those that are computed: none of a sequence that
+// has more than max_q.
+CKV_DEV void seq_rows(const AttArgs& p, int r, int& q0, int& rows) {
   if (p.a.cu) {
     q0 = min(max(p.a.cu[r], 0), p.a.tokens);
-    nq = min(max(min(p.a.cu[r + 1], p.a.tokens) - q0, 0), p.a.max_q);
+    rows = max(min(p.a.cu[r + 1], p.a.tokens) - q0, 0);
   } else {
     q0 = r;
-    nq = 1;
+    rows = 1;
   }
+}
+CKV_DEV void seq_queries(const AttArgs& p, int r, int& q0, int& nq) {
+  seq_rows(p, r, q0, nq);
+  if (nq > p.a.max_q) nq = 0;
 }
 CKV_DEV uint32_t steps_of(int n) { return (uint32_t)(n + kAttStep - 1) / kAttStep; }
 template <int NT> CKV_DEV uint32_t seq_units(const AttArgs& p, int nq) {
@@ -882,18 +888,21 @@ __global__ void __launch_bounds__(att_warps(D, NT, kTerms) * 32, 1) k_attend(con
     p.desc[cta] = make_int4(0, 0, 0, 0);
   }
 
-  // sequences with nothing to see: zeros
-  for (int r = cta; r < R; r += gridDim.x)
-    if (seq_len(p, r) == 0) {
-      int q0, nq;
-      seq_queries(p, r, q0, nq);
-      const int hq = p.c.num_kv_heads * p.group;
-      for (int i = tid; i < nq * hq * (D / 4); i += kWarps * 32) {
-        const int row = i / (D / 4), d = i % (D / 4) * 4, tok = q0 + row / hq, h = row % hq;
-        store_out4(p.a.out, p.a.dtype, tok * p.a.out_tok_stride + h * p.a.out_head_stride + d, make_float4(0.f, 0.f, 0.f, 0.f));
-        if (p.a.lse && d == 0) p.a.lse[(int64_t)tok * hq + h] = -INFINITY;
+  // sequences with nothing to see: zeros; with more rows than max_q: NaN
+  for (int r = cta; r < R; r += gridDim.x) {
+    int q0, rows;
+    seq_rows(p, r, q0, rows);
+    const bool many = rows > p.a.max_q;
+    if (!many && seq_len(p, r) != 0) continue;
+    const int hq = p.c.num_kv_heads * p.group;
+    const float x = many ? __uint_as_float(0x7fffffffu) : 0.f;
+    for (int tok = q0; tok < q0 + rows; ++tok)
+      for (int i = tid; i < hq * (D / 4); i += kWarps * 32) {
+        const int h = i / (D / 4), d = i % (D / 4) * 4;
+        store_out4(p.a.out, p.a.dtype, tok * p.a.out_tok_stride + h * p.a.out_head_stride + d, make_float4(x, x, x, x));
+        if (p.a.lse && d == 0) p.a.lse[(int64_t)tok * hq + h] = many ? x : -INFINITY;
       }
-    }
+  }
 }
 
 // CTA c merges the unit that begins in CTA c of k_attend and reaches past it: its slot 1 and

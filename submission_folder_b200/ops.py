@@ -587,8 +587,8 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """Attention of the new query tokens ``q`` ``[T, H, D]`` over a paged 8-bit cache
     (``ckv_cache_attention``), reading each code once; meant for a few query tokens per sequence.
 
-    Sequence ``r`` has query rows ``cu[r] .. cu[r + 1]`` (int32 ``[R + 1]``, at most ``max_q`` each;
-    None: one row each) and ``lens[r]`` cached tokens (int32 ``[R]``, the new ones included) in the
+    Sequence ``r`` has query rows ``cu[r] .. cu[r + 1]`` (int32 ``[R + 1]``, at most ``max_q`` each: the
+    rows of a sequence with more are NaN; None: one row each) and ``lens[r]`` cached tokens (int32 ``[R]``, the new ones included) in the
     blocks ``tables[r]`` (int32 ``[R, width]``).  ``causal``: the new tokens see one another in order.
     Query head ``h`` reads KV head ``h // (H // Hkv)``.  ``scale`` defaults to ``D ** -0.5``.  A row that
     sees nothing gives zeros (log-sum-exp -inf); rows past ``cu[R]`` are left as they were (in

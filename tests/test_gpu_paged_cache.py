@@ -710,6 +710,24 @@ def test_attention_nan_values_that_nobody_sees(dev):
         assert torch.isfinite(lse).all()            # the keys are sound
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_of_more_rows_than_max_q_is_nan(dev, dtype):
+    """The rows of a sequence with more query tokens than the call allows for are marked, all of them; the
+    other sequences are right and the padding is left alone."""
+    lens, queries = [100, 40, 0, 70], [2, 5, 3, 1]
+    pool, tables, n, q, k, v = _attention_case(dev, lens, 2, 4, 128, 16, E4M3, dtype, queries)
+    q = torch.cat([q, q[:2]])
+    cu = torch.tensor([0] + queries, device=dev).cumsum(0).int()
+    out = torch.full_like(q, 7.0)
+    got, lse = ops.cache_attention(q, *pool, tables, n, cu=cu, max_q=2, want_lse=True, out=out)
+    assert torch.isnan(got[2:10]).all() and torch.isnan(lse[2:10]).all()
+    # the others by the header's bounds (a larger max_q cuts the line of work elsewhere, so that sums in fp32
+    # come in another order: no other call gives the same bits)
+    _attention_check(got[:2], lse[:2], q[:2], k[:100], v[:100], [100], [2], 128 ** -0.5, True)
+    _attention_check(got[10:11], lse[10:11], q[10:11], k[140:], v[140:], [70], [1], 128 ** -0.5, True)
+    assert torch.all(got[11:] == 7.0)
+
+
 def test_attention_lengths_that_do_not_fit(dev):
     """Lengths below zero count as zero, lengths past the table as the table's; ``cu`` past the rows
     or falling leaves rows out, without a fault."""
