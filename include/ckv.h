@@ -412,7 +412,8 @@ typedef struct ckv_cache {
  * Outputs: out_lens; out_free_count; out_cu [requests + 1], the tokens asked for before each
  * request; per token t < total: out_slots (-1 for a refused request's tokens and for t past
  * out_cu[requests]) and out_positions = place in the request + shift[r] (0 past the end);
- * out_granted [requests].  out_lens may be lens and out_free_count may be free_count; called
+ * out_granted [requests]; out_seen [requests] (may be NULL): out_lens, but 0 for a refused request, as
+ * the lengths for the attention of the step's tokens.  out_lens may be lens and out_free_count may be free_count; called
  * again on the same lens and free_count, the step gives the same outputs. */
 typedef struct ckv_table_step {
   const int32_t* lens;
@@ -435,6 +436,7 @@ typedef struct ckv_table_step {
   int32_t* out_granted;
   int32_t* work;               /* [3 * requests + 4], scratch; may be NULL when requests + total is at
                                   most CKV_TABLES_SMALL */
+  int32_t* out_seen;
 } ckv_table_step;
 enum { CKV_TABLES_SMALL = 4096 };
 int ckv_block_tables(const ckv_table_step* step, ckv_stream_t stream);

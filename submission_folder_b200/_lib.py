@@ -116,7 +116,7 @@ class TableStep(ctypes.Structure):
         ("block_size", ctypes.c_int32), ("requests", ctypes.c_int32), ("total", ctypes.c_int32),
         ("out_lens", ctypes.c_void_p), ("out_free_count", ctypes.c_void_p), ("out_cu", ctypes.c_void_p),
         ("out_slots", ctypes.c_void_p), ("out_positions", ctypes.c_void_p), ("out_granted", ctypes.c_void_p),
-        ("work", ctypes.c_void_p),
+        ("work", ctypes.c_void_p), ("out_seen", ctypes.c_void_p),
     ]
 
 

@@ -167,8 +167,9 @@ class PagedKVCache:
 
     def attend(self, layer_idx: int, query_states: torch.Tensor, step: CacheStep, scale: Optional[float] = None,
                want_lse: bool = False):
-        """Attention of this step's queries ``[T, H, D]`` over layer ``layer_idx``; rows of padding are zeros."""
-        return ops.cache_attention(query_states, *self.layer(layer_idx), self.tables, step.tables.lens, cu=step.tables.cu,
+        """Attention of this step's queries ``[T, H, D]`` over layer ``layer_idx``; rows of padding and of
+        requests that did not fit are zeros."""
+        return ops.cache_attention(query_states, *self.layer(layer_idx), self.tables, step.tables.seen, cu=step.tables.cu,
                                    max_q=step.max_q, scale=scale, want_lse=want_lse,
                                    out=torch.zeros_like(query_states, memory_format=torch.contiguous_format))
 

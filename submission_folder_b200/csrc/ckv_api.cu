@@ -893,7 +893,7 @@ int ckv_block_tables(const ckv_table_step* s, ckv_stream_t stream) {
       (!s->work && (int64_t)s->requests + s->total > CKV_TABLES_SMALL))
     return fail(CKV_ERR_ARG, "null argument");
   if (!aligned_to(4, {s->lens, s->new_tokens, s->shift, s->tables, s->free_list, s->free_count, s->out_lens, s->out_free_count,
-                      s->out_cu, s->out_granted, s->work}) ||
+                      s->out_cu, s->out_granted, s->out_seen, s->work}) ||
       !aligned_to(8, {s->out_slots, s->out_positions}))
     return fail(CKV_ERR_ARG, "pointers must be aligned to their elements");
   if (s->requests < 1 || s->requests > kMaxRequests) return fail(CKV_ERR_ARG, "1 to 8192 requests");

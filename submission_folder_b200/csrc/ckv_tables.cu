@@ -172,10 +172,12 @@ __global__ void __launch_bounds__(kTabThreads) k_block_tables(const ckv_table_st
       else give[r] = -1;
     }
     const int granted = max(give[r], 0);
+    const bool refused = was != -2 && give[r] < 0;
     give[r] = granted;
     s.out_cu[r] = cu[r];
     s.out_granted[r] = granted;
     s.out_lens[r] = was == -2 ? 0 : len[r] + granted;
+    if (s.out_seen) s.out_seen[r] = was == -2 || refused ? 0 : len[r] + granted;
   }
   __syncthreads();
   const int taken = s_taken;

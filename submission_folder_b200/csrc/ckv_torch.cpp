@@ -91,7 +91,7 @@ CKV_FN(block_tables) {
       !fits(block) || !fits(R) || !fits(tables->size(1)) || !fits(list->numel()))
     return none();
   const auto i32 = lens->options(), i64 = i32.dtype(at::kLong);
-  Tensor cu = at::empty({R + 1}, i32), granted = at::empty({R}, i32);
+  Tensor cu = at::empty({R + 1}, i32), granted = at::empty({R}, i32), seen = at::empty({R}, i32);
   Tensor slots = at::empty({total}, i64), positions = at::empty({total}, i64);
   Tensor work;
   if (R + total > CKV_TABLES_SMALL) work = at::empty({3 * R + 4}, i32);
@@ -100,11 +100,11 @@ CKV_FN(block_tables) {
                             table_stride(tables), (int32_t)width, ptr<int32_t>(list), (int32_t)list->numel(),
                             ptr<int32_t>(count), (int32_t)block, (int32_t)R, (int32_t)total, ptr<int32_t>(lens_out),
                             ptr<int32_t>(count_out), ptr<int32_t>(&cu), ptr<int64_t>(&slots), ptr<int64_t>(&positions),
-                            ptr<int32_t>(&granted), work.defined() ? ptr<int32_t>(&work) : nullptr};
+                            ptr<int32_t>(&granted), work.defined() ? ptr<int32_t>(&work) : nullptr, ptr<int32_t>(&seen)};
   const int rc = call(dev, [&](ckv_stream_t st) { return ckv_block_tables(&s, st); });
   if (rc) return status(rc);
-  return Py_BuildValue("(NNNNNN)", THPVariable_Wrap(*lens_out), THPVariable_Wrap(*count_out), THPVariable_Wrap(cu),
-                       THPVariable_Wrap(slots), THPVariable_Wrap(positions), THPVariable_Wrap(granted));
+  return Py_BuildValue("(NNNNNNN)", THPVariable_Wrap(*lens_out), THPVariable_Wrap(*count_out), THPVariable_Wrap(cu),
+                       THPVariable_Wrap(slots), THPVariable_Wrap(positions), THPVariable_Wrap(granted), THPVariable_Wrap(seen));
   END_HANDLE_TH_ERRORS
 }
 

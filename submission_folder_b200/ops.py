@@ -466,7 +466,7 @@ def _failed(name: str, rc) -> None:
 
 
 class TableStep(NamedTuple):
-    """What ``block_tables`` says of a step: per request ``lens`` (after it) and ``granted``, the
+    """What ``block_tables`` says of a step: per request ``lens`` (after it), ``granted`` and ``seen``, the
     free count, ``cu`` (first token of each request), and each token's slot and position."""
 
     lens: torch.Tensor         # int32 [R]
@@ -475,6 +475,7 @@ class TableStep(NamedTuple):
     slots: torch.Tensor        # int64 [total], -1: no token
     positions: torch.Tensor    # int64 [total]
     granted: torch.Tensor      # int32 [R]
+    seen: torch.Tensor         # int32 [R], lens but 0 for a refused request: ``cache_attention``'s lens of this step
 
 
 def block_tables(lens: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, free_list: torch.Tensor,
@@ -488,7 +489,8 @@ def block_tables(lens: torch.Tensor, new: torch.Tensor, tables: torch.Tensor, fr
     unless ``lens_out`` / ``free_count_out`` take them.  ``total``: the number of token rows in
     this step's tensors, at least the sum of ``new`` where a token's slot matters; rows past the
     sum get slot -1.  ``shift`` int32 ``[R]`` is added to the positions (the number of tokens
-    evicted from the request).  A request that does not fit gets slots of -1 and ``granted`` 0.
+    evicted from the request).  A request that does not fit gets slots of -1, ``granted`` 0
+    and ``seen`` 0, so that its query rows attend to nothing.
     """
     r = _lib.torch_calls().block_tables(lens, new, tables, free_list, free_count, block_size, total, shift, lens_out,
                                         free_count_out)

@@ -1032,6 +1032,61 @@ def test_positions_of_a_row_that_is_used_again(dev):
     assert c.read(0, 0, 64)[0].shape == (1, 2, 64, 64) and c.read(0, 1, 0)[0].shape == (1, 2, 0, 64)
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_refused_requests_attend_to_nothing(dev, captured):
+    """A request that gets no room, for lack of blocks or of places in its row, gives zeros from ``decode``
+    while it keeps its length; the others, one refused earlier among them, go on as if it had not asked."""
+    D, R = 64, 4
+    new = torch.zeros(R, dtype=torch.int32, device=dev)
+    g = torch.Generator(device=dev).manual_seed(2)
+    x = [torch.zeros(2 * R, h, D, dtype=torch.bfloat16, device=dev) for h in (4, 2, 2)]
+
+    def run(c):
+        step = c.step(new, max_q=2)
+        return c.decode(0, *x, step), step
+
+    def fresh():
+        c = PagedKVCache(1, 7, R, 48, 2, D, 16, device=dev)
+        for r, n in enumerate((30, 46, 16, 16)):
+            z = torch.randn(1, 2, n, D, generator=torch.Generator().manual_seed(r)).bfloat16().to(dev)
+            assert int(c.admit(r, [(z, z)], n).tables.granted[r]) == n
+        return c
+
+    c, want = fresh(), fresh()
+    # (asked, granted): 0 blocks left; then one comes back with request 2's end
+    steps = [((1, 2, 1, 2), (1, 2, 0, 0)), ((1, 1, 0, 1), (1, 0, 0, 0)), ((0, 0, -1, 1), (0, 0, 0, 1)), ((2, 1, 1, 2), (0, 0, 0, 2))]
+    if captured:
+        run(fresh())
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got, step = run(c)
+    for asked, granted in steps:
+        for t in x:
+            t.normal_(generator=g)
+        new.copy_(torch.tensor(asked, dtype=torch.int32))
+        if captured:
+            graph.replay()
+        else:
+            got, step = run(c)
+        assert step.tables.granted.tolist() == list(granted)
+        a = 0
+        for r in range(R):
+            m = max(asked[r], 0)
+            if m and not granted[r]:
+                assert not got[a:a + m].any()
+            a += m
+        assert not got[a:].any()
+        # the same step without those that are refused
+        keep = [i for i, r in enumerate(r for r in range(R) for _ in range(max(asked[r], 0))) if granted[r]]
+        y = [torch.cat([t[keep], t[:2 * R - len(keep)]]) for t in x]
+        alone = want.step(torch.tensor([n if n < 0 else m for n, m in zip(asked, granted)], dtype=torch.int32, device=dev), max_q=2)
+        assert torch.equal(want.decode(0, *y, alone)[:len(keep)], got[keep])
+        assert torch.equal(want.lens, c.lens) and torch.equal(want.free_count, c.free_count)
+    if captured:
+        del graph
+
+
 def test_paged_cache_class_refusals(dev):
     c = PagedKVCache(1, 8, 2, 64, 2, 64, 16, device=dev)
     z = torch.zeros(1, 2, 20, 64, dtype=torch.bfloat16, device=dev)
