@@ -483,7 +483,7 @@ int ckv_cache_read(const ckv_cache* cache, void* k, void* v, int32_t dtype, cons
  * requests == tokens), lens[r] tokens in tables[r].  causal: query i of m sees the first
  * lens[r] - m + i + 1 tokens; a row that sees none gives 0 and lse -inf.  Query head h reads KV
  * head h / (q_heads / num_kv_heads).  lse (may be NULL): natural log of the sum of exponentials,
- * [tokens][q_heads] fp32.  Rows of q past cu[requests] are left alone.  A table entry outside the
+ * [tokens][q_heads] fp32.  Rows of q past cu[requests] are left alone; their lse is -inf.  A table entry outside the
  * pool reads as NaN.  Workspace: ckv_cache_attention_workspace bytes, 256-byte aligned. */
 typedef struct ckv_attention_args {
   const void* q;

@@ -888,6 +888,12 @@ __global__ void __launch_bounds__(att_warps(D, NT, kTerms) * 32, 1) k_attend(con
     p.desc[cta] = make_int4(0, 0, 0, 0);
   }
 
+  // log-sum-exp of rows of no sequence
+  if (p.a.lse && p.a.cu) {
+    const int64_t hq = p.c.num_kv_heads * p.group;
+    for (int64_t i = max(p.a.cu[R], 0) * hq + cta * kWarps * 32 + tid; i < p.a.tokens * hq; i += (int64_t)gridDim.x * kWarps * 32)
+      p.a.lse[i] = -INFINITY;
+  }
   // sequences with nothing to see: zeros; with more rows than max_q: NaN
   for (int r = cta; r < R; r += gridDim.x) {
     int q0, rows;

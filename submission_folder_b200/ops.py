@@ -594,7 +594,7 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     blocks ``tables[r]`` (int32 ``[R, width]``).  ``causal``: the new tokens see one another in order.
     Query head ``h`` reads KV head ``h // (H // Hkv)``.  ``scale`` defaults to ``D ** -0.5``.  A row that
     sees nothing gives zeros (log-sum-exp -inf); rows past ``cu[R]`` are left as they were (in
-    ``out``, if given).  Returns ``out``, or ``(out, lse)`` with ``want_lse``: natural-log
+    ``out``, if given; log-sum-exp -inf).  Returns ``out``, or ``(out, lse)`` with ``want_lse``: natural-log
     log-sum-exp, float32 ``[T, H]``.
     """
     r = _lib.torch_calls().cache_attention(q, k_cache, v_cache, k_scale, v_scale, tables, lens, cu, max_q, scale, causal,

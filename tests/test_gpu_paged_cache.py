@@ -728,6 +728,25 @@ def test_attention_of_more_rows_than_max_q_is_nan(dev, dtype):
     assert torch.all(got[11:] == 7.0)
 
 
+@pytest.mark.parametrize("pad", [1, 200])
+def test_lse_of_padding_rows(dev, pad):
+    """The log-sum-exp of rows of no sequence is -inf, whatever its memory held before."""
+    queries = [2, 0, 1]
+    pool, tables, n, q, k, v = _attention_case(dev, [40, 3, 5], 2, 4, 64, 16, INT8, torch.bfloat16, queries)
+    q = torch.cat([q, q[:1].repeat(pad, 1, 1)])
+    cu = torch.tensor([0] + queries, device=dev).cumsum(0).int()
+    for _ in range(3):
+        torch.full((q.shape[0], q.shape[1]), math.nan, device=dev)      # what the allocator gives next
+        _, lse = ops.cache_attention(q, *pool, tables, n, cu=cu, max_q=2, want_lse=True)
+        assert torch.isfinite(lse[:3]).all() and torch.all(lse[3:] == -math.inf)
+    c = PagedKVCache(1, 8, 3, 64, 2, 64, 16, device=dev)
+    step = c.step(torch.tensor([1, 0, 1], dtype=torch.int32, device=dev))
+    x = torch.ones(3, 2, 64, dtype=torch.bfloat16, device=dev)
+    c.write(0, x, x, step)
+    out, lse = c.attend(0, q[:3].contiguous(), step, want_lse=True)
+    assert torch.all(out[:2] == 1) and not out[2].any() and torch.isfinite(lse[:2]).all() and torch.all(lse[2] == -math.inf)
+
+
 def test_attention_lengths_that_do_not_fit(dev):
     """Lengths below zero count as zero, lengths past the table as the table's; ``cu`` past the rows
     or falling leaves rows out, without a fault."""
