@@ -468,7 +468,9 @@ int ckv_rotary(const ckv_rotary_args* args, ckv_stream_t stream);
  * slots.  Tokens of one block stand next to one another in the list (as ckv_block_tables
  * gives them); a slot outside the pool is no token; of a slot named twice in a row of such
  * neighbours the last token stays.  Neighbours that include a block's first place begin the
- * block anew; otherwise the block's other tokens stay, in the larger of its old and new scale. */
+ * block anew; otherwise the block's other tokens stay, in the larger of its old and new scale (an old
+ * one that is no power of two, as another program may have left it, is first rounded up to one; above
+ * 2^127 the block and head becomes NaN). */
 int ckv_cache_write(const ckv_cache* cache, const void* k, int64_t k_tok_stride, int64_t k_head_stride, const void* v,
                     int64_t v_tok_stride, int64_t v_head_stride, int32_t dtype, const int64_t* slots, int32_t tokens,
                     ckv_stream_t stream);

@@ -13,7 +13,8 @@
 // warps read the run's rows once into registers (16 rows per warp), the CTA agrees on the
 // largest magnitude, the block's scale follows, and the rows leave as codes.  A run that has
 // the block's first token begins the block anew; any other run keeps what the block holds,
-// rescaled when the scale grew.  One CTA per (run, head, K / V), so no atomics and the same
+// rescaled when the scale grew, or when another program left one that is no power of two (the next
+// one takes its place).  One CTA per (run, head, K / V), so no atomics and the same
 // result every time.
 //
 // Bound: HBM, (element size + 1) bytes per element, and the latency of a run's chain: 16 prompts of
@@ -38,20 +39,23 @@ template <int kFmt> CKV_DEV float scale_for(uint32_t amax_bits) {
   e = max(e, 1);   // 2^-126, also for zero and subnormal magnitudes
   return __uint_as_float((uint32_t)e << 23);
 }
-// 1 / scale of a power of two in [2^-126, 2^121].
-CKV_DEV float inv_pow2(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
+// 1 / scale of a power of two in [2^-126, 2^127] (a subnormal of the last).
+CKV_DEV float inv_pow2(float s) { return __uint_as_float(max((254u << 23) - __float_as_uint(s), 0x400000u)); }
+// The smallest power of two that is at least a positive s; infinity above 2^127.
+CKV_DEV float up_pow2(float s) { return __uint_as_float((__float_as_uint(s) + 0x7fffffu) & 0x7f800000u); }
 
-// Four codes from four values over the scale.
-// int8: adding 1.5 2^23 leaves the nearest whole number, ties to even, in the low byte.
-template <int kFmt> CKV_DEV uint32_t encode4(float a, float b, float c, float d) {
+// Four codes from four values over the scale, or (by) codes of another scale times its ratio to it.
+// int8: adding 1.5 2^23 leaves the nearest whole number, ties to even, in the low byte; with the
+// multiplication in one instruction, so that the product is not rounded first.
+template <int kFmt> CKV_DEV uint32_t encode4(float a, float b, float c, float d, float by = 1.f) {
   uint32_t r;
   if constexpr (kFmt == CKV_CACHE_E4M3) {
     asm("{\n.reg .b16 lo, hi;\ncvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\ncvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n"
-        "mov.b32 %0, {lo, hi};\n}\n" : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
+        "mov.b32 %0, {lo, hi};\n}\n" : "=r"(r) : "f"(a * by), "f"(b * by), "f"(c * by), "f"(d * by));
   } else {
     constexpr float kMagic = 12582912.f;
-    const uint32_t x = __float_as_uint(a + kMagic), y = __float_as_uint(b + kMagic);
-    const uint32_t z = __float_as_uint(c + kMagic), w = __float_as_uint(d + kMagic);
+    const uint32_t x = __float_as_uint(fmaf(a, by, kMagic)), y = __float_as_uint(fmaf(b, by, kMagic));
+    const uint32_t z = __float_as_uint(fmaf(c, by, kMagic)), w = __float_as_uint(fmaf(d, by, kMagic));
     r = __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
   }
   return r;
@@ -284,8 +288,8 @@ __global__ void __launch_bounds__(kCacheMaxBlock / kRowsPerWarp * 32) k_cache_wr
         for (int w = 0; w < nw; ++w) top = max(top, all[w]);
       }
       float scale = scale_for<kFmt>(top);
-      if (isnan(old) || isnan(scale)) scale = __uint_as_float(0x7fffffffu);
-      else scale = fmaxf(scale, old);
+      if (isnan(old) || isnan(scale) || isinf(up_pow2(old))) scale = __uint_as_float(0x7fffffffu);
+      else scale = fmaxf(scale, up_pow2(old));
       const bool bad = isnan(scale);
       const float inv = bad ? 0.f : inv_pow2(scale);
       auto put = [&](const Row16<T>& row, int o) {
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(kCacheMaxBlock / kRowsPerWarp * 32) k_cache_wr
           for (int e = 0; e < 4; ++e) {
             float f[4];
             decode4<kFmt>(w[e], f);
-            w[e] = encode4<kFmt>(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+            w[e] = encode4<kFmt>(f[0], f[1], f[2], f[3], ratio);
           }
           *p = make_uint4(w[0], w[1], w[2], w[3]);
         }

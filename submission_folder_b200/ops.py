@@ -549,7 +549,8 @@ def cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache
 
     A block's scale is the smallest power of two that holds its largest magnitude.  Tokens of one
     block stand next to one another in the list; if the block's first place is among them the block
-    begins anew, otherwise its other tokens stay (rescaled where the scale grew).  Slots outside the
+    begins anew, otherwise its other tokens stay (rescaled where the scale grew, or where another
+    program left one that is no power of two).  Slots outside the
     pool (-1) are no tokens.  A NaN or an infinity makes its block and head read as NaN.
     """
     r = _lib.torch_calls().cache_write(k, v, k_cache, v_cache, k_scale, v_scale, slots)

@@ -423,6 +423,39 @@ def test_cache_write_slots_named_again_and_again(dev, before, times):
     _check_pool(pool, refs, dim)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt", [E4M3, INT8])
+@pytest.mark.parametrize("exponent", [-126, -60, -5, 0, 30, 126, 127])
+@pytest.mark.parametrize("mantissa", [1.0, 1.0 + 2.0 ** -23, 1.3, 1.5, 2.0 - 2.0 ** -23])
+def test_cache_append_to_scales_of_other_programs(dev, fmt, dtype, exponent, mantissa):
+    """An append to a block whose scale is no power of two: the next one, or what the new rows need, takes its
+    place, and the held codes are brought to it by the true ratio and rounded once."""
+    block, dim, heads = 16, 64, 2
+    g = torch.Generator().manual_seed(exponent + 200)
+    old = float(torch.tensor(mantissa)) * 2.0 ** exponent         # as the fp32 scale holds it (1.3 is none)
+    codes = [round_to.clamp(-ref.LARGEST[fmt], ref.LARGEST[fmt]) for round_to in
+             (ref.round_code(torch.randn(heads, 3, dim, generator=g).double() * 100, fmt) for _ in range(2))]
+    pool = _pool(dev, 2, heads, block, dim, fmt)
+    for cache, scale, c in zip(pool[:2], pool[2:], codes):
+        cache[1, :, :3] = c.float().to(dev).to(fmt)
+        scale[1] = old
+    loud = torch.tensor([0.5, 4.0])[:, None] * min(old, 2.0 ** 100 if dtype != torch.float16 else 64.0) * 100    # the second head's scale grows
+    x = [(torch.randn(2, heads, dim, generator=g) * loud).to(dtype) for _ in range(2)]
+    ops.cache_write(x[0].to(dev), x[1].to(dev), *pool, torch.tensor([block + 3, block + 4], device=dev))
+    up = 2.0 ** exponent * (1 if mantissa == 1.0 else 2)
+    for cache, scale, c, rows in zip(pool[:2], pool[2:], codes, x):
+        got, sc = _codes64(cache)[1], scale[1].double().cpu()
+        for h in range(heads):
+            want = max(up, ref.block_scale(float(rows[:, h].abs().max()), fmt))
+            if up > 2.0 ** 127 or not torch.isfinite(rows[:, h]).all():       # fp16 rows may hold an infinity
+                assert torch.isnan(sc[h])
+                continue
+            assert sc[h] == want
+            moved = c[h] * (old / want)                         # e4m3: a product in fp32; int8: exact until its one rounding
+            held = c[h] if want == old else ref.round_code(moved if fmt == INT8 else moved.float().double(), fmt)
+            assert torch.equal(got[h, :3], held) and torch.equal(got[h, 3:5], ref.round_code(rows[:, h].double() / want, fmt))
+
+
 def test_cache_write_read_refusals(dev):
     pool = _pool(dev, 4, 2, 16, 64, E4M3)
     x, slots = torch.zeros(3, 2, 64, device=dev), torch.arange(3, device=dev)
