@@ -445,7 +445,9 @@ int ckv_block_tables(const ckv_table_step* step, ckv_stream_t stream);
  * (pairs (x[i], x[i + rotary_dim / 2]), or (x[2i], x[2i + 1]) when interleaved), cosine and
  * sine times factor; dimensions past rotary_dim pass through.  inverse: by the negative angle
  * (the gradient).  Angles are reduced in 64 bits.  k may be NULL with k_heads 0; out_q / out_k
- * may be q / k themselves, and may not overlap them otherwise.  Strides in elements. */
+ * may be q / k themselves, and may not overlap them otherwise.  Strides in elements.  Here and in
+ * the calls below, rows that are written may not share memory: of their strides each is at least
+ * the extent of the smaller ones. */
 typedef struct ckv_rotary_args {
   const void* q;
   int64_t q_tok_stride, q_head_stride;

@@ -7,6 +7,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <mutex>
 #include <string>
@@ -869,6 +870,24 @@ static bool aligned_to(size_t n, std::initializer_list<const void*> ps) {
     if ((uintptr_t)p % n) return false;
   return true;
 }
+// Whether no two rows of `width` share memory: sizes and strides of the dimensions that number
+// them, each stride at least the extent of the smaller ones.
+struct Dim {
+  int64_t size, stride;
+};
+static bool rows_apart(int64_t width, std::initializer_list<Dim> dims) {
+  Dim d[3];
+  int n = 0;
+  for (Dim x : dims)
+    if (x.size > 1) d[n++] = {x.size, x.stride < 0 ? -x.stride : x.stride};
+  std::sort(d, d + n, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+  int64_t extent = width;
+  for (int i = 0; i < n; ++i) {
+    if (d[i].stride < extent) return false;
+    extent += (d[i].size - 1) * d[i].stride;
+  }
+  return true;
+}
 static bool known_dtype(int dtype) { return dtype == CKV_BF16 || dtype == CKV_FP16 || dtype == CKV_FP32; }
 
 static int check_cache(const ckv_cache* c) {
@@ -918,6 +937,10 @@ int ckv_rotary(const ckv_rotary_args* a, ckv_stream_t stream) {
     return fail(CKV_ERR_ARG, "null argument");
   if (!aligned_to(8, {a->positions, a->inv_freq}) || !aligned_to(a->dtype == CKV_FP32 ? 4 : 2, {a->q, a->k, a->out_q, a->out_k}))
     return fail(CKV_ERR_ARG, "pointers must be aligned to their elements");
+  if (!rows_apart(a->head_dim, {{a->tokens, a->out_q_tok_stride}, {a->q_heads, a->out_q_head_stride}}) ||
+      (a->k_heads > 0 && (a->out_k == a->out_q ||
+                          !rows_apart(a->head_dim, {{a->tokens, a->out_k_tok_stride}, {a->k_heads, a->out_k_head_stride}}))))
+    return fail(CKV_ERR_ARG, "output rows overlap");
   const cudaError_t e = launch_rotary(*a, (cudaStream_t)stream);
   return e == cudaSuccess ? CKV_OK : cuda_fail(e, "rotary");
 }
@@ -944,6 +967,11 @@ int ckv_cache_write(const ckv_cache* cache, const void* k, int64_t k_tok_stride,
   const int rc = cache_rows(cache, const_cast<void*>(k), k_tok_stride, k_head_stride, const_cast<void*>(v), v_tok_stride,
                             v_head_stride, dtype, slots, tokens, &r);
   if (rc || tokens == 0) return rc;
+  const ckv_cache& c = *cache;
+  if (c.k == c.v || c.k_scale == c.v_scale ||
+      !rows_apart(c.head_dim, {{c.num_blocks, c.k_block_stride}, {c.num_kv_heads, c.k_head_stride}, {c.block_size, c.k_tok_stride}}) ||
+      !rows_apart(c.head_dim, {{c.num_blocks, c.v_block_stride}, {c.num_kv_heads, c.v_head_stride}, {c.block_size, c.v_tok_stride}}))
+    return fail(CKV_ERR_ARG, "cache rows overlap");
   const cudaError_t e = launch_cache_write(*cache, r, (cudaStream_t)stream);
   return e == cudaSuccess ? CKV_OK : cuda_fail(e, "cache write");
 }
@@ -995,6 +1023,8 @@ int ckv_cache_attention(const ckv_cache* cache, const ckv_attention_args* a, voi
   if (a->requests == 0 || a->tokens == 0) return CKV_OK;
   if (!a->q || !a->out || !a->tables || !a->lens) return fail(CKV_ERR_ARG, "null argument");
   if (!aligned_to(4, {a->tables, a->lens, a->cu, a->lse})) return fail(CKV_ERR_ARG, "pointers must be aligned to their elements");
+  if (!rows_apart(cache->head_dim, {{a->tokens, a->out_tok_stride}, {a->q_heads, a->out_head_stride}}))
+    return fail(CKV_ERR_ARG, "output rows overlap");
   const cudaError_t e = launch_cache_attention(*cache, *a, workspace, (cudaStream_t)stream);
   return e == cudaSuccess ? CKV_OK : cuda_fail(e, "cache attention");
 }

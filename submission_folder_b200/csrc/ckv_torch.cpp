@@ -126,6 +126,7 @@ CKV_FN(rotary) {
       !fits(2 * freq->numel()))
     return none();
   Tensor qo, ko;
+  if (a[7] == Py_None && a[8] != Py_None) return none();
   if (a[7] == Py_None) {
     qo = at::empty({T, H, D}, q->options());
     if (has_k) ko = at::empty({T, Hk, D}, q->options());

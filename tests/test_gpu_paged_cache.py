@@ -1139,6 +1139,24 @@ def test_refused_requests_attend_to_nothing(dev, captured):
         del graph
 
 
+def test_rows_that_overlap_are_refused(dev):
+    pool = _pool(dev, 4, 2, 16, 64, E4M3)
+    x, slots = torch.ones(3, 2, 64, device=dev), torch.arange(3, device=dev)
+    f, _ = rotary_frequencies(64, device=dev)
+    t, n = torch.zeros(3, 1, dtype=torch.int32, device=dev), torch.ones(3, dtype=torch.int32, device=dev)
+    same = torch.empty(1, 2, 64, device=dev).expand(3, 2, 64)
+    flat = pool[0].view(torch.uint8)[:1].expand(4, 2, 16, 64).view(E4M3)
+    for call in (lambda: ops.rotary(x, None, slots, f, out=(same, None)), lambda: ops.rotary(x, x, slots, f, out=(x.clone(), same)),
+                 lambda: ops.cache_write(x, x, flat, *pool[1:], slots), lambda: ops.cache_write(x, x, pool[0], *pool[:1], *pool[2:], slots),
+                 lambda: ops.cache_attention(x, *pool, t, n, out=same)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            call()
+    with pytest.raises(ValueError, match="out"):
+        ops.rotary(x, x, slots, f, out=(None, x.clone()))
+    ops.cache_read(flat, flat, *pool[2:], slots)               # reading them is fine
+    ops.rotary(same, same, slots, f)
+
+
 def test_paged_cache_class_refusals(dev):
     c = PagedKVCache(1, 8, 2, 64, 2, 64, 16, device=dev)
     z = torch.zeros(1, 2, 20, 64, dtype=torch.bfloat16, device=dev)

@@ -205,3 +205,28 @@ def test_rope_scaling_keys_that_would_be_lost_are_refused():
             rotary_frequencies(64, scaling={**yarn, **bad})
     same = rotary_frequencies(64, scaling={**yarn, "rope_theta": 10000, "finetuned": True, "mrope_section": [16, 24, 24], "partial_rotary_factor": 0.5, "beta_fast": None})
     assert torch.equal(same[0], rotary_frequencies(64, scaling=yarn)[0])
+
+
+def test_rows_that_overlap_are_refused():
+    """Written rows that share memory: a race on the device."""
+    lib = _lib.load()
+    write = lambda **o: lib.ckv_cache_write(ctypes.byref(_cache(k=P, v=2 * P, k_scale=3 * P, v_scale=4 * P, **o)), P, 256, 128, P,  # noqa: E731
+                                            256, 128, 0, P, 3, None)
+    for over in (dict(k_block_stride=0), dict(v_block_stride=0), dict(v_head_stride=0), dict(k_tok_stride=0), dict(k_tok_stride=64),
+                 dict(k_block_stride=2048), dict(v_tok_stride=256, v_head_stride=128, v_block_stride=2048)):
+        assert write(**over) == -1 and b"overlap" in lib.ckv_last_error_string(), over
+    for same in (dict(v=P), dict(v_scale=3 * P)):
+        c = _cache(**{**dict(k=P, v=2 * P, k_scale=3 * P, v_scale=4 * P), **same})
+        assert lib.ckv_cache_write(ctypes.byref(c), P, 256, 128, P, 256, 128, 0, P, 3, None) == -1
+    a = dict(q=P, q_tok_stride=1024, q_head_stride=128, out=P, out_tok_stride=1024, out_head_stride=128, tables=P, table_stride=4,
+             table_width=4, lens=P, requests=3, tokens=3, max_q=1, q_heads=8, scale=1.0)
+    for over in (dict(out_tok_stride=0), dict(out_head_stride=0), dict(out_tok_stride=128), dict(out_head_stride=64)):
+        s = _lib.AttentionArgs(**{**a, **over})
+        assert lib.ckv_cache_attention(ctypes.byref(_cache()), ctypes.byref(s), P, 1 << 40, None) == -1
+        assert b"overlap" in lib.ckv_last_error_string(), over
+    a = dict(q=P, q_tok_stride=128, q_head_stride=64, out_q=P, out_q_tok_stride=128, out_q_head_stride=64, positions=P, inv_freq=P, k=P,
+             k_tok_stride=64, k_head_stride=64, out_k=2 * P, out_k_tok_stride=64, out_k_head_stride=64, factor=1.0, tokens=2, q_heads=2,
+             k_heads=1, head_dim=64, rotary_dim=64, dtype=0)
+    for over in (dict(out_q_tok_stride=0), dict(out_q_head_stride=32), dict(out_k_tok_stride=32), dict(out_k=P)):
+        s = _lib.RotaryArgs(**{**a, **over})
+        assert lib.ckv_rotary(ctypes.byref(s), None) == -1 and b"overlap" in lib.ckv_last_error_string(), over
