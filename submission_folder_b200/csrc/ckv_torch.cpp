@@ -33,7 +33,11 @@ bool vec(const Tensor* t, int device, at::ScalarType type, int64_t n) {
 bool rows(const Tensor* t, int device) {
   return on(t, device) && t->dim() == 3 && (t->stride(2) == 1 || t->size(2) == 1) && dtype_code(t->scalar_type()) >= 0;
 }
-bool grad(const Tensor* t) { return t && t->requires_grad() && at::GradMode::is_enabled(); }
+// Whether autograd, of either mode, would follow this tensor.
+bool grad(const Tensor* t) {
+  return t && ((t->requires_grad() && at::GradMode::is_enabled()) ||
+               (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t->_fw_grad(0).defined()));
+}
 bool table(const Tensor* t, int device) {
   return on(t, device) && t->scalar_type() == at::kInt && t->dim() == 2 && t->stride(1) == 1;
 }

@@ -431,8 +431,9 @@ def _need_vector(t: torch.Tensor, dtype: torch.dtype, n: int, what: str) -> None
 def _need_rows(t: torch.Tensor, what: str) -> None:
     _need(t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1), f"{what} must be [tokens, heads, head_dim] with contiguous head_dim")
     _need(t.dtype in _DT, f"{what} must be bf16, fp16 or fp32, got {t.dtype}", TypeError)
-    _need(not (t.requires_grad and torch.is_grad_enabled()), f"{what} requires grad, but the paged cache's calls record no "
-          "autograd graph; call them on detached tensors", RuntimeError)
+    follows = (t.requires_grad and torch.is_grad_enabled()) or torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+    _need(not follows, f"{what} requires grad, but the paged cache's calls record no autograd graph and carry no tangents; "
+          "call them on detached tensors", RuntimeError)
 
 
 def _need_tables(t: torch.Tensor, requests: int) -> None:

@@ -1157,6 +1157,23 @@ def test_rows_that_overlap_are_refused(dev):
     ops.rotary(same, same, slots, f)
 
 
+def test_tangents_are_refused(dev):
+    """Forward-mode derivatives would be dropped quietly."""
+    import torch.autograd.forward_ad as fw
+    pool = _pool(dev, 4, 2, 16, 64, E4M3)
+    x, slots = torch.ones(3, 2, 64, device=dev), torch.arange(3, device=dev)
+    f, _ = rotary_frequencies(64, device=dev)
+    t, n = torch.zeros(3, 1, dtype=torch.int32, device=dev), torch.ones(3, dtype=torch.int32, device=dev)
+    with fw.dual_level():
+        d = fw.make_dual(x, x)
+        for call in (lambda y: ops.rotary(y, None, slots, f), lambda y: ops.rotary(x, y, slots, f),
+                     lambda y: ops.cache_write(y, x, *pool, slots), lambda y: ops.cache_write(x, y, *pool, slots),
+                     lambda y: ops.cache_attention(y, *pool, t, n), lambda y: ops.cache_attention(x, *pool, t, n, out=y)):
+            with pytest.raises(RuntimeError, match="tangents"):
+                call(d)
+            call(d.detach().clone())
+
+
 def test_paged_cache_class_refusals(dev):
     c = PagedKVCache(1, 8, 2, 64, 2, 64, 16, device=dev)
     z = torch.zeros(1, 2, 20, 64, dtype=torch.bfloat16, device=dev)
