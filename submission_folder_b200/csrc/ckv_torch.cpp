@@ -38,6 +38,10 @@ bool grad(const Tensor* t) {
   return t && ((t->requires_grad() && at::GradMode::is_enabled()) ||
                (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t->_fw_grad(0).defined()));
 }
+// Tells autograd that the tensor's values have changed.
+void wrote(const Tensor* t) {
+  if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
 bool table(const Tensor* t, int device) {
   return on(t, device) && t->scalar_type() == at::kInt && t->dim() == 2 && t->stride(1) == 1;
 }
@@ -107,6 +111,7 @@ CKV_FN(block_tables) {
                             ptr<int32_t>(&granted), work.defined() ? ptr<int32_t>(&work) : nullptr, ptr<int32_t>(&seen)};
   const int rc = call(dev, [&](ckv_stream_t st) { return ckv_block_tables(&s, st); });
   if (rc) return status(rc);
+  for (const Tensor* t : {lens_out, count_out, tables, list}) wrote(t);
   return Py_BuildValue("(NNNNNNN)", THPVariable_Wrap(*lens_out), THPVariable_Wrap(*count_out), THPVariable_Wrap(cu),
                        THPVariable_Wrap(slots), THPVariable_Wrap(positions), THPVariable_Wrap(granted), THPVariable_Wrap(seen));
   END_HANDLE_TH_ERRORS
@@ -156,6 +161,8 @@ CKV_FN(rotary) {
   r.dtype = dtype_code(q->scalar_type()); r.interleaved = inter; r.inverse = inverse;
   const int rc = call(dev, [&](ckv_stream_t st) { return ckv_rotary(&r, st); });
   if (rc) return status(rc);
+  if (a[7] != Py_None) wrote(&qo);
+  if (a[8] != Py_None) wrote(&ko);
   if (has_k) return Py_BuildValue("(NN)", THPVariable_Wrap(qo), THPVariable_Wrap(ko));
   return Py_BuildValue("(NO)", THPVariable_Wrap(qo), Py_None);
   END_HANDLE_TH_ERRORS
@@ -179,6 +186,7 @@ CKV_FN(cache_write) {
                            dtype_code(k->scalar_type()), ptr<int64_t>(slots), (int32_t)k->size(0), st);
   });
   if (rc) return status(rc);
+  for (int i = 2; i < 6; ++i) wrote(tensor(a[i]));
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
@@ -257,6 +265,7 @@ CKV_FN(cache_attention) {
   r.dtype = dtype_code(q->scalar_type());
   rc = call(dev, [&](ckv_stream_t st) { return ckv_cache_attention(&c, &r, ws.data_ptr(), bytes, st); });
   if (rc) return status(rc);
+  if (a[12] != Py_None) wrote(&out);
   if (want_lse) return Py_BuildValue("(NN)", THPVariable_Wrap(out), THPVariable_Wrap(lse));
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS

@@ -1174,6 +1174,37 @@ def test_tangents_are_refused(dev):
             call(d.detach().clone())
 
 
+def test_written_tensors_change_their_version(dev):
+    """Autograd sees that a saved tensor was overwritten; what is only read keeps its version."""
+    i32 = dict(dtype=torch.int32, device=dev)
+    pool = _pool(dev, 4, 2, 16, 64, E4M3)
+    x, slots = torch.ones(3, 2, 64, device=dev), torch.arange(3, device=dev)
+    f, _ = rotary_frequencies(64, device=dev)
+    a = [torch.zeros(3, **i32), torch.ones(3, **i32), torch.zeros(3, 2, **i32), torch.arange(4, **i32), torch.tensor([4], **i32)]
+    out = torch.empty_like(x), torch.empty_like(x)
+
+    def changed(ts, call):
+        before = [t._version for t in ts]
+        call()
+        return [t._version > b for t, b in zip(ts, before)]
+
+    assert changed(a, lambda: ops.block_tables(*a, 16, 3)) == [True, False, True, True, True]
+    apart = torch.empty(3, **i32), torch.empty(1, **i32)
+    assert changed([a[0], a[4], *apart], lambda: ops.block_tables(*a, 16, 3, lens_out=apart[0], free_count_out=apart[1])) == [False, False, True, True]
+    assert changed([x, *out], lambda: ops.rotary(x, x.clone(), slots, f, out=out)) == [False, True, True]
+    assert changed([x, *pool], lambda: ops.cache_write(x, x, *pool, slots)) == [False] + [True] * 4
+    assert changed(pool, lambda: ops.cache_read(*pool, slots)) == [False] * 4
+    assert changed([x, out[0], *pool], lambda: ops.cache_attention(x, *pool, a[2], a[1], out=out[0])) == [False, True] + [False] * 4
+    w = torch.ones(3, 2, 64, device=dev, requires_grad=True)
+    y = w * out[0]
+    ops.cache_attention(x, *pool, a[2], a[1], out=out[0])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        z = torch.empty_like(x)
+    ops.cache_attention(x, *pool, a[2], a[1], out=z)          # tensors of inference mode have no version
+
+
 def test_paged_cache_class_refusals(dev):
     c = PagedKVCache(1, 8, 2, 64, 2, 64, 16, device=dev)
     z = torch.zeros(1, 2, 20, 64, dtype=torch.bfloat16, device=dev)
