@@ -200,6 +200,8 @@ class PagedKVCache:
             rows.append((k[0, ::groups].transpose(0, 1), v[0, ::groups].transpose(0, 1)))
         if seen < kept:
             raise ValueError("seen counts the kept tokens too")
+        for i, (k, v) in enumerate(rows):      # what ``write`` would refuse, before any block is taken
+            ops.check_rows(k, v, *self.layer(i))
         new = torch.zeros_like(self.lens)
         new[request] = kept
         step = self.step(new, total=kept, max_q=kept)

@@ -459,6 +459,20 @@ def _need_cache(k_cache, v_cache, k_scale, v_scale) -> Tuple[int, int]:
     return k_cache.shape[1], k_cache.shape[3]
 
 
+def check_rows(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+               v_scale: torch.Tensor) -> None:
+    """Raises for rows ``k``, ``v`` and a cache that ``cache_write`` would refuse."""
+    _one_device(k, v, k_cache, v_cache, k_scale, v_scale)
+    _need_rows(k, "k")
+    _need_rows(v, "v")
+    _need(v.dtype == k.dtype and v.shape == k.shape, "k and v must agree in dtype and shape")
+    H, D = _need_cache(k_cache, v_cache, k_scale, v_scale)
+    _need(tuple(k.shape[1:]) == (H, D), f"k and v must be [tokens, {H}, {D}]")
+    for t in (k, v):
+        _need(not any(x * t.element_size() % 16 for x in (t.stride(0), t.stride(1))) and t.data_ptr() % 16 == 0,
+              "rows must start on 16 bytes")
+
+
 def _failed(name: str, rc) -> None:
     """Raises for what ckv_torch.cpp returned in place of a result."""
     if type(rc) is int:

@@ -1205,6 +1205,22 @@ def test_written_tensors_change_their_version(dev):
     ops.cache_attention(x, *pool, a[2], a[1], out=z)          # tensors of inference mode have no version
 
 
+def test_a_refused_prompt_takes_nothing(dev):
+    """Layers that cannot be written are refused before any block is taken: the cache is as it was."""
+    c = PagedKVCache(2, 8, 2, 64, 2, 64, 16, device=dev)
+    z = torch.zeros(1, 2, 20, 64, dtype=torch.bfloat16, device=dev)
+    c.admit(1, [(z, z)] * 2, 30)
+    state = [t.clone() for t in (c.lens, c.tables, c.free_list, c.free_count, c.shift)]
+    odd = torch.zeros(1, 2, 20, 65, dtype=torch.bfloat16, device=dev)[..., 1:]
+    for bad, err in [(z.double(), TypeError), (z.cpu(), RuntimeError), (torch.cat([z, z], -1), ValueError),
+                     (z.clone().requires_grad_(), RuntimeError), (odd, ValueError), (z.transpose(2, 3).contiguous().transpose(2, 3), ValueError)]:
+        for layers in ([(bad, bad)] * 2, [(z, z), (bad, bad)], [(z, z), (z, bad)]):
+            with pytest.raises((err, ValueError)):
+                c.admit(0, layers, 40)
+            assert all(torch.equal(a, b) for a, b in zip(state, (c.lens, c.tables, c.free_list, c.free_count, c.shift)))
+    assert c.admit(0, [(z, z)] * 2, 40).tables.granted.tolist() == [20, 0]
+
+
 def test_paged_cache_class_refusals(dev):
     c = PagedKVCache(1, 8, 2, 64, 2, 64, 16, device=dev)
     z = torch.zeros(1, 2, 20, 64, dtype=torch.bfloat16, device=dev)
