@@ -186,7 +186,8 @@ class PagedKVCache:
         """Put a prompt into the free row ``request``: ``layers`` are each layer's ``(key_states,
         value_states)`` ``[1, heads, B, D]`` as ``CircuitKVCluster.update_kv`` returns them (each KV head
         once, or in the repeat_kv layout), with the same B in every layer; ``seen``: the prompt's
-        length, so that the next token stands at position ``seen``."""
+        length, so that the next token stands at position ``seen``.  A row that is not free, or has no room,
+        gets nothing (``step.tables.granted``)."""
         if len(layers) != len(self):
             raise ValueError(f"expected {len(self)} layers, got {len(layers)}")
         kept = layers[0][0].shape[-2]
@@ -203,9 +204,10 @@ class PagedKVCache:
         for i, (k, v) in enumerate(rows):      # what ``write`` would refuse, before any block is taken
             ops.check_rows(k, v, *self.layer(i))
         new = torch.zeros_like(self.lens)
-        new[request] = kept
+        free = self.lens[request] == 0
+        new[request] = torch.where(free, kept, 0)
         step = self.step(new, total=kept, max_q=kept)
-        self.shift[request] = torch.where(step.tables.granted[request] == kept, seen - kept, self.shift[request])
+        self.shift[request] = torch.where(free & (step.tables.granted[request] == kept), seen - kept, self.shift[request])
         for i, (k, v) in enumerate(rows):
             self.write(i, k, v, step)
         return step

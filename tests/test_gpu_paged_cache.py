@@ -1221,6 +1221,20 @@ def test_a_refused_prompt_takes_nothing(dev):
     assert c.admit(0, [(z, z)] * 2, 40).tables.granted.tolist() == [20, 0]
 
 
+def test_admission_to_a_busy_row_changes_nothing(dev):
+    """A prompt for a row that holds a request: the request keeps its tokens, blocks and positions."""
+    c = PagedKVCache(1, 8, 2, 64, 2, 64, 16, device=dev)
+    z = [torch.randn(1, 2, n, 64, generator=torch.Generator().manual_seed(n)).bfloat16().to(dev) for n in (20, 7, 0)]
+    c.admit(0, [(z[0], z[0])], 500)
+    held = [t.clone() for t in (c.lens, c.tables, c.free_list, c.free_count, c.shift, c.k.view(torch.uint8), c.k_scale)]
+    for x in z[1:]:
+        step = c.admit(0, [(x, x)], 90)
+        assert int(step.tables.granted[0]) == 0 and step.tables.slots.tolist() == [-1] * x.shape[2]
+        now = (c.lens, c.tables, c.free_list, c.free_count, c.shift, c.k.view(torch.uint8), c.k_scale)
+        assert all(torch.equal(a, b) for a, b in zip(held, now))
+    assert c.step(torch.tensor([1, 0], dtype=torch.int32, device=dev)).tables.positions.tolist() == [500, 0]
+
+
 def test_paged_cache_class_refusals(dev):
     c = PagedKVCache(1, 8, 2, 64, 2, 64, 16, device=dev)
     z = torch.zeros(1, 2, 20, 64, dtype=torch.bfloat16, device=dev)
