@@ -3,6 +3,7 @@ frequencies, and the refusal to run on host tensors."""
 
 import ctypes
 import math
+import subprocess
 
 import pytest
 import torch
@@ -230,3 +231,19 @@ def test_rows_that_overlap_are_refused():
     for over in (dict(out_q_tok_stride=0), dict(out_q_head_stride=32), dict(out_k_tok_stride=32), dict(out_k=P)):
         s = _lib.RotaryArgs(**{**a, **over})
         assert lib.ckv_rotary(ctypes.byref(s), None) == -1 and b"overlap" in lib.ckv_last_error_string(), over
+
+
+def test_the_library_builds_without_torch(monkeypatch):
+    """libckv.so and the C ABI need neither Python's headers nor torch's: plain make does not ask for them, and the
+    build goes on without the module that does."""
+    from submission_folder_b200 import build as b
+    dry = subprocess.run(["make", "-n", "-B", "-C", b.CSRC, "PYTHON=false"], capture_output=True, text=True, check=True).stdout
+    assert "libckv.so" in dry and "ckv_torch" not in dry
+    assert "ckv_torch.cpp" in subprocess.run(["make", "-n", "-B", "-C", b.CSRC, "torch"], capture_output=True, text=True, check=True).stdout
+    assert b.torch_headers()
+    calls = []
+    monkeypatch.setattr(b, "_make", lambda target, verbose: calls.append(target))
+    assert b.build().endswith("libckv.so") and calls == ["../libckv.so", "torch"]
+    calls.clear()
+    monkeypatch.setattr(b.sysconfig, "get_paths", lambda: {"include": "/nonexistent"})
+    assert b.build().endswith("libckv.so") and calls == ["../libckv.so"]
