@@ -6,6 +6,7 @@
 // Every function returns its result, or None when an argument is not what the call takes (ops.py
 // then says which), or the C ABI's negative status as an int.
 #include <Python.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -18,6 +19,11 @@
 namespace {
 
 using at::Tensor;
+
+// A new tensor on a device, not filled.
+Tensor fresh_tensor(at::IntArrayRef size, at::ScalarType type, at::Device device) {
+  return Tensor(at::detail::empty_cuda(size, type, device, std::nullopt));
+}
 
 // The tensor behind a Python argument, or null.
 const Tensor* tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
@@ -98,11 +104,11 @@ CKV_FN(block_tables) {
       !table(tables, dev) || tables->size(0) != R || (a[7] != Py_None && !vec(shift, dev, at::kInt, R)) || !fits(total) ||
       !fits(block) || !fits(R) || !fits(tables->size(1)) || !fits(list->numel()))
     return none();
-  const auto i32 = lens->options(), i64 = i32.dtype(at::kLong);
-  Tensor cu = at::empty({R + 1}, i32), granted = at::empty({R}, i32), seen = at::empty({R}, i32);
-  Tensor slots = at::empty({total}, i64), positions = at::empty({total}, i64);
+  const at::Device at = lens->device();
+  Tensor cu = fresh_tensor({R + 1}, at::kInt, at), granted = fresh_tensor({R}, at::kInt, at), seen = fresh_tensor({R}, at::kInt, at);
+  Tensor slots = fresh_tensor({total}, at::kLong, at), positions = fresh_tensor({total}, at::kLong, at);
   Tensor work;
-  if (R + total > CKV_TABLES_SMALL) work = at::empty({3 * R + 4}, i32);
+  if (R + total > CKV_TABLES_SMALL) work = fresh_tensor({3 * R + 4}, at::kInt, at);
   const int64_t width = tables->size(1);
   const ckv_table_step s = {ptr<int32_t>(lens), ptr<int32_t>(fresh), ptr<int32_t>(shift), ptr<int32_t>(tables),
                             table_stride(tables), (int32_t)width, ptr<int32_t>(list), (int32_t)list->numel(),
@@ -137,8 +143,8 @@ CKV_FN(rotary) {
   Tensor qo, ko;
   if (a[7] == Py_None && a[8] != Py_None) return none();
   if (a[7] == Py_None) {
-    qo = at::empty({T, H, D}, q->options());
-    if (has_k) ko = at::empty({T, Hk, D}, q->options());
+    qo = fresh_tensor({T, H, D}, q->scalar_type(), q->device());
+    if (has_k) ko = fresh_tensor({T, Hk, D}, q->scalar_type(), q->device());
   } else {
     const Tensor *x = tensor(a[7]), *y = a[8] == Py_None ? nullptr : tensor(a[8]);
     if (!rows(x, dev) || x->sizes() != q->sizes() || x->scalar_type() != q->scalar_type() || grad(x)) return none();
@@ -203,8 +209,8 @@ CKV_FN(cache_read) {
   if (dtype_code(type) < 0 || !vec(slots, dev, at::kLong, slots->numel()) || !fits(slots->numel()) ||
       !cache_of(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), dev, &c))
     return none();
-  const auto opts = slots->options().dtype(type);
-  Tensor k = at::empty({slots->numel(), c.num_kv_heads, c.head_dim}, opts), v = at::empty_like(k);
+  const int64_t shape[] = {slots->numel(), c.num_kv_heads, c.head_dim};
+  Tensor k = fresh_tensor(shape, type, slots->device()), v = fresh_tensor(shape, type, slots->device());
   const int rc = call(dev, [&](ckv_stream_t st) {
     return ckv_cache_read(&c, k.data_ptr(), v.data_ptr(), dtype_code(type), ptr<int64_t>(slots), (int32_t)slots->numel(), st);
   });
@@ -239,7 +245,7 @@ CKV_FN(cache_attention) {
   if (max_q > INT32_MAX || max_q < INT32_MIN) return none();
   Tensor out;
   if (a[12] == Py_None) {
-    out = at::empty({T, H, D}, q->options());
+    out = fresh_tensor({T, H, D}, q->scalar_type(), q->device());
   } else {
     const Tensor* o = tensor(a[12]);
     if (!rows(o, dev) || o->sizes() != q->sizes() || o->scalar_type() != q->scalar_type() || grad(o)) return none();
@@ -249,9 +255,9 @@ CKV_FN(cache_attention) {
   int rc = ckv_cache_attention_workspace((int32_t)D, (int32_t)max_q, (int32_t)H, c.num_kv_heads, &bytes);
   if (rc) return status(rc);
   Tensor lse;
-  if (want_lse) lse = at::empty({T, H}, q->options().dtype(at::kFloat));
+  if (want_lse) lse = fresh_tensor({T, H}, at::kFloat, q->device());
   // from the allocator for each call: two streams, or two captured graphs, never share it
-  Tensor ws = at::empty({(int64_t)bytes}, q->options().dtype(at::kByte));
+  Tensor ws = fresh_tensor({(int64_t)bytes}, at::kByte, q->device());
   ckv_attention_args r = {};
   r.q = q->data_ptr(); r.q_tok_stride = q->stride(0); r.q_head_stride = q->stride(1);
   r.out = out.data_ptr(); r.out_tok_stride = out.stride(0); r.out_head_stride = out.stride(1);
