@@ -501,7 +501,7 @@ typedef struct ckv_attention_args {
   const int32_t* lens;
   const int32_t* cu;
   int32_t requests, tokens;
-  int32_t max_q;               /* at least the most query tokens of a sequence; the rows of one with more are NaN */
+  int32_t max_q;               /* at least the most query tokens of a sequence; the rows of one with more are NaN (0 if it is empty) */
   int32_t q_heads;
   int32_t causal;
   float scale;

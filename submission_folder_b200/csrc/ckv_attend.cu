@@ -898,8 +898,8 @@ __global__ void __launch_bounds__(att_warps(D, NT, kTerms) * 32, 1) k_attend(con
   for (int r = cta; r < R; r += gridDim.x) {
     int q0, rows;
     seq_rows(p, r, q0, rows);
-    const bool many = rows > p.a.max_q;
-    if (!many && seq_len(p, r) != 0) continue;
+    const bool empty = seq_len(p, r) == 0, many = !empty && rows > p.a.max_q;
+    if (!empty && !many) continue;
     const int hq = p.c.num_kv_heads * p.group;
     const float x = many ? __uint_as_float(0x7fffffffu) : 0.f;
     for (int tok = q0; tok < q0 + rows; ++tok)

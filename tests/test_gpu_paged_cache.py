@@ -747,13 +747,14 @@ def test_attention_nan_values_that_nobody_sees(dev):
 def test_attention_of_more_rows_than_max_q_is_nan(dev, dtype):
     """The rows of a sequence with more query tokens than the call allows for are marked, all of them; the
     other sequences are right and the padding is left alone."""
-    lens, queries = [100, 40, 0, 70], [2, 5, 3, 1]
+    lens, queries = [100, 40, 0, 70], [2, 5, 3, 1]      # the third sees nothing, however many rows it has
     pool, tables, n, q, k, v = _attention_case(dev, lens, 2, 4, 128, 16, E4M3, dtype, queries)
     q = torch.cat([q, q[:2]])
     cu = torch.tensor([0] + queries, device=dev).cumsum(0).int()
     out = torch.full_like(q, 7.0)
     got, lse = ops.cache_attention(q, *pool, tables, n, cu=cu, max_q=2, want_lse=True, out=out)
-    assert torch.isnan(got[2:10]).all() and torch.isnan(lse[2:10]).all()
+    assert torch.isnan(got[2:7]).all() and torch.isnan(lse[2:7]).all()
+    assert not got[7:10].any() and torch.all(lse[7:10] == -math.inf)
     # the others by the header's bounds (a larger max_q cuts the line of work elsewhere, so that sums in fp32
     # come in another order: no other call gives the same bits)
     _attention_check(got[:2], lse[:2], q[:2], k[:100], v[:100], [100], [2], 128 ** -0.5, True)
@@ -1233,6 +1234,15 @@ def test_admission_to_a_busy_row_changes_nothing(dev):
         now = (c.lens, c.tables, c.free_list, c.free_count, c.shift, c.k.view(torch.uint8), c.k_scale)
         assert all(torch.equal(a, b) for a, b in zip(held, now))
     assert c.step(torch.tensor([1, 0], dtype=torch.int32, device=dev)).tables.positions.tolist() == [500, 0]
+
+
+def test_a_refused_prompt_of_more_than_max_q_tokens(dev):
+    """Zeros, as for any request that did not fit, also where its rows are more than the step's ``max_q``."""
+    c = PagedKVCache(1, 4, 2, 64, 2, 64, 16, device=dev)
+    step = c.step(torch.tensor([1, 70], dtype=torch.int32, device=dev), total=9)
+    x = torch.ones(9, 2, 64, dtype=torch.bfloat16, device=dev)
+    out = c.decode(0, x, x, x, step)
+    assert step.tables.granted.tolist() == [1, 0] and torch.all(out[0] == 1) and not out[1:].any()
 
 
 def test_paged_cache_class_refusals(dev):
