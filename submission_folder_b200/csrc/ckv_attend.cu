@@ -33,10 +33,11 @@
 // there.  Pieces of one unit are merged in the CTA, then across CTAs by k_attend_merge in
 // a fixed order: no atomics, and the same bits every time.
 //
-// Bound: HBM (each code is read once) for large batches: 32 sequences of up to 32768 tokens, 8 of
-// 32 heads of 128 in bf16: 187 us, 6.1 TB/s.  One sequence of 131072 tokens: 50 us with one bf16 query
-// (5.4 TB/s), 57 us with four (two row tiles); 80 us with four fp32 queries, where the two terms'
-// products and their sums bound it.  One sequence of 512: 9.1 us, launches and the merges.
+// Bound (the kernels alone): HBM (each code is read once for 16 query rows of a KV head) for large
+// batches: 32 sequences of up to 32768 tokens, 8 of 32 heads of 128 in bf16: 190 us, 6.0 TB/s.  One
+// sequence of 131072 tokens: 51 us with one bf16 query (5.3 TB/s), 71 with four (two row tiles), 123 with
+// five (20 rows: two units, each reads and unpacks the codes); 84 us with four fp32 queries, where
+// the two terms' products and their sums bound it.  One sequence of 512: 8.1 us, launches and the merges.
 #include "ckv_cache.h"
 #include "ckv_common.cuh"
 

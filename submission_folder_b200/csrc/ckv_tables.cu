@@ -14,8 +14,10 @@
 // Bound: latency.  A small step is one CTA: scan, then stores, each token's request found by
 // binary search in shared memory.  Above CKV_TABLES_SMALL tokens and requests the stores go to a second
 // launch with CTAs for each request, which need no search but for blocks that came back in the
-// same step (1024 requests, 630,000 tokens: 126 us when a cluster of 8 CTAs searched for every
-// token, 17 us in two launches that did, 14 with CTAs by request).
+// same step (1024 requests, 602,000 tokens, kernels alone: 126 us when a cluster of 8 CTAs searched for
+// every token, 17 us in two launches that did, 12 with CTAs by request).  16 requests of 500, 2000, 4000 and
+// 8000 tokens in all: one CTA 3.5, 4.4, 5.9 and 9.0 us, two launches 4.3 to 4.4; 1000 requests of 1000 and 3000:
+// 5.0 and 7.1 against 6.0; 3000 of 1000: 10.2 against 11.7.
 #include <algorithm>
 
 #include "ckv_cache.h"

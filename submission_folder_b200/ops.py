@@ -603,7 +603,8 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     max_q: int = 1, scale: Optional[float] = None, causal: bool = True, want_lse: bool = False,
                     out: Optional[torch.Tensor] = None):
     """Attention of the new query tokens ``q`` ``[T, H, D]`` over a paged 8-bit cache
-    (``ckv_cache_attention``), reading each code once; meant for a few query tokens per sequence.
+    (``ckv_cache_attention``), reading each code once for every 16 query rows of its KV head (query tokens
+    times heads per KV head); meant for a few query tokens per sequence.
 
     Sequence ``r`` has query rows ``cu[r] .. cu[r + 1]`` (int32 ``[R + 1]``, at most ``max_q`` each: the
     rows of a sequence with more are NaN; None: one row each) and ``lens[r]`` cached tokens (int32 ``[R]``, the new ones included) in the
