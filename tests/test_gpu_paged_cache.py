@@ -781,6 +781,33 @@ def test_lse_of_padding_rows(dev, pad):
     assert torch.all(out[:2] == 1) and not out[2].any() and torch.isfinite(lse[:2]).all() and torch.all(lse[2] == -math.inf)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("bad", [slice(0, 1), slice(0, 3), slice(2, None, 2), slice(0, None)])
+def test_lse_beside_nan_values(dev, bad, sign, dtype):
+    """The log-sum-exp is the keys' alone: value scales of NaN in some or all blocks make the outputs NaN and
+    leave it as it is, for logits around 400 and around -400, in a short sequence and in one over many CTAs."""
+    lens = [16, 40, 3000]
+    pool, tables, n, q, k, v = _attention_case(dev, lens, 2, 2, 64, 16, INT8, dtype, [1] * 3)
+    kk = k.float()
+    kk[..., 0] = 8.0
+    slots = torch.cat([(tables[r].long()[:, None] * 16 + torch.arange(16, device=dev)).flatten()[:m] for r, m in enumerate(lens)])
+    ops.cache_write(kk, v.float(), *pool, slots)
+    k, v = (x.double() for x in ops.cache_read(*pool, slots, torch.float32))
+    q[..., 0] = 400.0
+    for r, m in enumerate(lens):
+        pool[3][tables[r, :-(-m // 16)][bad].long()] = math.nan
+    out, lse = ops.cache_attention(q, *pool, tables, n, scale=sign / 8, want_lse=True)
+    b = 0
+    for r, m in enumerate(lens):
+        _, wl = ref.attention(q[r:r + 1].double(), k[b:b + m], v[b:b + m], sign / 8, True)
+        mass = torch.einsum("mhd,nhd->mhn", q[r:r + 1].double().abs(), k[b:b + m].abs().repeat_interleave(2, 1)).amax(-1)
+        assert torch.all((lse[r:r + 1].double() - wl).abs() <= 2.0 ** -20 * (1 + mass / 8) + 2.0 ** -23 * wl.abs())
+        seen = tables[r, :-(-m // 16)][bad].numel() > 0
+        assert torch.isnan(out[r]).all() if seen else torch.isfinite(out[r]).all()
+        b += m
+
+
 def test_attention_lengths_that_do_not_fit(dev):
     """Lengths below zero count as zero, lengths past the table as the table's; ``cu`` past the rows
     or falling leaves rows out, without a fault."""
