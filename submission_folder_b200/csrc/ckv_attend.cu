@@ -16,10 +16,10 @@
 //
 // Precision: a query row is brought to [2^14, 2^15) by a power of two; a bf16 row is exact in fp16,
 // fp16 and fp32 rows take two fp16 terms, hi + lo (22 bits).  The weights, at most 2^15, take two terms
-// for every type: in one (11 bits) they put a bf16 output off by about 1.4e-4 before its own rounding, which flipped
-// the last bit of one output in forty.  The products of one step are summed apart and added in fp32
-// with rounding, because the tensor core's own sums truncate and a warp may take thousands of
-// steps.  (Second term and additions for bf16: 1 x 512 tokens 8.7 -> 8.0 us, on fewer warps; 16 ragged
+// for every type: in one (11 bits) they put a bf16 output off by about 1.4e-4 before its own
+// rounding, which flipped the last bit of one output in forty.  The products of one step are summed
+// apart and added in fp32 with rounding, because the tensor core's own sums truncate and a warp may
+// take thousands of steps.  (Second term and additions for bf16: 1 x 512 tokens 8.7 -> 8.0 us, on fewer warps; 16 ragged
 // sequences 20.5 -> 21.7; 32 of up to 32768 tokens 187 -> 192; 131072 tokens x 4 queries 57 -> 71.)
 //
 // The references m, m' only move when a logit passes them by more than 2^kSlack, so a step
@@ -36,7 +36,7 @@
 // Bound (the kernels alone): HBM (each code is read once for 16 query rows of a KV head) for large
 // batches: 32 sequences of up to 32768 tokens, 8 of 32 heads of 128 in bf16: 190 us, 6.0 TB/s.  One
 // sequence of 131072 tokens: 51 us with one bf16 query (5.3 TB/s), 71 with four (two row tiles), 123 with
-// five (20 rows: two units, each reads and unpacks the codes); 84 us with four fp32 queries, where
+// five (20 rows: two units, each reads and unpacks the codes); 83 us with four fp32 queries, where
 // the two terms' products and their sums bound it.  One sequence of 512: 8.1 us, launches and the merges.
 #include "ckv_cache.h"
 #include "ckv_common.cuh"
